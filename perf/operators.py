@@ -226,7 +226,7 @@ def _own(s):
         return nn.gated_scan_backward(s["dh"], s["x"], s["g"], s["h"], s["h0"], s["reset"], s["dh_last"])
     if op == "orth":
         return nn.orthogonalize(s["g"])
-    nn.muon_update(s["w"], s["g"], s["m"], lr=LR, momentum=MOMENTUM, weight_decay=DECAY)
+    nn.muon_update(s["w"], s["g"], s["m"], lr=LR, mu=MOMENTUM, weight_decay=DECAY)
     return s["w"], s["m"]
 
 
