@@ -273,6 +273,156 @@ pub struct phyzb_return_cfg {
     pub normalize: i32,
 }
 
+// ── recurrent-block operators ────────────────────────────────────────────
+
+pub const PHYZB_DT_F32: i32 = 0;
+pub const PHYZB_DT_BF16: i32 = 1;
+pub const PHYZB_DT_F16: i32 = 2;
+pub const PHYZB_ACT_NONE: i32 = 0;
+pub const PHYZB_ACT_RELU: i32 = 1;
+pub const PHYZB_ACT_TANH: i32 = 2;
+pub const PHYZB_ACT_SILU: i32 = 3;
+pub const PHYZB_ACT_GELU: i32 = 4;
+pub const PHYZB_MUON_MAX_SIDE: i32 = 16384;
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct phyzb_linear_args {
+    pub dtype: i32,
+    pub activation: i32,
+    pub device: i32,
+    pub m: i64,
+    pub k: i64,
+    pub n: i64,
+    pub x: *const c_void,
+    pub x_stride: [i64; 2],
+    pub w: *const c_void,
+    pub w_stride: [i64; 2],
+    pub bias: *const f32,
+    pub residual: *const c_void,
+    pub residual_stride: [i64; 2],
+    pub y: *mut c_void,
+    pub y_stride: [i64; 2],
+    pub pre: *mut c_void,
+    pub pre_stride: [i64; 2],
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct phyzb_linear_grad_args {
+    pub dtype: i32,
+    pub activation: i32,
+    pub device: i32,
+    pub m: i64,
+    pub k: i64,
+    pub n: i64,
+    pub dy: *const c_void,
+    pub dy_stride: [i64; 2],
+    pub pre: *const c_void,
+    pub pre_stride: [i64; 2],
+    pub x: *const c_void,
+    pub x_stride: [i64; 2],
+    pub w: *const c_void,
+    pub w_stride: [i64; 2],
+    pub dx: *mut c_void,
+    pub dx_stride: [i64; 2],
+    pub dw: *mut c_void,
+    pub dw_stride: [i64; 2],
+    pub dbias: *mut f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct phyzb_scan_args {
+    pub dtype: i32,
+    pub device: i32,
+    pub b: i64,
+    pub t: i64,
+    pub c: i64,
+    pub x: *const c_void,
+    pub x_stride: [i64; 3],
+    pub gate: *const c_void,
+    pub gate_stride: [i64; 3],
+    pub h0: *const f32,
+    pub h0_stride: [i64; 2],
+    pub reset: *const u8,
+    pub reset_stride: [i64; 3],
+    pub h: *mut c_void,
+    pub h_stride: [i64; 3],
+    pub h_last: *mut f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct phyzb_scan_grad_args {
+    pub dtype: i32,
+    pub device: i32,
+    pub b: i64,
+    pub t: i64,
+    pub c: i64,
+    pub dh: *const c_void,
+    pub dh_stride: [i64; 3],
+    pub x: *const c_void,
+    pub x_stride: [i64; 3],
+    pub gate: *const c_void,
+    pub gate_stride: [i64; 3],
+    pub h: *const c_void,
+    pub h_stride: [i64; 3],
+    pub h0: *const f32,
+    pub h0_stride: [i64; 2],
+    pub reset: *const u8,
+    pub reset_stride: [i64; 3],
+    pub dh_last: *const f32,
+    pub dh_last_stride: [i64; 2],
+    pub dx: *mut c_void,
+    pub dx_stride: [i64; 3],
+    pub dgate: *mut c_void,
+    pub dgate_stride: [i64; 3],
+    pub dh0: *mut f32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct phyzb_muon_args {
+    pub dtype: i32,
+    pub device: i32,
+    pub nesterov: i32,
+    pub steps: i32,
+    pub batch: i64,
+    pub rows: i64,
+    pub cols: i64,
+    pub grad: *const c_void,
+    pub grad_stride: [i64; 3],
+    pub momentum: *mut f32,
+    pub momentum_stride: [i64; 3],
+    pub weight: *mut f32,
+    pub weight_stride: [i64; 3],
+    pub copy_dtype: i32,
+    pub reserved: i32,
+    pub copy: *mut c_void,
+    pub copy_stride: [i64; 3],
+    pub lr: f64,
+    pub mu: f64,
+    pub weight_decay: f64,
+    pub scale: f64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct phyzb_orthogonalize_args {
+    pub dtype: i32,
+    pub device: i32,
+    pub steps: i32,
+    pub reserved: i32,
+    pub batch: i64,
+    pub rows: i64,
+    pub cols: i64,
+    pub x: *const c_void,
+    pub x_stride: [i64; 3],
+    pub out: *mut c_void,
+    pub out_stride: [i64; 3],
+}
+
 #[link(name = "phyzb200")]
 extern "C" {
     pub fn phyzb_last_error() -> *const c_char;
@@ -385,6 +535,26 @@ extern "C" {
     pub fn phyzb_reduce_objective_device(sim: *mut phyzb_sim, comm: *mut phyzb_comm, kind: c_int,
                                          out_device_scalar: *mut c_void) -> c_int;
     pub fn phyzb_comm_sync(comm: *mut phyzb_comm, sim: *mut phyzb_sim, timeout_s: f64) -> c_int;
+
+    // recurrent-block operators
+    pub fn phyzb_linear_workspace(a: *const phyzb_linear_args, bytes: *mut i64) -> c_int;
+    pub fn phyzb_linear(a: *const phyzb_linear_args, workspace: *mut c_void,
+                        workspace_bytes: i64, stream: *mut c_void) -> c_int;
+    pub fn phyzb_linear_grad_workspace(a: *const phyzb_linear_grad_args, bytes: *mut i64) -> c_int;
+    pub fn phyzb_linear_grad(a: *const phyzb_linear_grad_args, workspace: *mut c_void,
+                             workspace_bytes: i64, stream: *mut c_void) -> c_int;
+    pub fn phyzb_gated_scan_workspace(a: *const phyzb_scan_args, bytes: *mut i64) -> c_int;
+    pub fn phyzb_gated_scan(a: *const phyzb_scan_args, workspace: *mut c_void,
+                            workspace_bytes: i64, stream: *mut c_void) -> c_int;
+    pub fn phyzb_gated_scan_grad_workspace(a: *const phyzb_scan_grad_args, bytes: *mut i64) -> c_int;
+    pub fn phyzb_gated_scan_grad(a: *const phyzb_scan_grad_args, workspace: *mut c_void,
+                                 workspace_bytes: i64, stream: *mut c_void) -> c_int;
+    pub fn phyzb_muon_workspace(a: *const phyzb_muon_args, bytes: *mut i64) -> c_int;
+    pub fn phyzb_muon_update(a: *const phyzb_muon_args, workspace: *mut c_void,
+                             workspace_bytes: i64, stream: *mut c_void) -> c_int;
+    pub fn phyzb_orthogonalize_workspace(a: *const phyzb_orthogonalize_args, bytes: *mut i64) -> c_int;
+    pub fn phyzb_orthogonalize(a: *const phyzb_orthogonalize_args, workspace: *mut c_void,
+                               workspace_bytes: i64, stream: *mut c_void) -> c_int;
 
     // measurement and kernel selection
     pub fn phyzb_flops_per_world_step(sim: *const phyzb_sim, flops: *mut f64, transcendentals: *mut f64) -> c_int;

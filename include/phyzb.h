@@ -648,6 +648,180 @@ int phyzb_set_world_lanes(phyzb_sim* sim, int32_t lanes);
  * kernel with the current settings (plans and packs the split if needed). */
 int phyzb_get_world_lanes(phyzb_sim* sim, int32_t* lanes, int32_t* active);
 
+/* ── recurrent-block operators (no reference counterpart) ──────────────── */
+
+/* A policy or dynamics model with memory is a stack of these: a linear layer
+ * with its epilogue, a gated recurrence over the control steps of a rollout,
+ * and the Muon update of the layers' matrices. They work on caller-owned
+ * device memory, allocate nothing, keep nothing between calls and run on
+ * `stream` (a cudaStream_t, NULL = the default stream) of the current context
+ * of `device`, asynchronously. Strides count elements and may take any order;
+ * outputs must not overlap each other or the inputs, except where said.
+ * `workspace` is device memory of at least the bytes that the matching
+ * phyzb_*_workspace reports for the same arguments (256-byte aligned; NULL when it reports
+ * 0), free again when the call's work on `stream` is done. */
+
+/* Element type of an operator's arrays. */
+#define PHYZB_DT_F32 0
+#define PHYZB_DT_BF16 1
+#define PHYZB_DT_F16 2
+/* Activation of a linear layer (GELU in its tanh form). */
+#define PHYZB_ACT_NONE 0
+#define PHYZB_ACT_RELU 1
+#define PHYZB_ACT_TANH 2
+#define PHYZB_ACT_SILU 3
+#define PHYZB_ACT_GELU 4
+
+/* y = act(x w^T + bias) + residual: x [m][k], w [n][k], bias [n] (f32, may be
+ * NULL), residual and y [m][n] (residual may be NULL, or y itself), and, when
+ * `pre` is given, pre = x w^T + bias [m][n] for the backward pass. Every array
+ * but bias is of `dtype`; sums are f32 and rounded once. f32 operands are
+ * multiplied at f32 accuracy: on the FMA units where the layer is small, else
+ * as three bf16 terms each, six products (an infinity there gives NaN). m may
+ * be 0. */
+typedef struct {
+    int32_t dtype, activation, device;
+    int64_t m, k, n;
+    const void* x;
+    int64_t x_stride[2];
+    const void* w;
+    int64_t w_stride[2];
+    const float* bias;
+    const void* residual;
+    int64_t residual_stride[2];
+    void* y;
+    int64_t y_stride[2];
+    void* pre;
+    int64_t pre_stride[2];
+} phyzb_linear_args;
+int phyzb_linear_workspace(const phyzb_linear_args* a, int64_t* bytes);
+int phyzb_linear(const phyzb_linear_args* a, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradients of phyzb_linear: dz = dy act'(pre) (pre may be NULL without an
+ * activation), dx = dz w [m][k], dw = dz^T x [n][k], dbias = sum of dz over
+ * the rows [n] (f32). Each of dx, dw, dbias may be NULL: not wanted. dz is
+ * rounded to `dtype` for the two products and summed unrounded into dbias;
+ * the residual's gradient is dy. The order of every sum is fixed. */
+typedef struct {
+    int32_t dtype, activation, device;
+    int64_t m, k, n;
+    const void* dy;
+    int64_t dy_stride[2];
+    const void* pre;
+    int64_t pre_stride[2];
+    const void* x;
+    int64_t x_stride[2];
+    const void* w;
+    int64_t w_stride[2];
+    void* dx;
+    int64_t dx_stride[2];
+    void* dw;
+    int64_t dw_stride[2];
+    float* dbias;
+} phyzb_linear_grad_args;
+int phyzb_linear_grad_workspace(const phyzb_linear_grad_args* a, int64_t* bytes);
+int phyzb_linear_grad(const phyzb_linear_grad_args* a, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gated linear recurrence along t of [b][t][c] arrays:
+ *   a_t = sigmoid(gate_t),  h_t = a_t h_{t-1} + (1 - a_t) x_t,
+ * from h_{-1} = h0 [b][c] (f32, NULL = zeros), and where reset_t is not 0
+ * (an episode begins at t) from h_{t-1} = 0, which is dropped, not multiplied:
+ * a non-finite state does not survive a reset. reset is [b][t][c] bytes; a
+ * stride of 0 shares it over an axis. The state is f32; x, gate and h are of
+ * `dtype`. h_last [b][c] (f32, contiguous, may be NULL) is h at the last step,
+ * unrounded, and h0 where t = 0; with t = 1 it may be h0 itself (contiguous).
+ * The policy history's [step][feature][world] is the view b = feature,
+ * t = step, c = world. t = 1 is one control step. */
+typedef struct {
+    int32_t dtype, device;
+    int64_t b, t, c;
+    const void* x;
+    int64_t x_stride[3];
+    const void* gate;
+    int64_t gate_stride[3];
+    const float* h0;
+    int64_t h0_stride[2];
+    const uint8_t* reset;
+    int64_t reset_stride[3];
+    void* h;
+    int64_t h_stride[3];
+    float* h_last;
+} phyzb_scan_args;
+int phyzb_gated_scan_workspace(const phyzb_scan_args* a, int64_t* bytes);
+int phyzb_gated_scan(const phyzb_scan_args* a, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gradients of phyzb_gated_scan from dh [b][t][c] and dh_last [b][c] (f32, may
+ * be NULL), with the forward's inputs and its h:
+ *   d_t = dh_t + (reset_{t+1} ? 0 : a_{t+1} d_{t+1})  (dh_last at the end),
+ *   dx_t = (1 - a_t) d_t,  dgate_t = a_t (1 - a_t) (h_{t-1} - x_t) d_t,
+ * and dh0 [b][c] (f32, contiguous, may be NULL). Sums are f32. */
+typedef struct {
+    int32_t dtype, device;
+    int64_t b, t, c;
+    const void* dh;
+    int64_t dh_stride[3];
+    const void* x;
+    int64_t x_stride[3];
+    const void* gate;
+    int64_t gate_stride[3];
+    const void* h;
+    int64_t h_stride[3];
+    const float* h0;
+    int64_t h0_stride[2];
+    const uint8_t* reset;
+    int64_t reset_stride[3];
+    const float* dh_last;
+    int64_t dh_last_stride[2];
+    void* dx;
+    int64_t dx_stride[3];
+    void* dgate;
+    int64_t dgate_stride[3];
+    float* dh0;
+} phyzb_scan_grad_args;
+int phyzb_gated_scan_grad_workspace(const phyzb_scan_grad_args* a, int64_t* bytes);
+int phyzb_gated_scan_grad(const phyzb_scan_grad_args* a, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The Muon update of `batch` matrices [rows][cols], in place:
+ *   m <- mu m + g,  u = nesterov ? g + mu m : m,
+ *   X = u / (|u|_F + 1e-7), `steps` times
+ *     G = X X^T, X <- 3.4445 X + (-4.7750 G + 2.0315 G G) X
+ *     (from the right when rows > cols),
+ *   w <- (1 - lr weight_decay) w - lr scale X.
+ * grad is of `dtype`, momentum and weight are f32. copy (may be NULL) gets the
+ * new weights in `copy_dtype` (bf16 or f16: what phyzb_linear reads). Every
+ * array is [batch][rows][cols] with strides. steps = 1..16, sides at most
+ * 16384. The products take f16 pairs (high and low part) and sum in f32: as
+ * near the f64 result as f32 products are. */
+#define PHYZB_MUON_MAX_SIDE 16384
+typedef struct {
+    int32_t dtype, device, nesterov, steps;
+    int64_t batch, rows, cols;
+    const void* grad;
+    int64_t grad_stride[3];
+    float* momentum;
+    int64_t momentum_stride[3];
+    float* weight;
+    int64_t weight_stride[3];
+    int32_t copy_dtype, reserved;
+    void* copy;
+    int64_t copy_stride[3];
+    double lr, mu, weight_decay, scale;
+} phyzb_muon_args;
+int phyzb_muon_workspace(const phyzb_muon_args* a, int64_t* bytes);
+int phyzb_muon_update(const phyzb_muon_args* a, void* workspace, int64_t workspace_bytes, void* stream);
+/* The orthogonalised direction alone: out = X after `steps` iterations from
+ * X = x / (|x|_F + 1e-7); x and out of `dtype`. */
+typedef struct {
+    int32_t dtype, device, steps, reserved;
+    int64_t batch, rows, cols;
+    const void* x;
+    int64_t x_stride[3];
+    void* out;
+    int64_t out_stride[3];
+} phyzb_orthogonalize_args;
+int phyzb_orthogonalize_workspace(const phyzb_orthogonalize_args* a, int64_t* bytes);
+int phyzb_orthogonalize(const phyzb_orthogonalize_args* a, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

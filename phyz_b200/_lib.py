@@ -161,6 +161,12 @@ class PhyzbReturnCfg(C.Structure):
 
 KINEMATICS_STRIDE = 18
 
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_TANH, ACT_SILU, ACT_GELU = 0, 1, 2, 3, 4
+MUON_MAX_SIDE = 16384
+NN_OPS = ("linear", "linear_grad", "gated_scan", "gated_scan_grad", "muon_update", "orthogonalize")
+NN_WORKSPACES = ("linear", "linear_grad", "gated_scan", "gated_scan_grad", "muon", "orthogonalize")
+
 _P = C.c_void_p
 _D = C.POINTER(C.c_double)
 _I32P = C.POINTER(C.c_int32)
@@ -247,6 +253,9 @@ SIGNATURES = {
     "phyzb_comm_destroy": (C.c_int, [_P]),
     "phyzb_reduce_objective": (C.c_int, [_P, _P, C.c_int, C.c_double, C.POINTER(C.c_double)]),
     "phyzb_measure_fma_peak": (C.c_int, [C.c_int, _D]),
+    # recurrent-block operators: the argument structs are packed by nn.py
+    **{f"phyzb_{op}": (C.c_int, [C.c_char_p, _P, C.c_int64, _P]) for op in NN_OPS},
+    **{f"phyzb_{op}_workspace": (C.c_int, [C.c_char_p, C.POINTER(C.c_int64)]) for op in NN_WORKSPACES},
 }
 
 _lib = None

@@ -23,7 +23,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libphyzb200.so"
 OBJ = PKG / "_build"
 SOURCES = ["stepper.cu", "capi.cu", "capi_policy.cu", "capi_train.cu", "policy.cu", "train.cu", "flops.cpp",
-           "peaks.cu", "capi_noalloc.cu", "spec.cu"]
+           "peaks.cu", "capi_noalloc.cu", "spec.cu", "capi_nn.cu", "linear.cu", "scan.cu", "muon.cu"]
 VARIANT_SOURCE = "rollout_variants.cu"
 LANES_SOURCE = "lanes_variants.cu"
 FEAT_COUNT = 64  # pz_variants.h; bit 8 only with bit 4, bits 16 and 32 only with bit 2 (feat_valid)
@@ -31,7 +31,7 @@ VARIANTS = [(t, f) for t in ("float", "double") for f in range(FEAT_COUNT)
             if not (f & 8 and not f & 4) and not (f & 16 and not f & 2) and not (f & 32 and not f & 2)]
 HEADERS = ["pz_types.cuh", "pz_model.cuh", "pz_world.cuh", "pz_launch.h", "pz_pack.h", "pz_variants.h",
            "stepper_kernels.cuh", "pz_policy.h", "capi_internal.h", "pz_mlp.cuh", "pz_train.h", "pz_spec.h",
-           "pz_lanes.h", "stepper_lanes.cuh", "pz_lanes_sweep.cuh"]
+           "pz_lanes.h", "stepper_lanes.cuh", "pz_lanes_sweep.cuh", "pz_nn.h", "pz_nn.cuh", "simt_gemm.cuh"]
 # The lanes kernel (one world over several threads): ball / free, contact and
 # relabel bits only (pz_variants.h LANES_FEAT_COUNT)
 LANES_VARIANTS = [(t, f) for t in ("float", "double") for f in range(16) if not (f & 8 and not f & 4)]

@@ -1,0 +1,224 @@
+"""Operators of a recurrent policy or dynamics model on the device: the linear
+layer with its epilogue, the gated recurrence over the steps of a rollout, and
+the Muon update of the layers' matrices, each with the gradients that training
+it needs. Torch CUDA tensors in and out, over the C ABI's phyzb_linear,
+phyzb_gated_scan and phyzb_muon_update families (include/phyzb.h); no autograd.
+
+Tensors may have any strides (the policy history's [step][feature][world] is a
+view), and a call runs on the current stream of its tensors' device, without
+waiting for it. Scratch comes from torch's allocator on that stream.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+import struct
+
+import torch
+
+from . import _lib
+
+_DT = {torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+_ACT = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "tanh": _lib.ACT_TANH, "silu": _lib.ACT_SILU,
+        "gelu": _lib.ACT_GELU}
+
+# phyzb_linear_args and its siblings, field for field (native alignment)
+_LINEAR = struct.Struct("3i3qP2qP2qPP2qP2qP2q")
+_LINEAR_GRAD = struct.Struct("3i3qP2qP2qP2qP2qP2qP2qP")
+_SCAN = struct.Struct("2i3qP3qP3qP2qP3qP3qP")
+_SCAN_GRAD = struct.Struct("2i3qP3qP3qP3qP3qP2qP3qP2qP3qP3qP")
+_MUON = struct.Struct("4i3qP3qP3qP3q2iP3q4d")
+_ORTH = struct.Struct("4i3qP3qP3q")
+
+_NO2, _NO3 = (0, (0, 0)), (0, (0, 0, 0))
+
+
+def _need(ok: bool, msg: str) -> None:
+    if not ok:
+        raise ValueError(msg)
+
+
+def _dtype(t: torch.Tensor, name: str) -> int:
+    d = _DT.get(t.dtype)
+    if d is None:
+        raise ValueError(f"{name} is {t.dtype}: float32, bfloat16 or float16 is wanted")
+    return d
+
+
+def _arr(t, name: str, shape: tuple, dtype, device, none=None) -> tuple:
+    """(address, strides) of a tensor that must have this shape, type and device."""
+    if t is None:
+        _need(none is not None, f"{name} is missing")
+        return none
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}: {tuple(shape)} {dtype} on {device} is wanted")
+    return t.data_ptr(), t.stride()
+
+
+def _device(t: torch.Tensor, name: str) -> int:
+    _need(t.is_cuda, f"{name} is on {t.device}: a CUDA device is wanted")
+    return t.device.index
+
+
+def _activation(name: str) -> int:
+    a = _ACT.get(name)
+    _need(a is not None, f"activation {name!r} is none of {', '.join(_ACT)}")
+    return a
+
+
+def _call(op: str, query: str, args: bytes, device: torch.device) -> None:
+    lib = _lib.load()
+    need = C.c_int64(0)
+    _lib.check(getattr(lib, query)(args, C.byref(need)))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    _lib.check(getattr(lib, op)(args, ws.data_ptr() if ws is not None else None, need.value, stream))
+
+
+def _like(x: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    """An [rows, cols] output in x's order: feature-major where x is."""
+    if x.stride(0) == 1 and x.stride(1) != 1 and x.shape[0] > 1:
+        return torch.empty((cols, rows), dtype=x.dtype, device=x.device).t()
+    return torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+
+
+def linear(x, weight, bias=None, *, activation: str = "none", residual=None, save_pre: bool = False, out=None):
+    """act(x @ weight.T + bias) + residual for x [m, k], weight [n, k] of one type, bias [n] float32 and residual
+    [m, n] as x. The output takes x's order (feature-major in, feature-major out) unless `out` is given (which may be
+    the residual). With `save_pre` also returns x @ weight.T + bias, which the backward pass reads."""
+    _need(x.dim() == 2 and weight.dim() == 2, "x and weight must be matrices")
+    m, k = x.shape
+    n = weight.shape[0]
+    dt, dev, act = _dtype(x, "x"), _device(x, "x"), _activation(activation)
+    y = _like(x, m, n) if out is None else out
+    pre = _like(x, m, n) if save_pre else None
+    d, t = x.device, x.dtype
+    pw, sw = _arr(weight, "weight", (n, k), t, d)
+    py, sy = _arr(y, "out", (m, n), t, d)
+    pr, sr = _arr(residual, "residual", (m, n), t, d, _NO2)
+    pp, sp = _arr(pre, "pre", (m, n), t, d, _NO2)
+    pb = 0
+    if bias is not None:
+        pb, sb = _arr(bias, "bias", (n,), torch.float32, d)
+        _need(sb[0] == 1 or n == 1, "bias must be contiguous")
+    args = _LINEAR.pack(dt, act, dev, m, k, n, x.data_ptr(), *x.stride(), pw, *sw, pb, pr, *sr, py, *sy, pp, *sp)
+    _call("phyzb_linear", "phyzb_linear_workspace", args, d)
+    return (y, pre) if save_pre else y
+
+
+def linear_backward(dy, x, weight, pre=None, *, activation: str = "none", bias: bool = True, need_dx: bool = True,
+                    need_dw: bool = True):
+    """Gradients (dx, dweight, dbias) of `linear` from dy [m, n], with the forward's x, weight and pre-activations
+    (not needed without an activation). dx and dweight have the inputs' type, dbias is float32; what is not wanted is
+    None. The residual's gradient is dy itself."""
+    _need(x.dim() == 2 and weight.dim() == 2, "x and weight must be matrices")
+    m, k = x.shape
+    n = weight.shape[0]
+    dt, dev, act = _dtype(x, "x"), _device(x, "x"), _activation(activation)
+    d, t = x.device, x.dtype
+    pw, sw = _arr(weight, "weight", (n, k), t, d)
+    pd, sd = _arr(dy, "dy", (m, n), t, d)
+    pp, sp = _arr(pre, "pre", (m, n), t, d, _NO2 if act == 0 else None)
+    dx = _like(x, m, k) if need_dx else None
+    dw = torch.empty((n, k), dtype=t, device=d) if need_dw else None
+    db = torch.empty(n, dtype=torch.float32, device=d) if bias else None
+    px, sx = (dx.data_ptr(), dx.stride()) if need_dx else _NO2
+    pg, sg = (dw.data_ptr(), dw.stride()) if need_dw else _NO2
+    args = _LINEAR_GRAD.pack(dt, act, dev, m, k, n, pd, *sd, pp, *sp, x.data_ptr(), *x.stride(), pw, *sw, px, *sx,
+                             pg, *sg, db.data_ptr() if bias else 0)
+    _call("phyzb_linear_grad", "phyzb_linear_grad_workspace", args, d)
+    return dx, dw, db
+
+
+def _reset(reset, shape, device) -> tuple:
+    if reset is None:
+        return _NO3
+    if reset.dtype == torch.bool:
+        reset = reset.view(torch.uint8)
+    if reset.dim() == 2:
+        reset = reset.unsqueeze(2)
+    _need(reset.dtype == torch.uint8 and reset.device == device, f"reset must be uint8 or bool on {device}")
+    return reset.data_ptr(), reset.expand(shape).stride()
+
+
+def gated_scan(x, gate, h0=None, reset=None, *, out=None):
+    """h_t = a_t h_{t-1} + (1 - a_t) x_t along dim 1 of x, gate [b, t, c], a = sigmoid(gate), from h0 [b, c] (float32;
+    zeros without). Where reset ([b, t], or [b, t, c] with broadcasting) is not 0 the state before that step is
+    dropped. Returns (h in x's type and order, the last state [b, c] in float32)."""
+    _need(x.dim() == 3, "x must be [b, t, c]")
+    b, t, c = shape = x.shape
+    dt, dev, d = _dtype(x, "x"), _device(x, "x"), x.device
+    h = torch.empty_like(x) if out is None else out
+    last = torch.empty((b, c), dtype=torch.float32, device=d)
+    pg, sg = _arr(gate, "gate", shape, x.dtype, d)
+    p0, s0 = _arr(h0, "h0", (b, c), torch.float32, d, _NO2)
+    pr, sr = _reset(reset, shape, d)
+    ph, sh = _arr(h, "out", shape, x.dtype, d)
+    args = _SCAN.pack(dt, dev, b, t, c, x.data_ptr(), *x.stride(), pg, *sg, p0, *s0, pr, *sr, ph, *sh,
+                      last.data_ptr())
+    _call("phyzb_gated_scan", "phyzb_gated_scan_workspace", args, d)
+    return h, last
+
+
+def gated_scan_backward(dh, x, gate, h, h0=None, reset=None, dh_last=None):
+    """Gradients (dx, dgate, dh0) of `gated_scan` from dh [b, t, c] and dh_last [b, c] (float32), with the forward's
+    inputs and its h."""
+    _need(x.dim() == 3, "x must be [b, t, c]")
+    b, t, c = shape = x.shape
+    dt, dev, d = _dtype(x, "x"), _device(x, "x"), x.device
+    dx, dg = torch.empty_like(x), torch.empty_like(gate)
+    dh0 = torch.empty((b, c), dtype=torch.float32, device=d)
+    pd, sd = _arr(dh, "dh", shape, x.dtype, d)
+    pg, sg = _arr(gate, "gate", shape, x.dtype, d)
+    ph, sh = _arr(h, "h", shape, x.dtype, d)
+    p0, s0 = _arr(h0, "h0", (b, c), torch.float32, d, _NO2)
+    pr, sr = _reset(reset, shape, d)
+    pl, sl = _arr(dh_last, "dh_last", (b, c), torch.float32, d, _NO2)
+    args = _SCAN_GRAD.pack(dt, dev, b, t, c, pd, *sd, x.data_ptr(), *x.stride(), pg, *sg, ph, *sh, p0, *s0, pr, *sr,
+                           pl, *sl, dx.data_ptr(), *dx.stride(), dg.data_ptr(), *dg.stride(), dh0.data_ptr())
+    _call("phyzb_gated_scan_grad", "phyzb_gated_scan_grad_workspace", args, d)
+    return dx, dg, dh0
+
+
+def _matrices(t, name: str, shape=None):
+    _need(t.dim() in (2, 3), f"{name} must be [rows, cols] or [batch, rows, cols]")
+    t = t if t.dim() == 3 else t.unsqueeze(0)
+    if shape is not None:
+        _need(t.shape == shape, f"{name} is {tuple(t.shape)}: {tuple(shape)} is wanted")
+    return t
+
+
+def muon_update(weight, grad, momentum, *, lr: float, mu: float = 0.95, nesterov: bool = True,
+                weight_decay: float = 0.0, steps: int = 5, scale: float | None = None, copy=None) -> None:
+    """Muon step of one matrix [rows, cols] or a stack [batch, rows, cols], in place: momentum <- mu momentum + grad,
+    weight <- (1 - lr weight_decay) weight - lr scale NewtonSchulz(grad + mu momentum). weight and momentum are
+    float32, grad any type, scale sqrt(max(1, rows / cols)) unless given; `copy` (bfloat16 or float16) gets the new
+    weights too."""
+    w = _matrices(weight, "weight")
+    shape, d = w.shape, w.device
+    g = _matrices(grad, "grad", shape)
+    dt, dev = _dtype(g, "grad"), _device(w, "weight")
+    b, r, c = shape
+    pw, sw = _arr(w, "weight", shape, torch.float32, d)
+    pg, sg = _arr(g, "grad", shape, g.dtype, d)
+    pm, sm = _arr(_matrices(momentum, "momentum", shape), "momentum", shape, torch.float32, d)
+    pc, sc, cdt = 0, (0, 0, 0), 0
+    if copy is not None:
+        _need(copy.dtype in (torch.bfloat16, torch.float16), f"copy is {copy.dtype}: bfloat16 or float16 is wanted")
+        pc, sc = _arr(_matrices(copy, "copy", shape), "copy", shape, copy.dtype, d)
+        cdt = _DT[copy.dtype]
+    scale = math.sqrt(max(1.0, r / c)) if scale is None else scale
+    args = _MUON.pack(dt, dev, int(bool(nesterov)), steps, b, r, c, pg, *sg, pm, *sm, pw, *sw, cdt, 0, pc, *sc,
+                      lr, mu, weight_decay, scale)
+    _call("phyzb_muon_update", "phyzb_muon_workspace", args, d)
+
+
+def orthogonalize(x, *, steps: int = 5):
+    """The Newton-Schulz iterate of one matrix or a stack of them, X = x / |x|_F first: singular values towards 1 (the
+    Muon coefficients leave them within about 0.7 .. 1.2). In x's type."""
+    v = _matrices(x, "x")
+    dt, dev = _dtype(v, "x"), _device(v, "x")
+    out = torch.empty_like(v, memory_format=torch.contiguous_format)
+    args = _ORTH.pack(dt, dev, steps, 0, *v.shape, v.data_ptr(), *v.stride(), out.data_ptr(), *out.stride())
+    _call("phyzb_orthogonalize", "phyzb_orthogonalize_workspace", args, v.device)
+    return out if x.dim() == 3 else out[0]
