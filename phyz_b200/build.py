@@ -31,7 +31,8 @@ VARIANTS = [(t, f) for t in ("float", "double") for f in range(FEAT_COUNT)
             if not (f & 8 and not f & 4) and not (f & 16 and not f & 2) and not (f & 32 and not f & 2)]
 HEADERS = ["pz_types.cuh", "pz_model.cuh", "pz_world.cuh", "pz_launch.h", "pz_pack.h", "pz_variants.h",
            "stepper_kernels.cuh", "pz_policy.h", "capi_internal.h", "pz_mlp.cuh", "pz_train.h", "pz_spec.h",
-           "pz_lanes.h", "stepper_lanes.cuh", "pz_lanes_sweep.cuh", "pz_nn.h", "pz_nn.cuh", "simt_gemm.cuh"]
+           "pz_lanes.h", "stepper_lanes.cuh", "pz_lanes_sweep.cuh", "pz_nn.h", "pz_nn.cuh", "pz_tma.h", "pz_tma.cuh", "gemm.cuh",
+           "simt_gemm.cuh"]
 # The lanes kernel (one world over several threads): ball / free, contact and
 # relabel bits only (pz_variants.h LANES_FEAT_COUNT)
 LANES_VARIANTS = [(t, f) for t in ("float", "double") for f in range(16) if not (f & 8 and not f & 4)]

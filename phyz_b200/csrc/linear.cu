@@ -1,154 +1,776 @@
 // The linear layer y = act(x w^T + b) + r and its gradients.
+//
+// Forward: one product with everything else in its epilogue. Backward: dz =
+// dy act'(z) and its column sums (db) in one pass, then dx = dz w and dw =
+// dz^T x, the long sum of dw over the rows cut into splits that fill the GPU.
+// A product computes D[i][j] with i the contiguous side of its result, so that
+// a warp's lanes read and write neighbours in the epilogue.
+//
+// Three ways to multiply:
+//   rows_kernel       a few rows (serving): the weights go by once, on the FMA
+//                     units, a warp to a feature.
+//   gemm.cuh          tensor cores, bf16 and f16 as they are, f32 as three bf16
+//                     planes.
+//   simt_gemm.cuh     f32 on the FMA units, where the layer is small.
+// Operands that TMA cannot address (odd strides, odd bases) and f32 planes are
+// written to the workspace first, in the order in which they are.
+#include <type_traits>
+
+#include "gemm.cuh"
 #include "simt_gemm.cuh"
 
 namespace pz {
 
 namespace {
 
+__device__ unsigned int g_linear_fault;  // waits that ran out (pz_tma.cuh)
+
+// Each device's address of g_linear_fault (a kernel of another file's template
+// gets it as an argument).
+unsigned int* fault_word() {
+    static std::atomic<unsigned int*> at[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return nullptr;
+    unsigned int* p = at[dev].load(std::memory_order_acquire);
+    if (!p) {
+        void* q = nullptr;
+        if (cudaGetSymbolAddress(&q, g_linear_fault) != cudaSuccess) return nullptr;
+        at[dev].store(p = (unsigned int*)q, std::memory_order_release);
+    }
+    return p;
+}
+
+long long up(long long v, long long to = 256) { return (v + to - 1) / to * to; }
+long long esize(int dtype) { return dtype == PHYZB_DT_F32 ? 4 : 2; }
+
+// ── epilogues ─────────────────────────────────────────────────────────────
+
+// An array seen from D: element (i, j) at p[i * is + j * js].
+template <class T>
+struct Out {
+    T* p = nullptr;
+    long long is = 0, js = 0;
+};
+
+// four neighbours along the contiguous side, in one access where they are
+// aligned
+template <class T>
+__device__ __forceinline__ bool whole4(const T* p, long long stride, int n) {
+    return n == 4 && stride == 1 && ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0;
+}
+__device__ __forceinline__ void load4(const float* p, long long stride, int n, float* v) {
+    if (whole4(p, stride, n)) {
+        *(float4*)v = *(const float4*)p;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = e < n ? p[e * stride] : 0.0f;
+    }
+}
+__device__ __forceinline__ void store4(float* p, long long stride, int n, const float* v) {
+    if (whole4(p, stride, n)) {
+        *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (e < n) p[e * stride] = v[e];
+    }
+}
+
 template <class T>
 struct LinearEpi {
     const float* bias;
-    NnMat res, y, pre;
+    int by_i;  // bias along i
     int act;
-    __device__ void operator()(long long, long long i, long long j, float z) const {
-        if (bias) z += bias[j];
-        if (pre.p) ((T*)pre.p)[i * pre.rs + j * pre.cs] = from_f32<T>(z);
+    Out<const T> res;
+    Out<T> y, pre;
+    long long m;  // rows of D
+
+    __device__ __forceinline__ void one(long long i, long long j, float z) const {
+        if (bias) z += bias[by_i ? i : j];
+        if (pre.p) pre.p[i * pre.is + j * pre.js] = from_f32<T>(z);
         float v = act_f32(z, act);
-        if (res.p) v += to_f32(((const T*)res.p)[i * res.rs + j * res.cs]);
-        ((T*)y.p)[i * y.rs + j * y.cs] = from_f32<T>(v);
+        if (res.p) v += to_f32(res.p[i * res.is + j * res.js]);
+        y.p[i * y.is + j * y.js] = from_f32<T>(v);
+    }
+    __device__ __forceinline__ void four(int, long long i, long long j, const float* sum, int n, bool along_i) const {
+        if constexpr (sizeof(T) == 4) {
+            float z[4], r[4] = {};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                z[e] = sum[e];
+                if (bias && e < n) z[e] += bias[(by_i != 0) == along_i ? (along_i ? i : j) + e : by_i ? i : j];
+            }
+            if (pre.p) store4(pre.p + i * pre.is + j * pre.js, along_i ? pre.is : pre.js, n, z);
+            if (res.p) load4(res.p + i * res.is + j * res.js, along_i ? res.is : res.js, n, r);
+#pragma unroll
+            for (int e = 0; e < 4; e++) z[e] = act_f32(z[e], act) + r[e];
+            store4(y.p + i * y.is + j * y.js, along_i ? y.is : y.js, n, z);
+        }
+    }
+    __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, const float* sum) const {
+        if (i >= m) return;
+        float r[32];
+        if (res.p) {  // (the residual may be y itself: all 32 are read before any is written)
+            const T* p = res.p + i * res.is + j0 * res.js;
+#pragma unroll
+            for (int c = 0; c < 32; c++) {
+                r[c] = c < cols ? to_f32(*p) : 0.0f;
+                p += res.js;
+            }
+        }
+        const float b = bias && by_i ? bias[i] : 0.0f;
+        T* py = y.p + i * y.is + j0 * y.js;
+        T* pp = pre.p + i * pre.is + j0 * pre.js;
+#pragma unroll
+        for (int c = 0; c < 32; c++) {
+            if (c >= cols) break;
+            float z = sum[c] + b;
+            if (bias && !by_i) z += bias[j0 + c];
+            if (pre.p) {
+                *pp = from_f32<T>(z);
+                pp += pre.js;
+            }
+            z = act_f32(z, act);
+            if (res.p) z += r[c];
+            *py = from_f32<T>(z);
+            py += y.js;
+        }
     }
 };
 
 template <class T>
 struct StoreEpi {
-    NnMat out;
-    __device__ void operator()(long long, long long i, long long j, float v) const {
-        ((T*)out.p)[i * out.rs + j * out.cs] = from_f32<T>(v);
+    Out<T> out;
+    long long m;
+    __device__ __forceinline__ void one(long long i, long long j, float v) const {
+        out.p[i * out.is + j * out.js] = from_f32<T>(v);
+    }
+    __device__ __forceinline__ void four(int, long long i, long long j, const float* v, int n, bool along_i) const {
+        if constexpr (sizeof(T) == 4) store4(out.p + i * out.is + j * out.js, along_i ? out.is : out.js, n, v);
+    }
+    __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, const float* v) const {
+        if (i >= m) return;
+        T* p = out.p + i * out.is + j0 * out.js;
+#pragma unroll
+        for (int c = 0; c < 32; c++) {
+            if (c >= cols) break;
+            *p = from_f32<T>(v[c]);
+            p += out.js;
+        }
     }
 };
 
-// Partial sums of a split product, [split][M][N] f32.
+// A split's part, [split][n][m] f32.
 struct PartEpi {
     float* part;
-    long long M, N;
-    __device__ void operator()(long long z, long long i, long long j, float v) const {
-        part[(z * M + i) * N + j] = v;
+    long long m, n;
+    __device__ __forceinline__ void four(int split, long long i, long long j, const float* v, int k, bool along_i) const {
+        store4(part + (split * n + j) * m + i, along_i ? 1 : m, k, v);
+    }
+    __device__ __forceinline__ void operator()(const GemmUnit& q, long long i, int j0, int cols, const float* v) const {
+        if (i >= m) return;
+        float* p = part + (q.split * n + j0) * m + i;
+#pragma unroll
+        for (int c = 0; c < 32; c++) {
+            if (c >= cols) break;
+            *p = v[c];
+            p += m;
+        }
+    }
+};
+
+// The parts in order, through the epilogue.
+template <class Epi>
+__global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, long long m, long long n, Epi epi) {
+    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (e >= m * n) return;
+    float v = 0.0f;
+#pragma unroll 8
+    for (int s = 0; s < splits; s++) v += part[s * m * n + e];
+    epi.one(e % m, e / m, v);
+}
+
+// ── operands ──────────────────────────────────────────────────────────────
+
+// x as three bf16 terms that sum to it to 2^-24 (each the nearest to what is
+// left). What is past bf16's range towards infinity is cut, not rounded up; an
+// infinity or a NaN is in the first term alone.
+__device__ __forceinline__ void planes_of(float x, __nv_bfloat16* p) {
+    float left = x;
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+        p[k] = __float2bfloat16_rn(left);
+        if (isinf(__bfloat162float(p[k])) && !isinf(left)) p[k] = __float2bfloat16_rz(left);
+        left = isfinite(left) ? left - __bfloat162float(p[k]) : 0.0f;
+    }
+}
+
+// rows x k values into 16-bit planes [outer][inner padded], in the order of src:
+// inner is the side that is contiguous there.
+template <class T>
+__global__ void __launch_bounds__(256) pack_kernel(const T* src, long long os, long long is, long long outer,
+                                                   long long inner, long long pitch, uint16_t* dst, long long plane) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= inner) return;
+    for (long long o = blockIdx.y; o < outer; o += gridDim.y) {
+        const T v = src[o * os + i * is];
+        if constexpr (sizeof(T) == 2) {
+            dst[o * pitch + i] = *reinterpret_cast<const uint16_t*>(&v);
+        } else {
+            __nv_bfloat16 p[3];
+            planes_of(v, p);
+#pragma unroll
+            for (int k = 0; k < 3; k++) dst[k * plane + o * pitch + i] = *reinterpret_cast<const uint16_t*>(&p[k]);
+        }
+    }
+}
+
+// An operand of a tensor-core product: where it is, and whether it has to be
+// packed first (f32 always).
+struct Operand {
+    GemmMat mat;  // as given; element strides
+    long long rows, k;
+    int dtype;
+    bool pack;
+    long long pitch, plane, bytes;
+
+    Operand(const void* p, long long rs, long long ks, long long rows, long long k, int dtype)
+        : mat{p, rs, ks, 0}, rows(rows), k(k), dtype(dtype) {
+        pack = dtype == PHYZB_DT_F32 || !gemm_tma_ok(mat, rows, k, 1);
+        const bool mn = gemm_mn(mat, k);
+        pitch = up(mn ? rows : k, 8);
+        plane = up(pitch * (mn ? k : rows), 128);
+        bytes = pack ? plane * 2 * (dtype == PHYZB_DT_F32 ? 3 : 1) : 0;
+    }
+    // the planes, packed into ws where need be
+    cudaError_t ready(char* ws, GemmMat* out, cudaStream_t st) const {
+        if (!pack) {
+            out[0] = mat;
+            return cudaSuccess;
+        }
+        const bool mn = gemm_mn(mat, k);
+        const long long outer = mn ? k : rows, inner = mn ? rows : k, os = mn ? mat.ks : mat.rs, is = mn ? 1 : mat.ks;
+        const dim3 grid((unsigned)((inner + 255) / 256), (unsigned)(outer < 65535 ? outer : 65535));
+        if (dtype == PHYZB_DT_F32)
+            pack_kernel<<<grid, 256, 0, st>>>((const float*)mat.p, os, is, outer, inner, pitch, (uint16_t*)ws, plane);
+        else
+            pack_kernel<<<grid, 256, 0, st>>>((const __half*)mat.p, os, is, outer, inner, pitch, (uint16_t*)ws, plane);
+        for (int p = 0; p < (dtype == PHYZB_DT_F32 ? 3 : 1); p++)
+            out[p] = {ws + p * plane * 2, mn ? 1 : pitch, mn ? pitch : 1, 0};
+        return cudaGetLastError();
+    }
+};
+
+// ── tensor-core products ──────────────────────────────────────────────────
+
+// How a product is cut: columns of a tile (256, 128 or 64; 128 at most for
+// planes), splits of k. The widest tile does most work per byte of shared
+// memory; narrower ones are taken where the wide ones leave SMs idle in the last
+// round (a tile costs about its width and 32 columns more).
+struct Cut {
+    int bn, splits;
+};
+Cut cut_of(long long rows, long long cols, long long k, bool f32) {
+    const long long ti = (rows + 127) / 128;
+    Cut c{0, 1};
+    long long best = 0;
+    for (int bn = f32 ? 128 : 256; bn >= 64; bn /= 2) {
+        const long long tiles = ti * ((cols + bn - 1) / bn);
+        const long long cost = (tiles + GEMM_SMS - 1) / GEMM_SMS * (bn + 32);
+        if (!c.bn || cost < best) {
+            c.bn = bn;
+            best = cost;
+        }
+    }
+    const long long kb = (k + GEMM_BK - 1) / GEMM_BK;
+    if (ti * ((cols + 255) / 256) < GEMM_SMS / 2) {
+        // too few tiles: cut k as well, into tiles as wide as they were
+        int bn = f32 ? 128 : 256;
+        while (bn > 64 && bn / 2 >= cols) bn /= 2;
+        const int s = gemm_splits(ti * ((cols + bn - 1) / bn), kb);
+        if (s > 1) return {bn, s};
+    }
+    return c;
+}
+
+long long part_bytes(const Cut& c, long long rows, long long cols) {
+    return c.splits > 1 ? up(c.splits * rows * cols * 4) : 0;
+}
+
+// T's planes: three for f32, else the values themselves.
+template <class T, class Epi>
+cudaError_t multiply_cut(const GemmMat* a, const GemmMat* b, long long rows, long long cols, long long k, const Cut& c,
+                         const Epi& epi, cudaStream_t st) {
+    unsigned int* fault = fault_word();
+    if (!fault) return cudaErrorInvalidSymbol;
+    constexpr bool bf16 = !std::is_same<T, __half>::value;
+    constexpr int PL = sizeof(T) == 4 ? 3 : 1;
+    if constexpr (PL == 1)
+        if (c.bn == 256) return gemm_launch<256, PL>(a, b, rows, cols, k, 1, c.splits, false, bf16, epi, fault, st);
+    if (c.bn == 128) return gemm_launch<128, PL>(a, b, rows, cols, k, 1, c.splits, false, bf16, epi, fault, st);
+    return gemm_launch<64, PL>(a, b, rows, cols, k, 1, c.splits, false, bf16, epi, fault, st);
+}
+
+// D = A B^T through `epi`; part: room for the splits' parts.
+template <class T, class Epi>
+cudaError_t multiply(const GemmMat* a, const GemmMat* b, long long rows, long long cols, long long k, const Cut& c,
+                     char* part, const Epi& epi, cudaStream_t st) {
+    if (c.splits == 1) return multiply_cut<T>(a, b, rows, cols, k, c, epi, st);
+    const cudaError_t e = multiply_cut<T>(a, b, rows, cols, k, c, PartEpi{(float*)part, rows, cols}, st);
+    if (e != cudaSuccess) return e;
+    join_kernel<<<(unsigned)((rows * cols + 255) / 256), 256, 0, st>>>((const float*)part, c.splits, rows, cols, epi);
+    return cudaGetLastError();
+}
+
+// ── f32 on the FMA units ──────────────────────────────────────────────────
+
+// Rough times of both ways in microseconds: the FMA units at 25 TFLOP/s; the
+// tensor cores at 200 (six products) behind two packing launches that move ten
+// bytes a value at 4 TB/s.
+bool simt_is_faster(double rows, double cols, double k) {
+    const double flop = 2e-6 * rows * cols * k;
+    return flop / 25.0 < flop / 200.0 + 10e-6 * (rows + cols) * k / 4.0 + 12.0;
+}
+
+// Splits of k so that the 128 x 64 tiles are two to an SM, each of 256 at least.
+int simt_splits(long long rows, long long cols, long long k) {
+    const long long tiles = ((rows + 127) / 128) * ((cols + 63) / 64);
+    if (tiles >= GEMM_SMS / 2) return 1;
+    long long s = 2 * GEMM_SMS / tiles;
+    if (s > k / 256) s = k / 256;
+    return s < 2 ? 1 : (int)s;
+}
+
+template <class Epi>
+cudaError_t simt_multiply(const SimtOperand& a, const SimtOperand& b, long long rows, long long cols, long long k,
+                          int splits, bool along_i, char* part, const Epi& epi, cudaStream_t st) {
+    if (splits == 1) return simt_gemm(a, b, rows, cols, k, 1, along_i, epi, st);
+    const cudaError_t e = simt_gemm(a, b, rows, cols, k, splits, true, PartEpi{(float*)part, rows, cols}, st);
+    if (e != cudaSuccess) return e;
+    join_kernel<<<(unsigned)((rows * cols + 255) / 256), 256, 0, st>>>((const float*)part, splits, rows, cols, epi);
+    return cudaGetLastError();
+}
+
+// ── a few rows ────────────────────────────────────────────────────────────
+
+constexpr int FEW = 8;
+
+// A warp takes a feature: its weights once, 16 bytes a lane where V > 1, against
+// M rows of x (which stay in the caches), sums in f32, joined by shuffles; lane r
+// finishes row r.
+template <class T, int M, int V>
+__global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ phyzb_linear_args a, LinearEpi<T> epi) {
+    const int lane = threadIdx.x % 32;
+    const long long n = (long long)blockIdx.x * 4 + threadIdx.x / 32;
+    if (n >= a.n) return;
+    const T* w = (const T*)a.w + n * a.w_stride[0];
+    const T* x = (const T*)a.x;
+    float sum[M] = {};
+#pragma unroll 4
+    for (long long k = lane * V; k < a.k; k += 32 * V) {
+        T wv[V];
+        if constexpr (V > 1) {
+            *reinterpret_cast<uint4*>(wv) = *reinterpret_cast<const uint4*>(w + k);
+        } else {
+            wv[0] = w[k * a.w_stride[1]];
+        }
+#pragma unroll
+        for (int r = 0; r < M; r++) {
+            if (r >= a.m) break;
+            T xv[V];
+            if constexpr (V > 1) {
+                *reinterpret_cast<uint4*>(xv) = *reinterpret_cast<const uint4*>(x + r * a.x_stride[0] + k);
+            } else {
+                xv[0] = x[r * a.x_stride[0] + k * a.x_stride[1]];
+            }
+#pragma unroll
+            for (int v = 0; v < V; v++) sum[r] = fmaf(to_f32(wv[v]), to_f32(xv[v]), sum[r]);
+        }
+    }
+    float mine = 0.0f;
+#pragma unroll
+    for (int r = 0; r < M; r++) {
+#pragma unroll
+        for (int o = 16; o; o /= 2) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], o);
+        if (lane == r) mine = sum[r];
+    }
+    if (lane < a.m) epi.one(n, lane, mine);
+}
+
+template <class T>
+bool rows_wide(const phyzb_linear_args& a) {
+    const int v = 16 / (int)sizeof(T);
+    return a.k % v == 0 && a.w_stride[1] == 1 && a.x_stride[1] == 1 && (uintptr_t)a.w % 16 == 0 &&
+           (uintptr_t)a.x % 16 == 0 && (a.n == 1 || a.w_stride[0] % v == 0) && (a.m == 1 || a.x_stride[0] % v == 0);
+}
+
+// ── forward ───────────────────────────────────────────────────────────────
+
+enum Way { ROWS, SIMT, TENSOR };
+
+Way way_of(const phyzb_linear_args& a) {
+    // (a warp's lanes walk k: weights with n contiguous would be read a sector a value)
+    if (a.m <= FEW && (a.w_stride[1] == 1 || a.k == 1)) return ROWS;
+    return a.dtype == PHYZB_DT_F32 && simt_is_faster((double)a.m, (double)a.n, (double)a.k) ? SIMT : TENSOR;
+}
+
+// i is the side along which y is contiguous: the features, unless only the rows are.
+struct Forward {
+    bool rows_first;  // i = rows of x
+    long long di, dj;
+    Operand x, w;
+    Cut cut;
+    long long ws_x, ws_w, ws_part, total;
+    explicit Forward(const phyzb_linear_args& a)
+        : rows_first(a.y_stride[1] != 1 && a.y_stride[0] == 1),
+          di(rows_first ? a.m : a.n),
+          dj(rows_first ? a.n : a.m),
+          x(a.x, a.x_stride[0], a.x_stride[1], a.m, a.k, a.dtype),
+          w(a.w, a.w_stride[0], a.w_stride[1], a.n, a.k, a.dtype),
+          cut(cut_of(di, dj, a.k, a.dtype == PHYZB_DT_F32)) {
+        ws_x = 0;
+        ws_w = up(x.bytes);
+        ws_part = ws_w + up(w.bytes);
+        total = ws_part + part_bytes(cut, di, dj);
     }
 };
 
 template <class T>
-__global__ void join_kernel(const float* part, int splits, long long M, long long N, NnMat out) {
-    const long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (e >= M * N) return;
-    float v = 0.0f;
-    for (int s = 0; s < splits; s++) v += part[s * M * N + e];
-    ((T*)out.p)[e / N * out.rs + e % N * out.cs] = from_f32<T>(v);
+LinearEpi<T> epilogue(const phyzb_linear_args& a, bool rows_first) {
+    auto turn = [&](auto* p, const int64_t* s) {
+        return Out<std::remove_pointer_t<decltype(p)>>{p, rows_first ? s[0] : s[1], rows_first ? s[1] : s[0]};
+    };
+    return {a.bias, !rows_first, a.activation, turn((const T*)a.residual, a.residual_stride), turn((T*)a.y, a.y_stride),
+            turn((T*)a.pre, a.pre_stride), rows_first ? a.m : a.n};
 }
 
-constexpr int DZ_ROWS = 256;  // rows per block of dz_kernel
-
-// dz = dy act'(pre) into [m][n], and each block's column sums of the unrounded
-// dz into part [row block][n].
 template <class T>
-__global__ void __launch_bounds__(128) dz_kernel(const phyzb_linear_grad_args a, T* dz, float* part) {
-    const long long j = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (j >= a.n) return;
-    const long long i0 = (long long)blockIdx.y * DZ_ROWS, i1 = i0 + DZ_ROWS < a.m ? i0 + DZ_ROWS : a.m;
+cudaError_t forward(const phyzb_linear_args& a, char* ws, cudaStream_t st) {
+    const Way way = way_of(a);
+    if (way == ROWS) {
+        const LinearEpi<T> epi = epilogue<T>(a, false);
+        const unsigned grid = (unsigned)((a.n + 3) / 4);
+        constexpr int V = 16 / sizeof(T);
+        const bool wide = rows_wide<T>(a);
+        auto run = [&](auto m) {
+            constexpr int M = decltype(m)::value;
+            if (wide)
+                rows_kernel<T, M, V><<<grid, 128, 0, st>>>(a, epi);
+            else
+                rows_kernel<T, M, 1><<<grid, 128, 0, st>>>(a, epi);
+            return cudaGetLastError();
+        };
+        if (a.m == 1) return run(std::integral_constant<int, 1>());
+        if (a.m <= 4) return run(std::integral_constant<int, 4>());
+        return run(std::integral_constant<int, FEW>());
+    }
+    if constexpr (sizeof(T) == 4) {
+        if (way == SIMT) {
+            // (i = rows here; the epilogue takes either order)
+            const bool along_i = a.y_stride[1] != 1 && a.y_stride[0] == 1;
+            return simt_multiply({(const float*)a.x, a.x_stride[0], a.x_stride[1]},
+                                 {(const float*)a.w, a.w_stride[0], a.w_stride[1]}, a.m, a.n, a.k,
+                                 simt_splits(a.m, a.n, a.k), along_i, ws, epilogue<T>(a, true), st);
+        }
+    }
+    const Forward f(a);
+    GemmMat x[3], w[3];
+    cudaError_t e = f.x.ready(ws + f.ws_x, x, st);
+    if (e == cudaSuccess) e = f.w.ready(ws + f.ws_w, w, st);
+    if (e != cudaSuccess) return e;
+    return multiply<T>(f.rows_first ? x : w, f.rows_first ? w : x, f.di, f.dj, a.k, f.cut, ws + f.ws_part,
+                    epilogue<T>(a, f.rows_first), st);
+}
+
+// ── backward ──────────────────────────────────────────────────────────────
+
+// dz = dy act'(pre) in dy's order (inner: its contiguous side), and the sums of
+// the unrounded dz over the rows: each block's part to part[block][n]. dz
+// [outer][pitch]: T, or three bf16 planes. dz or part may be null.
+struct DzArgs {
+    const void *dy, *pre;
+    long long dy_o, dy_i, pre_o, pre_i;  // strides along outer and inner
+    long long outer, inner, pitch, plane;
+    void* dz;
+    float* part;
+    int act, planes;
+};
+constexpr int DZ_OUTER = 64;    // outer lines of a block
+constexpr int DZ_INNER = 2048;  // inner values of a block, where it sums along them
+
+template <class T>
+__device__ __forceinline__ float dz_value(const DzArgs& a, long long o, long long i) {
+    float v = to_f32(((const T*)a.dy)[o * a.dy_o + i * a.dy_i]);
+    if (a.act != PHYZB_ACT_NONE) v *= act_grad_f32(to_f32(((const T*)a.pre)[o * a.pre_o + i * a.pre_i]), a.act);
+    return v;
+}
+template <class T>
+__device__ __forceinline__ void dz_store(const DzArgs& a, long long o, long long i, float v) {
+    if (!a.dz) return;
+    if (a.planes == 3) {
+        __nv_bfloat16 p[3];
+        planes_of(v, p);
+#pragma unroll
+        for (int k = 0; k < 3; k++) ((__nv_bfloat16*)a.dz)[k * a.plane + o * a.pitch + i] = p[k];
+    } else {
+        ((T*)a.dz)[o * a.pitch + i] = from_f32<T>(v);
+    }
+}
+
+// inner = features. V neighbours per thread, 256 threads = 32 along the features
+// x 8 rows.
+template <class T, int V>
+__global__ void __launch_bounds__(256) dz_rows_kernel(const __grid_constant__ DzArgs a) {
+    __shared__ float sums[8][32 * V];
+    const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+    const long long i0 = ((long long)blockIdx.x * 32 + tx) * V;
+    const long long o1 = (blockIdx.y + 1) * (long long)DZ_OUTER < a.outer ? (blockIdx.y + 1) * (long long)DZ_OUTER : a.outer;
+    float sum[V] = {};
+    if (i0 < a.inner) {
+#pragma unroll 4
+        for (long long o = blockIdx.y * (long long)DZ_OUTER + ty; o < o1; o += 8) {
+            float v[V];
+            if constexpr (V > 1) {
+                T d[V], z[V], out[V];
+                *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>((const T*)a.dy + o * a.dy_o + i0);
+                if (a.act != PHYZB_ACT_NONE)
+                    *reinterpret_cast<uint4*>(z) = *reinterpret_cast<const uint4*>((const T*)a.pre + o * a.pre_o + i0);
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    v[e] = to_f32(d[e]);
+                    if (a.act != PHYZB_ACT_NONE) v[e] *= act_grad_f32(to_f32(z[e]), a.act);
+                    out[e] = from_f32<T>(v[e]);
+                }
+                if (a.planes == 3) {
+#pragma unroll
+                    for (int e = 0; e < V; e++) dz_store<T>(a, o, i0 + e, v[e]);
+                } else if (a.dz) {
+                    *reinterpret_cast<uint4*>((T*)a.dz + o * a.pitch + i0) = *reinterpret_cast<const uint4*>(out);
+                }
+            } else {
+                v[0] = dz_value<T>(a, o, i0);
+                dz_store<T>(a, o, i0, v[0]);
+            }
+#pragma unroll
+            for (int e = 0; e < V; e++) sum[e] += v[e];
+        }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int e = 0; e < V; e++) sums[ty][tx * V + e] = sum[e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 32 * V; c += 256) {
+        float s = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 8; r++) s += sums[r][c];
+        const long long i = (long long)blockIdx.x * 32 * V + c;
+        if (i < a.inner) a.part[blockIdx.y * a.inner + i] = s;
+    }
+}
+
+// inner = rows: a block takes DZ_INNER of one feature's.
+template <class T>
+__global__ void __launch_bounds__(256) dz_features_kernel(const __grid_constant__ DzArgs a) {
+    __shared__ float sums[8];
+    const long long i0 = (long long)blockIdx.x * DZ_INNER, o = blockIdx.y;
     float sum = 0.0f;
-    for (long long i = i0; i < i1; i++) {
-        float v = to_f32(((const T*)a.dy)[i * a.dy_stride[0] + j * a.dy_stride[1]]);
-        if (a.activation != PHYZB_ACT_NONE)
-            v *= act_grad_f32(to_f32(((const T*)a.pre)[i * a.pre_stride[0] + j * a.pre_stride[1]]), a.activation);
-        sum += v;
-        dz[i * a.n + j] = from_f32<T>(v);
+#pragma unroll
+    for (int u = 0; u < DZ_INNER / 256; u++) {
+        const long long i = i0 + u * 256 + threadIdx.x;
+        if (i < a.inner) {
+            const float v = dz_value<T>(a, o, i);
+            dz_store<T>(a, o, i, v);
+            sum += v;
+        }
     }
-    part[blockIdx.y * a.n + j] = sum;
+#pragma unroll
+    for (int s = 16; s; s /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0 && a.part) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; w++) s += sums[w];
+        a.part[blockIdx.x * a.outer + o] = s;
+    }
 }
 
-__global__ void column_sum_kernel(const float* part, long long rows, long long n, float* out) {
-    const long long j = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (j >= n) return;
+// out[j] = sum over the blocks of part[block][j]: 8 warps take every 8th block.
+__global__ void __launch_bounds__(256) column_sum_kernel(const float* part, long long blocks, long long n, float* out) {
+    __shared__ float sums[8][32];
+    const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+    const long long j = (long long)blockIdx.x * 32 + tx;
     float v = 0.0f;
-    for (long long r = 0; r < rows; r++) v += part[r * n + j];
-    out[j] = v;
+    if (j < n) {
+#pragma unroll 8
+        for (long long r = ty; r < blocks; r += 8) v += part[r * n + j];
+    }
+    sums[ty][tx] = v;
+    __syncthreads();
+    if (ty == 0 && j < n) {
+#pragma unroll
+        for (int r = 1; r < 8; r++) v += sums[r][tx];
+        out[j] = v;
+    }
 }
 
-long long up(long long v) { return (v + 255) / 256 * 256; }
-long long esize(int dtype) { return dtype == PHYZB_DT_F32 ? 4 : 2; }
+struct Backward {
+    bool features;            // dy has its rows contiguous: dz is [n][m padded]
+    bool simt_dx, simt_dw;    // f32 on the FMA units
+    bool own_dz;              // dz is written (else dy is used as it is)
+    int planes;               // of dz: 0 = T
+    long long outer, inner, pitch, plane, blocks;
+    bool dx_rows_first;       // dx: i = rows
+    Cut cut_dx, cut_dw;
+    int split_dx, split_dw;   // of the FMA products
+    long long ws_dz, ws_part, ws_w, ws_x, ws_sum, total;
 
-// Splits of dw's sum over the rows: enough that its tiles fill the SMs, at
-// least 512 rows each.
-int dw_splits(const phyzb_linear_grad_args& a) {
-    const long long tiles = ((a.n + 127) / 128) * ((a.k + 63) / 64);
-    long long s = 444 / tiles, most = a.m / 512;
-    s = s < most ? s : most;
-    return (int)(s < 1 ? 1 : s > 128 ? 128 : s);
-}
-
-struct GradWs {
-    long long dz, part, dw, total;
+    static Operand w_of(const phyzb_linear_grad_args& a) {
+        return Operand(a.w, a.w_stride[1], a.w_stride[0], a.k, a.n, a.dtype);
+    }
+    static Operand x_of(const phyzb_linear_grad_args& a) {
+        return Operand(a.x, a.x_stride[1], a.x_stride[0], a.k, a.m, a.dtype);
+    }
+    explicit Backward(const phyzb_linear_grad_args& a) {
+        const bool f32 = a.dtype == PHYZB_DT_F32;
+        features = a.dy_stride[0] == 1 && a.dy_stride[1] != 1 && a.m > 1;
+        outer = features ? a.n : a.m;
+        inner = features ? a.m : a.n;
+        pitch = up(inner, 8);
+        plane = up(pitch * outer, 128);
+        blocks = features ? (inner + DZ_INNER - 1) / DZ_INNER : (outer + DZ_OUTER - 1) / DZ_OUTER;
+        // (both products of a layer have the same size: one way serves both)
+        simt_dx = simt_dw = f32 && simt_is_faster((double)a.m, (double)a.n, (double)a.k);
+        planes = f32 && !simt_dx ? 3 : 0;
+        const GemmMat dy{a.dy, a.dy_stride[0], a.dy_stride[1], 0}, dyt{a.dy, a.dy_stride[1], a.dy_stride[0], 0};
+        own_dz = a.activation != PHYZB_ACT_NONE || planes ||
+                 (!f32 && !(gemm_tma_ok(dy, a.m, a.n, 1) && gemm_tma_ok(dyt, a.n, a.m, 1)));
+        dx_rows_first = a.dx_stride[1] != 1 && a.dx_stride[0] == 1;
+        cut_dx = dx_rows_first ? cut_of(a.m, a.k, a.n, f32) : cut_of(a.k, a.m, a.n, f32);
+        cut_dw = cut_of(a.k, a.n, a.m, f32);
+        split_dx = simt_splits(a.m, a.k, a.n);
+        split_dw = simt_splits(a.n, a.k, a.m);
+        long long at = 0;
+        auto take = [&](long long bytes) {
+            const long long o = at;
+            at += up(bytes);
+            return o;
+        };
+        ws_dz = take(own_dz ? (planes ? 3 * plane * 2 : pitch * outer * esize(a.dtype)) : 0);
+        ws_part = take(a.dbias ? blocks * a.n * 4 : 0);
+        ws_w = take(a.dx && !simt_dx ? w_of(a).bytes : 0);
+        ws_x = take(a.dw && !simt_dw ? x_of(a).bytes : 0);
+        long long dxs = 0, dws = 0;
+        if (a.dx) dxs = simt_dx ? (split_dx > 1 ? split_dx * a.m * a.k * 4 : 0) : part_bytes(cut_dx, a.m, a.k);
+        if (a.dw) dws = simt_dw ? (split_dw > 1 ? split_dw * a.n * a.k * 4 : 0) : part_bytes(cut_dw, a.n, a.k);
+        ws_sum = take(dxs > dws ? dxs : dws);  // the products run one after the other
+        total = at;
+    }
 };
-GradWs grad_ws(const phyzb_linear_grad_args& a) {
-    GradWs w{};
-    long long at = 0;
-    w.dz = at;
-    at += up(a.m * a.n * esize(a.dtype));
-    w.part = at;
-    at += up((a.m + DZ_ROWS - 1) / DZ_ROWS * a.n * 4);
-    w.dw = at;
-    const int s = dw_splits(a);
-    if (s > 1) at += up((long long)s * a.n * a.k * 4);
-    w.total = at;
-    return w;
-}
 
 template <class T>
-cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t s) {
-    const GradWs w = grad_ws(a);
-    T* dz = (T*)(ws + w.dz);
-    float* part = (float*)(ws + w.part);
-    const unsigned nb = (unsigned)((a.n + 127) / 128);
-    const long long rb = (a.m + DZ_ROWS - 1) / DZ_ROWS;
-    if (a.m) dz_kernel<T><<<dim3(nb, (unsigned)rb), 128, 0, s>>>(a, dz, part);
-    if (a.dbias) column_sum_kernel<<<nb, 128, 0, s>>>(part, rb, a.n, a.dbias);
-    cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess && a.dx && a.m)
-        e = simt_gemm<T, T>({dz, a.n, 1, 0}, {a.w, a.w_stride[1], a.w_stride[0], 0}, a.m, a.k, a.n, 1, 1,
-                            StoreEpi<T>{{a.dx, a.dx_stride[0], a.dx_stride[1]}}, s);
-    if (e == cudaSuccess && a.dw) {
-        const GemmOperand A{dz, 1, a.n, 0}, B{a.x, a.x_stride[1], a.x_stride[0], 0};
-        const NnMat dw{a.dw, a.dw_stride[0], a.dw_stride[1]};
-        const int splits = dw_splits(a);
-        if (splits == 1) return simt_gemm<T, T>(A, B, a.n, a.k, a.m, 1, 1, StoreEpi<T>{dw}, s);
-        float* p = (float*)(ws + w.dw);
-        e = simt_gemm<T, T>(A, B, a.n, a.k, a.m, 1, splits, PartEpi{p, a.n, a.k}, s);
-        if (e != cudaSuccess) return e;
-        join_kernel<T><<<(unsigned)((a.n * a.k + 255) / 256), 256, 0, s>>>(p, splits, a.n, a.k, dw);
+cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st) {
+    const Out<T> dw{(T*)a.dw, a.dw_stride[1], a.dw_stride[0]};  // i = k
+    if (a.m == 0) {  // no rows: sums of nothing
+        if (a.dw) join_kernel<<<(unsigned)((a.n * a.k + 255) / 256), 256, 0, st>>>(nullptr, 0, a.k, a.n, StoreEpi<T>{dw, a.k});
+        if (a.dbias) column_sum_kernel<<<(unsigned)((a.n + 31) / 32), 256, 0, st>>>(nullptr, 0, a.n, a.dbias);
+        return cudaGetLastError();
+    }
+    const Backward p(a);
+    cudaError_t e = cudaSuccess;
+    if (p.own_dz || a.dbias) {
+        DzArgs d{};
+        d.dy = a.dy;
+        d.pre = a.pre;
+        d.dy_o = a.dy_stride[p.features ? 1 : 0];
+        d.dy_i = a.dy_stride[p.features ? 0 : 1];
+        d.pre_o = a.pre_stride[p.features ? 1 : 0];
+        d.pre_i = a.pre_stride[p.features ? 0 : 1];
+        d.outer = p.outer;
+        d.inner = p.inner;
+        d.pitch = p.pitch;
+        d.plane = p.plane;
+        d.dz = p.own_dz ? ws + p.ws_dz : nullptr;
+        d.part = a.dbias ? (float*)(ws + p.ws_part) : nullptr;
+        d.act = a.activation;
+        d.planes = p.planes;
+        constexpr int V = 16 / sizeof(T);
+        auto wide = [&](const void* q, long long os, long long is) {
+            return (uintptr_t)q % 16 == 0 && is == 1 && (p.outer == 1 || os % V == 0);
+        };
+        if (p.features) {
+            dz_features_kernel<T><<<dim3((unsigned)p.blocks, (unsigned)p.outer), 256, 0, st>>>(d);
+        } else if (p.inner % V == 0 && wide(d.dy, d.dy_o, d.dy_i) &&
+                   (a.activation == PHYZB_ACT_NONE || wide(d.pre, d.pre_o, d.pre_i))) {
+            dz_rows_kernel<T, V><<<dim3((unsigned)((p.inner + 32 * V - 1) / (32 * V)), (unsigned)p.blocks), 256, 0, st>>>(d);
+        } else {
+            dz_rows_kernel<T, 1><<<dim3((unsigned)((p.inner + 31) / 32), (unsigned)p.blocks), 256, 0, st>>>(d);
+        }
+        if (a.dbias)
+            column_sum_kernel<<<(unsigned)((a.n + 31) / 32), 256, 0, st>>>(d.part, p.blocks, a.n, a.dbias);
         e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+    }
+    // dz as rows x n
+    const long long zr = p.own_dz ? (p.features ? 1 : p.pitch) : a.dy_stride[0];
+    const long long zn = p.own_dz ? (p.features ? p.pitch : 1) : a.dy_stride[1];
+    const char* zp = p.own_dz ? ws + p.ws_dz : (const char*)a.dy;
+    GemmMat dz[3], dzt[3];
+    for (int k = 0; k < 3; k++) {
+        dz[k] = {zp + k * p.plane * 2, zr, zn, 0};
+        dzt[k] = {zp + k * p.plane * 2, zn, zr, 0};
+    }
+    char* const part = ws + p.ws_sum;
+    if (a.dx) {
+        const bool rf = p.dx_rows_first;
+        if constexpr (sizeof(T) == 4) {
+            if (p.simt_dx) {
+                e = simt_multiply({(const float*)zp, zr, zn}, {(const float*)a.w, a.w_stride[1], a.w_stride[0]}, a.m, a.k,
+                                  a.n, p.split_dx, rf, part,
+                                  StoreEpi<T>{{(T*)a.dx, a.dx_stride[0], a.dx_stride[1]}, a.m}, st);
+            }
+        }
+        if (!p.simt_dx) {
+            GemmMat w[3];
+            e = Backward::w_of(a).ready(ws + p.ws_w, w, st);
+            if (e != cudaSuccess) return e;
+            const StoreEpi<T> epi{{(T*)a.dx, a.dx_stride[rf ? 0 : 1], a.dx_stride[rf ? 1 : 0]}, rf ? a.m : a.k};
+            e = multiply<T>(rf ? dz : w, rf ? w : dz, rf ? a.m : a.k, rf ? a.k : a.m, a.n, p.cut_dx, part, epi, st);
+        }
+        if (e != cudaSuccess) return e;
+    }
+    if (a.dw) {
+        if constexpr (sizeof(T) == 4) {
+            if (p.simt_dw)
+                return simt_multiply({(const float*)zp, zn, zr}, {(const float*)a.x, a.x_stride[1], a.x_stride[0]}, a.n,
+                                     a.k, a.m, p.split_dw, false, part,
+                                     StoreEpi<T>{{(T*)a.dw, a.dw_stride[0], a.dw_stride[1]}, a.n}, st);
+        }
+        GemmMat x[3];
+        e = Backward::x_of(a).ready(ws + p.ws_x, x, st);
+        if (e != cudaSuccess) return e;
+        e = multiply<T>(x, dzt, a.k, a.n, a.m, p.cut_dw, part, StoreEpi<T>{dw, a.k}, st);
     }
     return e;
 }
 
-template <class T>
-cudaError_t forward(const phyzb_linear_args& a, cudaStream_t s) {
-    const LinearEpi<T> epi{a.bias,
-                           {(void*)a.residual, a.residual_stride[0], a.residual_stride[1]},
-                           {a.y, a.y_stride[0], a.y_stride[1]},
-                           {a.pre, a.pre_stride[0], a.pre_stride[1]},
-                           a.activation};
-    return simt_gemm<T, T>({a.x, a.x_stride[0], a.x_stride[1], 0}, {a.w, a.w_stride[0], a.w_stride[1], 0}, a.m, a.n,
-                           a.k, 1, 1, epi, s);
-}
-
 }  // namespace
 
-long long linear_workspace(const phyzb_linear_args&) { return 0; }
-long long linear_grad_workspace(const phyzb_linear_grad_args& a) { return grad_ws(a).total; }
+long long linear_workspace(const phyzb_linear_args& a) {
+    const Way way = way_of(a);
+    if (way == ROWS) return 0;
+    if (way == SIMT) {
+        const int s = simt_splits(a.m, a.n, a.k);
+        return s > 1 ? s * a.m * a.n * 4 : 0;
+    }
+    return Forward(a).total;
+}
+long long linear_grad_workspace(const phyzb_linear_grad_args& a) { return a.m ? Backward(a).total : 0; }
 
-cudaError_t linear_forward(const phyzb_linear_args& a, void*, cudaStream_t s) {
-    if (a.dtype == PHYZB_DT_F32) return forward<float>(a, s);
-    if (a.dtype == PHYZB_DT_BF16) return forward<__nv_bfloat16>(a, s);
-    return forward<__half>(a, s);
+cudaError_t linear_forward(const phyzb_linear_args& a, void* ws, cudaStream_t s) {
+    if (a.dtype == PHYZB_DT_F32) return forward<float>(a, (char*)ws, s);
+    if (a.dtype == PHYZB_DT_BF16) return forward<__nv_bfloat16>(a, (char*)ws, s);
+    return forward<__half>(a, (char*)ws, s);
 }
 
 cudaError_t linear_backward(const phyzb_linear_grad_args& a, void* ws, cudaStream_t s) {
@@ -156,5 +778,7 @@ cudaError_t linear_backward(const phyzb_linear_grad_args& a, void* ws, cudaStrea
     if (a.dtype == PHYZB_DT_BF16) return backward<__nv_bfloat16>(a, (char*)ws, s);
     return backward<__half>(a, (char*)ws, s);
 }
+
+cudaError_t linear_faults(unsigned int* n) { return cudaMemcpyFromSymbol(n, g_linear_fault, sizeof(*n)); }
 
 }  // namespace pz

@@ -29,15 +29,6 @@ namespace pz {
 
 namespace {
 
-// The sigmoid by the approximate exp2 and reciprocal (2 ulp and 1 ulp each):
-// within 2^-22 of itself near 1 and of e^z near 0; exactly 0 and 1 at the ends.
-__device__ __forceinline__ float gate_of(float z) {
-    float e, a;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.0f + e));
-    return a;
-}
-
 constexpr float DROP = -1.0f;  // A of a stretch that begins anew within itself
 
 // one more step (a, b) behind the stretch (A, B); drop: the state before the
@@ -80,7 +71,7 @@ __global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ phyzb
     for (int v = 0; v < V; v++) h[v] = hp ? hp[v * a.h0_stride[1]] : 0.0f;
 #pragma unroll
     for (int v = 0; v < V; v++) {
-        const float s = gate_of(to_f32(g[v]));
+        const float s = sigmoid_f32(to_f32(g[v]));
         const float u = (1.0f - s) * to_f32(x[v]);
         h[v] = rp && rp[v * a.reset_stride[2]] ? u : fmaf(s, h[v], u);
         y[v] = from_f32<T>(h[v]);
@@ -293,7 +284,7 @@ __global__ void __launch_bounds__(NT, (Lane<T, BWD, OUT>::BLOCKS)) lane_kernel(c
 #pragma unroll
                 for (int v = 0; v < S; v++) {
                     const int e = (BWD ? S - 1 - v : v) * NT;
-                    g[v] = gate_of(to_f32(in[e]));
+                    g[v] = sigmoid_f32(to_f32(in[e]));
                     x[v] = to_f32(in[BOX + e]);
                     if (!BWD) x[v] *= 1.0f - g[v];
                     if constexpr (NIN == 4) {
@@ -413,7 +404,7 @@ __global__ void __launch_bounds__(NT) loose_kernel(const __grid_constant__ Side 
         bool drop[L];
 #pragma unroll
         for (int u = 0; u < L; u++) {
-            g[u] = gate_of(to_f32(raw[0][u]));
+            g[u] = sigmoid_f32(to_f32(raw[0][u]));
             x[u] = to_f32(raw[1][u]);
             if (!BWD) x[u] *= 1.0f - g[u];
             drop[u] = RESET && drops[u];

@@ -1,39 +1,32 @@
-// Products on the FMA units: D[i][j] = sum_k A[i][k] B[j][k] in f32, for
-// operands of any type and strides, with the sum handed to an epilogue.
+// Products on the FMA units, for f32 layers too small for the tensor cores'
+// plane products: D[i][j] = sum_k A[i][k] B[j][k], operands of any strides.
 #pragma once
 
 #include "pz_nn.cuh"
 
 namespace pz {
 
-// Element (i, k) at p[i * is + k * ks], batch z at p + z * zs.
-struct GemmOperand {
-    const void* p = nullptr;
-    long long is = 0, ks = 0, zs = 0;
+// Element (i, k) at p[i * is + k * ks].
+struct SimtOperand {
+    const float* p = nullptr;
+    long long is = 0, ks = 0;
 };
 
 // 256 threads compute a 128 x 64 tile, 8 x 4 values each (two groups of four
 // rows 64 apart, four columns), from stages of 16 k in shared memory; the next
-// stage is loaded into registers while the current one is multiplied.
-// blockIdx = (tiles of i, tiles of j, batch or split). With `splits` > 1, z is
-// a split of the k range instead of a batch.
-template <class TA, class TB, class Epi>
-__global__ void __launch_bounds__(256) simt_gemm_kernel(GemmOperand A, GemmOperand B, long long M, long long N,
-                                                        long long K, int splits, Epi epi) {
+// stage is loaded into registers while the current one is multiplied. blockIdx
+// = (tiles of i, tiles of j, split of the k range). ALONG_I: D is contiguous in
+// i; lanes then run along i, and the epilogue gets four values along it.
+// Epi: void four(int split, long long i, long long j, const float* v, int n, bool along_i)
+template <bool ALONG_I, class Epi>
+__global__ void __launch_bounds__(256) simt_gemm_kernel(SimtOperand A, SimtOperand B, long long M, long long N,
+                                                        long long K, long long per, Epi epi) {
     constexpr int TM = 128, TN = 64, TK = 16;
     __shared__ __align__(16) float As[TK][TM + 4];
     __shared__ __align__(16) float Bs[TK][TN + 4];
     const long long i0 = (long long)blockIdx.x * TM, j0 = (long long)blockIdx.y * TN;
-    const long long z = blockIdx.z;
-    const TA* a = (const TA*)A.p + (splits > 1 ? 0 : z * A.zs);
-    const TB* b = (const TB*)B.p + (splits > 1 ? 0 : z * B.zs);
-    long long k0 = 0, k1 = K;
-    if (splits > 1) {
-        const long long per = (K + splits - 1) / splits;
-        k0 = z * per;
-        k1 = k0 + per < K ? k0 + per : K;
-    }
-    const int t = threadIdx.x, tj = t % 16, ti = t / 16;
+    const long long k0 = blockIdx.z * per, k1 = k0 + per < K ? k0 + per : K;
+    const int t = threadIdx.x, tj = ALONG_I ? t / 16 : t % 16, ti = ALONG_I ? t % 16 : t / 16;
     // consecutive threads walk the operand's unit stride
     const bool ak = A.ks == 1, bk = B.ks == 1;
     float acc[8][4] = {};
@@ -42,12 +35,12 @@ __global__ void __launch_bounds__(256) simt_gemm_kernel(GemmOperand A, GemmOpera
 #pragma unroll
         for (int u = 0; u < 8; u++) {
             const int e = t + u * 256, ii = ak ? e / TK : e % TM, kk = ak ? e % TK : e / TM;
-            ra[u] = i0 + ii < M && k + kk < k1 ? to_f32(a[(i0 + ii) * A.is + (k + kk) * A.ks]) : 0.0f;
+            ra[u] = i0 + ii < M && k + kk < k1 ? A.p[(i0 + ii) * A.is + (k + kk) * A.ks] : 0.0f;
         }
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             const int e = t + u * 256, jj = bk ? e / TK : e % TN, kk = bk ? e % TK : e / TN;
-            rb[u] = j0 + jj < N && k + kk < k1 ? to_f32(b[(j0 + jj) * B.is + (k + kk) * B.ks]) : 0.0f;
+            rb[u] = j0 + jj < N && k + kk < k1 ? B.p[(j0 + jj) * B.is + (k + kk) * B.ks] : 0.0f;
         }
     };
     if (k0 < k1) load(k0);
@@ -77,23 +70,36 @@ __global__ void __launch_bounds__(256) simt_gemm_kernel(GemmOperand A, GemmOpera
         }
         __syncthreads();
     }
+    auto left = [](long long n) { return n < 4 ? (int)n : 4; };
+    const long long jj = j0 + tj * 4;
+    if (ALONG_I) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const long long ii = i0 + (i / 4) * 64 + ti * 4 + i % 4;
-        if (ii >= M) continue;
+        for (int h = 0; h < 2; h++) {
+            const long long ii = i0 + h * 64 + ti * 4;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const long long jj = j0 + tj * 4 + j;
-            if (jj < N) epi(z, ii, jj, acc[i][j]);
+            for (int j = 0; j < 4; j++) {
+                const float v[4] = {acc[h * 4][j], acc[h * 4 + 1][j], acc[h * 4 + 2][j], acc[h * 4 + 3][j]};
+                if (ii < M && jj + j < N) epi.four(blockIdx.z, ii, jj + j, v, left(M - ii), true);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const long long ii = i0 + (i / 4) * 64 + ti * 4 + i % 4;
+            if (ii < M && jj < N) epi.four(blockIdx.z, ii, jj, acc[i], left(N - jj), false);
         }
     }
 }
 
-template <class TA, class TB, class Epi>
-cudaError_t simt_gemm(const GemmOperand& A, const GemmOperand& B, long long M, long long N, long long K, int batch,
-                      int splits, const Epi& epi, cudaStream_t s) {
-    const dim3 grid((unsigned)((M + 127) / 128), (unsigned)((N + 63) / 64), (unsigned)(splits > 1 ? splits : batch));
-    simt_gemm_kernel<TA, TB><<<grid, 256, 0, s>>>(A, B, M, N, K, splits, epi);
+template <class Epi>
+cudaError_t simt_gemm(const SimtOperand& A, const SimtOperand& B, long long M, long long N, long long K, int splits,
+                      bool along_i, const Epi& epi, cudaStream_t s) {
+    const dim3 grid((unsigned)((M + 127) / 128), (unsigned)((N + 63) / 64), (unsigned)splits);
+    const long long per = (K + splits - 1) / splits;
+    if (along_i)
+        simt_gemm_kernel<true><<<grid, 256, 0, s>>>(A, B, M, N, K, per, epi);
+    else
+        simt_gemm_kernel<false><<<grid, 256, 0, s>>>(A, B, M, N, K, per, epi);
     return cudaGetLastError();
 }
 
