@@ -3,8 +3,9 @@
 // Forward: one product with everything else in its epilogue. Backward: dz =
 // dy act'(z) and its column sums (db) in one pass, then dx = dz w and dw =
 // dz^T x, the long sum of dw over the rows cut into splits that fill the GPU.
-// A product computes D[i][j] with i the contiguous side of its result, so that
-// a warp's lanes read and write neighbours in the epilogue.
+// In the epilogue of a product D[i][j] a lane has 32 neighbours in j, a warp 32 in
+// i: j is the contiguous side of the result where a lane can take its neighbours
+// by 16 or 32 bytes, else i is.
 //
 // Three ways to multiply:
 //   rows_kernel       a few rows (serving): the weights go by once, on the FMA
@@ -109,32 +110,32 @@ struct LinearEpi {
     }
     __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, const float* sum) const {
         if (i >= m) return;
-        float r[32];
-        if (res.p) {  // (the residual may be y itself: all 32 are read before any is written)
-            const T* p = res.p + i * res.is + j0 * res.js;
+        T t[32];
+        // (the residual may be y itself: all 32 are read before any is written)
+        T r[32];
+        if (res.p) load32(res.p + i * res.is + j0 * res.js, res.js, cols, r);
+        float z[32];
+        if (bias && !by_i) {
+            load32(bias + j0, 1, cols, z);
 #pragma unroll
-            for (int c = 0; c < 32; c++) {
-                r[c] = c < cols ? to_f32(*p) : 0.0f;
-                p += res.js;
-            }
-        }
-        const float b = bias && by_i ? bias[i] : 0.0f;
-        T* py = y.p + i * y.is + j0 * y.js;
-        T* pp = pre.p + i * pre.is + j0 * pre.js;
+            for (int c = 0; c < 32; c++) z[c] += sum[c];
+        } else {
+            const float b = bias ? bias[i] : 0.0f;
 #pragma unroll
-        for (int c = 0; c < 32; c++) {
-            if (c >= cols) break;
-            float z = sum[c] + b;
-            if (bias && !by_i) z += bias[j0 + c];
-            if (pre.p) {
-                *pp = from_f32<T>(z);
-                pp += pre.js;
-            }
-            z = act_f32(z, act);
-            if (res.p) z += r[c];
-            *py = from_f32<T>(z);
-            py += y.js;
+            for (int c = 0; c < 32; c++) z[c] = sum[c] + b;
         }
+        if (pre.p) {
+#pragma unroll
+            for (int c = 0; c < 32; c++) t[c] = from_f32<T>(z[c]);
+            store32(pre.p + i * pre.is + j0 * pre.js, pre.js, cols, t);
+        }
+        with_act(act, [&](auto kind) {
+#pragma unroll
+            for (int c = 0; c < 32; c++) z[c] = act_f32(z[c], decltype(kind)::value);
+        });
+#pragma unroll
+        for (int c = 0; c < 32; c++) t[c] = from_f32<T>(res.p ? z[c] + to_f32(r[c]) : z[c]);
+        store32(y.p + i * y.is + j0 * y.js, y.js, cols, t);
     }
 };
 
@@ -150,36 +151,26 @@ struct StoreEpi {
     }
     __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, const float* v) const {
         if (i >= m) return;
-        T* p = out.p + i * out.is + j0 * out.js;
+        T t[32];
 #pragma unroll
-        for (int c = 0; c < 32; c++) {
-            if (c >= cols) break;
-            *p = from_f32<T>(v[c]);
-            p += out.js;
-        }
+        for (int c = 0; c < 32; c++) t[c] = from_f32<T>(v[c]);
+        store32(out.p + i * out.is + j0 * out.js, out.js, cols, t);
     }
 };
 
-// A split's part, [split][n][m] f32.
+// A split's part, [split][m][n] f32.
 struct PartEpi {
     float* part;
     long long m, n;
     __device__ __forceinline__ void four(int split, long long i, long long j, const float* v, int k, bool along_i) const {
-        store4(part + (split * n + j) * m + i, along_i ? 1 : m, k, v);
+        store4(part + (split * m + i) * n + j, along_i ? n : 1, k, v);
     }
     __device__ __forceinline__ void operator()(const GemmUnit& q, long long i, int j0, int cols, const float* v) const {
-        if (i >= m) return;
-        float* p = part + (q.split * n + j0) * m + i;
-#pragma unroll
-        for (int c = 0; c < 32; c++) {
-            if (c >= cols) break;
-            *p = v[c];
-            p += m;
-        }
+        if (i < m) store32(part + (q.split * m + i) * n + j0, 1, cols, v);
     }
 };
 
-// The parts in order, through the epilogue.
+// The parts in order, through the epilogue; threads along D's contiguous side.
 template <class Epi>
 __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, long long m, long long n, Epi epi) {
     const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -187,7 +178,7 @@ __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits
     float v = 0.0f;
 #pragma unroll 8
     for (int s = 0; s < splits; s++) v += part[s * m * n + e];
-    epi.one(e % m, e / m, v);
+    epi.one(e / n, e % n, v);
 }
 
 // ── operands ──────────────────────────────────────────────────────────────
@@ -345,7 +336,7 @@ template <class Epi>
 cudaError_t simt_multiply(const SimtOperand& a, const SimtOperand& b, long long rows, long long cols, long long k,
                           int splits, bool along_i, char* part, const Epi& epi, cudaStream_t st) {
     if (splits == 1) return simt_gemm(a, b, rows, cols, k, 1, along_i, epi, st);
-    const cudaError_t e = simt_gemm(a, b, rows, cols, k, splits, true, PartEpi{(float*)part, rows, cols}, st);
+    const cudaError_t e = simt_gemm(a, b, rows, cols, k, splits, false, PartEpi{(float*)part, rows, cols}, st);
     if (e != cudaSuccess) return e;
     join_kernel<<<(unsigned)((rows * cols + 255) / 256), 256, 0, st>>>((const float*)part, splits, rows, cols, epi);
     return cudaGetLastError();
@@ -414,7 +405,19 @@ Way way_of(const phyzb_linear_args& a) {
     return a.dtype == PHYZB_DT_F32 && simt_is_faster((double)a.m, (double)a.n, (double)a.k) ? SIMT : TENSOR;
 }
 
-// i is the side along which y is contiguous: the features, unless only the rows are.
+// Whether D's i should be the first index of a result [r][c] (see above).
+bool first_is_i(const void* p, const int64_t* stride, int e) {
+    auto wide = [&](int64_t other) { return (uintptr_t)p % 16 == 0 && other * e % 16 == 0; };
+    if (stride[1] == 1) return wide(stride[0]);
+    if (stride[0] == 1) return !wide(stride[1]);
+    return true;
+}
+
+// A tile is 128 along i: up to 64 rows are left to j, whose tiles can be 64.
+bool rows_are_i(long long m, const void* p, const int64_t* stride, int dtype) {
+    return m > 64 && first_is_i(p, stride, (int)esize(dtype));
+}
+
 struct Forward {
     bool rows_first;  // i = rows of x
     long long di, dj;
@@ -422,7 +425,7 @@ struct Forward {
     Cut cut;
     long long ws_x, ws_w, ws_part, total;
     explicit Forward(const phyzb_linear_args& a)
-        : rows_first(a.y_stride[1] != 1 && a.y_stride[0] == 1),
+        : rows_first(rows_are_i(a.m, a.y, a.y_stride, a.dtype)),
           di(rows_first ? a.m : a.n),
           dj(rows_first ? a.n : a.m),
           x(a.x, a.x_stride[0], a.x_stride[1], a.m, a.k, a.dtype),
@@ -495,7 +498,7 @@ struct DzArgs {
     float* part;
     int act, planes;
 };
-constexpr int DZ_OUTER = 64;    // outer lines of a block
+constexpr int DZ_OUTER = 128;   // outer lines of a block
 constexpr int DZ_INNER = 2048;  // inner values of a block, where it sums along them
 
 template <class T>
@@ -526,35 +529,39 @@ __global__ void __launch_bounds__(256) dz_rows_kernel(const __grid_constant__ Dz
     const long long i0 = ((long long)blockIdx.x * 32 + tx) * V;
     const long long o1 = (blockIdx.y + 1) * (long long)DZ_OUTER < a.outer ? (blockIdx.y + 1) * (long long)DZ_OUTER : a.outer;
     float sum[V] = {};
-    if (i0 < a.inner) {
+    with_act(a.act, [&](auto kind) {
+        if (i0 >= a.inner) return;
+        constexpr int ACT = decltype(kind)::value;
 #pragma unroll 4
         for (long long o = blockIdx.y * (long long)DZ_OUTER + ty; o < o1; o += 8) {
-            float v[V];
+            T d[V], z[V], out[V];
+            const T *pd = (const T*)a.dy + o * a.dy_o + i0 * a.dy_i, *pz = (const T*)a.pre + o * a.pre_o + i0 * a.pre_i;
             if constexpr (V > 1) {
-                T d[V], z[V], out[V];
-                *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>((const T*)a.dy + o * a.dy_o + i0);
-                if (a.act != PHYZB_ACT_NONE)
-                    *reinterpret_cast<uint4*>(z) = *reinterpret_cast<const uint4*>((const T*)a.pre + o * a.pre_o + i0);
-#pragma unroll
-                for (int e = 0; e < V; e++) {
-                    v[e] = to_f32(d[e]);
-                    if (a.act != PHYZB_ACT_NONE) v[e] *= act_grad_f32(to_f32(z[e]), a.act);
-                    out[e] = from_f32<T>(v[e]);
-                }
-                if (a.planes == 3) {
-#pragma unroll
-                    for (int e = 0; e < V; e++) dz_store<T>(a, o, i0 + e, v[e]);
-                } else if (a.dz) {
-                    *reinterpret_cast<uint4*>((T*)a.dz + o * a.pitch + i0) = *reinterpret_cast<const uint4*>(out);
-                }
+                *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(pd);
+                if (ACT != PHYZB_ACT_NONE) *reinterpret_cast<uint4*>(z) = *reinterpret_cast<const uint4*>(pz);
             } else {
-                v[0] = dz_value<T>(a, o, i0);
-                dz_store<T>(a, o, i0, v[0]);
+                d[0] = *pd;
+                if (ACT != PHYZB_ACT_NONE) z[0] = *pz;
             }
+            float v[V];
 #pragma unroll
-            for (int e = 0; e < V; e++) sum[e] += v[e];
+            for (int e = 0; e < V; e++) {
+                v[e] = to_f32(d[e]);
+                if (ACT != PHYZB_ACT_NONE) v[e] *= act_grad_f32(to_f32(z[e]), ACT);
+                sum[e] += v[e];
+                out[e] = from_f32<T>(v[e]);
+            }
+            if (!a.dz) continue;
+            if (sizeof(T) == 4 && a.planes == 3) {
+#pragma unroll
+                for (int e = 0; e < V; e++) dz_store<T>(a, o, i0 + e, v[e]);
+            } else if constexpr (V > 1) {
+                *reinterpret_cast<uint4*>((T*)a.dz + o * a.pitch + i0) = *reinterpret_cast<const uint4*>(out);
+            } else {
+                ((T*)a.dz)[o * a.pitch + i0] = out[0];
+            }
         }
-    }
+    });
     if (!a.part) return;
 #pragma unroll
     for (int e = 0; e < V; e++) sums[ty][tx * V + e] = sum[e];
@@ -621,6 +628,7 @@ struct Backward {
     int planes;               // of dz: 0 = T
     long long outer, inner, pitch, plane, blocks;
     bool dx_rows_first;       // dx: i = rows
+    bool dw_n_first;          // dw: i = n
     Cut cut_dx, cut_dw;
     int split_dx, split_dw;   // of the FMA products
     long long ws_dz, ws_part, ws_w, ws_x, ws_sum, total;
@@ -645,9 +653,10 @@ struct Backward {
         const GemmMat dy{a.dy, a.dy_stride[0], a.dy_stride[1], 0}, dyt{a.dy, a.dy_stride[1], a.dy_stride[0], 0};
         own_dz = a.activation != PHYZB_ACT_NONE || planes ||
                  (!f32 && !(gemm_tma_ok(dy, a.m, a.n, 1) && gemm_tma_ok(dyt, a.n, a.m, 1)));
-        dx_rows_first = a.dx_stride[1] != 1 && a.dx_stride[0] == 1;
+        dx_rows_first = rows_are_i(a.m, a.dx, a.dx_stride, a.dtype);
+        dw_n_first = first_is_i(a.dw, a.dw_stride, (int)esize(a.dtype));
         cut_dx = dx_rows_first ? cut_of(a.m, a.k, a.n, f32) : cut_of(a.k, a.m, a.n, f32);
-        cut_dw = cut_of(a.k, a.n, a.m, f32);
+        cut_dw = dw_n_first ? cut_of(a.n, a.k, a.m, f32) : cut_of(a.k, a.n, a.m, f32);
         split_dx = simt_splits(a.m, a.k, a.n);
         split_dw = simt_splits(a.n, a.k, a.m);
         long long at = 0;
@@ -670,9 +679,9 @@ struct Backward {
 
 template <class T>
 cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st) {
-    const Out<T> dw{(T*)a.dw, a.dw_stride[1], a.dw_stride[0]};  // i = k
+    const Out<T> dw{(T*)a.dw, a.dw_stride[0], a.dw_stride[1]};  // i = n
     if (a.m == 0) {  // no rows: sums of nothing
-        if (a.dw) join_kernel<<<(unsigned)((a.n * a.k + 255) / 256), 256, 0, st>>>(nullptr, 0, a.k, a.n, StoreEpi<T>{dw, a.k});
+        if (a.dw) join_kernel<<<(unsigned)((a.n * a.k + 255) / 256), 256, 0, st>>>(nullptr, 0, a.n, a.k, StoreEpi<T>{dw, a.n});
         if (a.dbias) column_sum_kernel<<<(unsigned)((a.n + 31) / 32), 256, 0, st>>>(nullptr, 0, a.n, a.dbias);
         return cudaGetLastError();
     }
@@ -744,12 +753,15 @@ cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st)
             if (p.simt_dw)
                 return simt_multiply({(const float*)zp, zn, zr}, {(const float*)a.x, a.x_stride[1], a.x_stride[0]}, a.n,
                                      a.k, a.m, p.split_dw, false, part,
-                                     StoreEpi<T>{{(T*)a.dw, a.dw_stride[0], a.dw_stride[1]}, a.n}, st);
+                                     StoreEpi<T>{dw, a.n}, st);
         }
         GemmMat x[3];
         e = Backward::x_of(a).ready(ws + p.ws_x, x, st);
         if (e != cudaSuccess) return e;
-        e = multiply<T>(x, dzt, a.k, a.n, a.m, p.cut_dw, part, StoreEpi<T>{dw, a.k}, st);
+        if (p.dw_n_first)
+            e = multiply<T>(dzt, x, a.n, a.k, a.m, p.cut_dw, part, StoreEpi<T>{dw, a.n}, st);
+        else
+            e = multiply<T>(x, dzt, a.k, a.n, a.m, p.cut_dw, part, StoreEpi<T>{{dw.p, dw.js, dw.is}, a.k}, st);
     }
     return e;
 }

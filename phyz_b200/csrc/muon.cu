@@ -20,7 +20,7 @@ namespace {
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f, NS_EPS = 1e-7f;
 constexpr float SCALE = 4096.0f;
-constexpr int NORM_BLOCKS = 64;  // partial sums of a matrix's |u|^2
+constexpr int NORM_BLOCKS = 512;  // partial sums of a matrix's |u|^2, at most
 
 __device__ unsigned int g_muon_fault;  // waits that ran out (pz_tma.cuh)
 
@@ -56,22 +56,10 @@ __device__ __forceinline__ float load_as(const void* p, long long e, int dtype) 
            : dtype == PHYZB_DT_BF16 ? __bfloat162float(((const __nv_bfloat16*)p)[e])
                                     : __half2float(((const __half*)p)[e]);
 }
-__device__ __forceinline__ void store_as(void* p, long long e, int dtype, float v) {
-    if (dtype == PHYZB_DT_F32)
-        ((float*)p)[e] = v;
-    else if (dtype == PHYZB_DT_BF16)
-        ((__nv_bfloat16*)p)[e] = __float2bfloat16_rn(v);
-    else
-        ((__half*)p)[e] = __float2half_rn(v);
-}
-
 // f16 pairs of a stack of matrices [batch][rows][pitch], at SCALE.
 struct Pair {
     __half* p = nullptr;
     long long lo = 0, zs = 0, pitch = 0;  // offset of the low plane; strides
-    __device__ __forceinline__ float get(long long e) const {
-        return __half2float(p[e]) + __half2float(p[e + lo]);
-    }
     __device__ __forceinline__ void put(long long e, float v) const {
         const __half h = __float2half_rn(v);
         p[e] = h;
@@ -79,29 +67,66 @@ struct Pair {
     }
 };
 
-// The direction at (z, r, c) from the advanced momentum.
-__device__ __forceinline__ float direction(const Problem& q, int z, long long r, long long c) {
-    const float g = load_as(q.g.p, z * q.g.zs + r * q.g.rs + c * q.g.cs, q.dtype);
-    if (!q.m.p) return g;
-    const float m = ((const float*)q.m.p)[z * q.m.zs + r * q.m.rs + c * q.m.cs];
-    return q.nesterov ? fmaf(q.mu, m, g) : m;
+// V neighbours of row r from column c: momentum advanced (ADVANCE) or as it is,
+// and the direction u from it.
+template <int V, bool ADVANCE>
+__device__ __forceinline__ void direction(const Problem& q, int z, int r, int c, float* u) {
+    const long long eg = z * q.g.zs + r * q.g.rs + c * q.g.cs;
+    if constexpr (V == 4) {
+        if (q.dtype == PHYZB_DT_F32) {
+            *(float4*)u = *(const float4*)((const float*)q.g.p + eg);
+        } else {
+            const uint2 w = *(const uint2*)((const uint16_t*)q.g.p + eg);
+            const uint16_t h[4] = {(uint16_t)w.x, (uint16_t)(w.x >> 16), (uint16_t)w.y, (uint16_t)(w.y >> 16)};
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+                u[v] = q.dtype == PHYZB_DT_BF16 ? __bfloat162float(*(const __nv_bfloat16*)&h[v])
+                                                : __half2float(*(const __half*)&h[v]);
+        }
+    } else {
+        u[0] = load_as(q.g.p, eg, q.dtype);
+    }
+    if (!q.m.p) return;
+    float* pm = (float*)q.m.p + z * q.m.zs + r * q.m.rs + c * q.m.cs;
+    float m[V];
+    if constexpr (V == 4)
+        *(float4*)m = *(const float4*)pm;
+    else
+        m[0] = *pm;
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+        if (ADVANCE) m[v] = fmaf(q.mu, m[v], u[v]);
+        u[v] = q.nesterov ? fmaf(q.mu, m[v], u[v]) : m[v];
+    }
+    if (!ADVANCE) return;
+    if constexpr (V == 4)
+        *(float4*)pm = *(const float4*)m;
+    else
+        *pm = m[0];
 }
 
-// Momentum advanced, and each block's sum of u^2 (rows r = block, block + 64, ..).
+// Stretches of 256 V columns of a row, one to a block at a time: f(row, column).
+template <int V, class F>
+__device__ __forceinline__ void each_stretch(const Problem& q, F f) {
+    const int per = (q.cols + 256 * V - 1) / (256 * V), n = per * q.rows;
+#pragma unroll 2
+    for (int i = blockIdx.x; i < n; i += gridDim.x) {
+        const int r = i / per, c = (i - r * per) * 256 * V + threadIdx.x * V;
+        if (c < q.cols) f(r, c);
+    }
+}
+
+// Momentum advanced, and each block's sum of u^2.
+template <int V>
 __global__ void __launch_bounds__(256) momentum_kernel(const __grid_constant__ Problem q, float* part) {
     const int z = blockIdx.y;
     float sum = 0.0f;
-    const long long n = (long long)q.rows * q.cols, per = (n + NORM_BLOCKS - 1) / NORM_BLOCKS;
-    const long long e0 = blockIdx.x * per, e1 = e0 + per < n ? e0 + per : n;
-    for (long long e = e0 + threadIdx.x; e < e1; e += 256) {
-        const int r = (int)e / q.cols, c = (int)e - r * q.cols;  // (at most 2^28 elements)
-        if (q.m.p) {
-            float* m = (float*)q.m.p + z * q.m.zs + r * q.m.rs + c * q.m.cs;
-            *m = fmaf(q.mu, *m, load_as(q.g.p, z * q.g.zs + r * q.g.rs + c * q.g.cs, q.dtype));
-        }
-        const float u = direction(q, z, r, c);
-        sum = fmaf(u, u, sum);
-    }
+    each_stretch<V>(q, [&](int r, int c) {
+        float u[V];
+        direction<V, true>(q, z, r, c, u);
+#pragma unroll
+        for (int v = 0; v < V; v++) sum = fmaf(u[v], u[v], sum);
+    });
     __shared__ float sm[8];
 #pragma unroll
     for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -115,26 +140,60 @@ __global__ void __launch_bounds__(256) momentum_kernel(const __grid_constant__ P
     }
 }
 
-// 1 / (|u| + eps) from the blocks' sums, the same in every thread of a warp.
-__device__ __forceinline__ float inverse_norm(const float* part, int z) {
-    const int lane = threadIdx.x % 32;
-    float s = part[z * NORM_BLOCKS + lane] + part[z * NORM_BLOCKS + 32 + lane];
+// 1 / (|u| + eps) from `blocks` sums, the same in every thread of a warp.
+__device__ __forceinline__ float inverse_norm(const float* part, int z, int blocks) {
+    float s = 0.0f;
+#pragma unroll 4
+    for (int k = threadIdx.x % 32; k < blocks; k += 32) s += part[z * NORM_BLOCKS + k];
 #pragma unroll
     for (int o = 16; o; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
     return 1.0f / (sqrtf(s) + NS_EPS);
 }
 
+template <int V>
 __global__ void __launch_bounds__(256) normalize_kernel(const __grid_constant__ Problem q, const float* part, Pair x) {
     const int z = blockIdx.y;
-    const float k = inverse_norm(part, z) * SCALE;
-    const long long n = (long long)q.rows * q.cols;
-    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long long)gridDim.x * 256) {
-        const int r = (int)e / q.cols, c = (int)e - r * q.cols;
-        x.put(z * x.zs + r * x.pitch + c, direction(q, z, r, c) * k);
-    }
+    const float k = inverse_norm(part, z, gridDim.x) * SCALE;
+    each_stretch<V>(q, [&](int r, int c) {
+        float u[V];
+        direction<V, false>(q, z, r, c, u);
+        __half h[V], l[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            h[v] = __float2half_rn(u[v] * k);
+            l[v] = __float2half_rn(u[v] * k - __half2float(h[v]));
+        }
+        __half* p = x.p + z * x.zs + r * x.pitch + c;
+        if constexpr (V == 4) {
+            *(uint2*)p = *(const uint2*)h;
+            *(uint2*)(p + x.lo) = *(const uint2*)l;
+        } else {
+            p[0] = h[0];
+            p[x.lo] = l[0];
+        }
+    });
 }
 
 // ── epilogues: D is at SCALE^2 ────────────────────────────────────────────
+
+// 32 neighbours of a pair's row
+__device__ __forceinline__ void pair_load(const Pair& x, long long e, int n, float* v) {
+    __half h[32], l[32];
+    load32(x.p + e, 1, n, h);
+    load32(x.p + x.lo + e, 1, n, l);
+#pragma unroll
+    for (int k = 0; k < 32; k++) v[k] = __half2float(h[k]) + __half2float(l[k]);
+}
+__device__ __forceinline__ void pair_store(const Pair& x, long long e, int n, const float* v) {
+    __half h[32], l[32];
+#pragma unroll
+    for (int k = 0; k < 32; k++) {
+        h[k] = __float2half_rn(v[k]);
+        l[k] = __float2half_rn(v[k] - __half2float(h[k]));
+    }
+    store32(x.p + e, 1, n, h);
+    store32(x.p + x.lo + e, 1, n, l);
+}
 
 // G = sum, or b G + c sum, and its mirror image: D[i][j] = D[j][i].
 struct SquareEpi {
@@ -143,40 +202,33 @@ struct SquareEpi {
     int s;
     __device__ __forceinline__ void operator()(const GemmUnit& q, long long i, int j0, int cols, const float* sum) const {
         if (i >= s) return;
-        const long long z = q.z * out.zs;
-        // the tile's mirror image, unless it is inside a diagonal block
-        const bool mirror = j0 < q.i * GEMM_BM;
+        const long long z = q.z * out.zs, e = z + i * out.pitch + j0;
         float v[32];
-        if (g.p) {
+        if (g.p) pair_load(g, e, cols, v);
 #pragma unroll
-            for (int k = 0; k < 32; k++) v[k] = k < cols ? g.get(z + (j0 + k) * g.pitch + i) : 0.0f;
-        }
-#pragma unroll
-        for (int k = 0; k < 32; k++) {
-            v[k] = g.p ? fmaf(b, v[k], c * sum[k]) : c * sum[k];
-            if (k < cols) out.put(z + (j0 + k) * out.pitch + i, v[k]);
-        }
-        if (mirror) {
+        for (int k = 0; k < 32; k++) v[k] = g.p ? fmaf(b, v[k], c * sum[k]) : c * sum[k];
+        pair_store(out, e, cols, v);
+        // the tile's mirror image, unless it is inside a diagonal block
+        if (j0 < q.i * GEMM_BM) {
 #pragma unroll
             for (int k = 0; k < 32; k++)
-                if (k < cols) out.put(z + i * out.pitch + j0 + k, v[k]);
+                if (k < cols) out.put(z + (j0 + k) * out.pitch + i, v[k]);
         }
     }
 };
 
-// a X + sum; i along the columns of X, j along its rows.
+// a X + sum; i along the rows of X, j along its columns.
 struct StepEpi {
     Pair x, out;
-    int cols_;
+    int rows;
     __device__ __forceinline__ void operator()(const GemmUnit& q, long long i, int j0, int cols, const float* sum) const {
-        if (i >= cols_) return;
-        const long long e = q.z * x.zs + j0 * x.pitch + i;
+        if (i >= rows) return;
+        const long long e = q.z * x.zs + i * x.pitch + j0;
         float v[32];
+        pair_load(x, e, cols, v);
 #pragma unroll
-        for (int k = 0; k < 32; k++) v[k] = k < cols ? x.get(e + k * x.pitch) : 0.0f;
-#pragma unroll
-        for (int k = 0; k < 32; k++)
-            if (k < cols) out.put(e + k * x.pitch, fmaf(NS_A, v[k], sum[k] * (1.0f / SCALE)));
+        for (int k = 0; k < 32; k++) v[k] = fmaf(NS_A, v[k], sum[k] * (1.0f / SCALE));
+        pair_store(out, e, cols, v);
     }
 };
 
@@ -184,32 +236,34 @@ struct StepEpi {
 struct LastEpi {
     Pair x;
     Problem q;
-    __device__ __forceinline__ void operator()(const GemmUnit& u, long long i, int j0, int cols, const float* sum) const {
-        if (i >= q.cols) return;
-        const long long z = u.z, e = z * x.zs + j0 * x.pitch + i;
-        float v[32];
+    template <class T>
+    __device__ __forceinline__ static void write(const View& o, long long z, long long i, int j0, int cols,
+                                                 const float* v) {
+        T t[32];
 #pragma unroll
-        for (int k = 0; k < 32; k++) v[k] = k < cols ? x.get(e + k * x.pitch) : 0.0f;
+        for (int k = 0; k < 32; k++) t[k] = from_f32<T>(v[k]);
+        store32((T*)o.p + z * o.zs + i * o.rs + j0 * o.cs, o.cs, cols, t);
+    }
+    __device__ __forceinline__ static void write(const View& o, int dtype, long long z, long long i, int j0, int cols,
+                                                 const float* v) {
+        if (dtype == PHYZB_DT_F32) return write<float>(o, z, i, j0, cols, v);
+        if (dtype == PHYZB_DT_BF16) return write<__nv_bfloat16>(o, z, i, j0, cols, v);
+        return write<__half>(o, z, i, j0, cols, v);
+    }
+    __device__ __forceinline__ void operator()(const GemmUnit& u, long long i, int j0, int cols, const float* sum) const {
+        if (i >= q.rows) return;
+        float v[32];
+        pair_load(x, u.z * x.zs + i * x.pitch + j0, cols, v);
 #pragma unroll
         for (int k = 0; k < 32; k++) v[k] = fmaf(NS_A, v[k], sum[k] * (1.0f / SCALE)) * (1.0f / SCALE);
-        if (q.out.p) {
-#pragma unroll
-            for (int k = 0; k < 32; k++)
-                if (k < cols) store_as(q.out.p, z * q.out.zs + (j0 + k) * q.out.rs + i * q.out.cs, q.out_dtype, v[k]);
-            return;
-        }
-        float* w = (float*)q.w.p + z * q.w.zs + j0 * q.w.rs + i * q.w.cs;
+        if (q.out.p) return write(q.out, q.out_dtype, u.z, i, j0, cols, v);
         float old[32];
+        float* w = (float*)q.w.p + u.z * q.w.zs + i * q.w.rs + j0 * q.w.cs;
+        load32(w, q.w.cs, cols, old);
 #pragma unroll
-        for (int k = 0; k < 32; k++) old[k] = k < cols ? w[k * q.w.rs] : 0.0f;
-#pragma unroll
-        for (int k = 0; k < 32; k++) {
-            if (k >= cols) break;
-            const float t = fmaf(-q.lr, v[k], q.decay * old[k]);
-            w[k * q.w.rs] = t;
-            if (q.copy.p)
-                store_as(q.copy.p, z * q.copy.zs + (j0 + k) * q.copy.rs + i * q.copy.cs, q.copy_dtype, t);
-        }
+        for (int k = 0; k < 32; k++) v[k] = fmaf(-q.lr, v[k], q.decay * old[k]);
+        store32(w, q.w.cs, cols, v);
+        if (q.copy.p) write(q.copy, q.copy_dtype, u.z, i, j0, cols, v);
     }
 };
 
@@ -226,7 +280,7 @@ Ws layout(long long batch, long long rows, long long cols) {
     const long long s = rows < cols ? rows : cols;
     long long at = 0;
     auto take = [&](Pair& p, long long r, long long c) {
-        p.pitch = up(c, 8);
+        p.pitch = up(c, 16);
         p.zs = r * p.pitch;
         p.lo = up(batch * p.zs, 128);
         const long long o = at;
@@ -270,10 +324,20 @@ cudaError_t solve(const Problem& q, char* ws, cudaStream_t st) {
     float* part = (float*)(ws + o.part_at);
     const bool tall = q.rows > q.cols;
     const int s = tall ? q.cols : q.rows, l = tall ? q.rows : q.cols;
-    const long long n = (long long)q.rows * q.cols;
-    momentum_kernel<<<dim3(NORM_BLOCKS, (unsigned)q.batch), 256, 0, st>>>(q, part);
-    const long long blocks = (n + 1023) / 1024;
-    normalize_kernel<<<dim3((unsigned)(blocks < 1024 ? blocks : 1024), (unsigned)q.batch), 256, 0, st>>>(q, part, o.x);
+    auto wide = [&](const View& v, int e) {
+        return !v.p || ((uintptr_t)v.p % (4 * e) == 0 && v.cs == 1 && v.rs % 4 == 0 && v.zs % 4 == 0);
+    };
+    const bool by4 = q.cols % 4 == 0 && wide(q.g, q.dtype == PHYZB_DT_F32 ? 4 : 2) && wide(q.m, 4);
+    // blocks of a few stretches, at most NORM_BLOCKS
+    const long long stretches = q.rows * ((q.cols + (by4 ? 1023 : 255)) / (by4 ? 1024 : 256));
+    const dim3 grid((unsigned)(stretches < NORM_BLOCKS ? stretches : NORM_BLOCKS), (unsigned)q.batch);
+    if (by4) {
+        momentum_kernel<4><<<grid, 256, 0, st>>>(q, part);
+        normalize_kernel<4><<<grid, 256, 0, st>>>(q, part, o.x);
+    } else {
+        momentum_kernel<1><<<grid, 256, 0, st>>>(q, part);
+        normalize_kernel<1><<<grid, 256, 0, st>>>(q, part, o.x);
+    }
     cudaError_t e = cudaGetLastError();
     Pair x = o.x, y = o.y;
     for (int k = 0; k < q.steps && e == cudaSuccess; k++) {
@@ -282,12 +346,12 @@ cudaError_t solve(const Problem& q, char* ws, cudaStream_t st) {
         if (e != cudaSuccess) break;
         e = multiply(o.g, false, o.g, false, s, s, s, q.batch, true, SquareEpi{o.p, o.g, NS_B, NS_C / SCALE, s}, fault, st);
         if (e != cudaSuccess) break;
-        // i = columns of X. Wide: X^T's rows by P's; tall: P's rows by X's
-        const Pair &a = tall ? o.p : x, &b = tall ? x : o.p;
+        // i = rows of X, j = columns. Wide: P's rows by X^T's; tall: X's rows by P's
+        const Pair &a = tall ? x : o.p, &b = tall ? o.p : x;
         if (k + 1 < q.steps)
-            e = multiply(a, !tall, b, false, q.cols, q.rows, s, q.batch, false, StepEpi{x, y, q.cols}, fault, st);
+            e = multiply(a, false, b, !tall, q.rows, q.cols, s, q.batch, false, StepEpi{x, y, q.rows}, fault, st);
         else
-            e = multiply(a, !tall, b, false, q.cols, q.rows, s, q.batch, false, LastEpi{x, q}, fault, st);
+            e = multiply(a, false, b, !tall, q.rows, q.cols, s, q.batch, false, LastEpi{x, q}, fault, st);
         const Pair t = x;
         x = y;
         y = t;

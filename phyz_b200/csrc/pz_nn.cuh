@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "pz_nn.h"
 
 namespace pz {
@@ -26,6 +28,68 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) {
     return __float2half_rn(x);
+}
+
+// 32 neighbours of an array whose elements are `stride` apart, n of them there
+// (the others read 0 and are not written): by 32 or 16 bytes a time where they are
+// contiguous and aligned.
+__device__ __forceinline__ void load32b(const void* p, uint32_t* r) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "l"(p)
+                 : "memory");
+}
+__device__ __forceinline__ void store32b(void* p, const uint32_t* r) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+template <class T>
+__device__ __forceinline__ void load32(const T* p, long long stride, int n, T* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    constexpr int W = 8 * sizeof(T);  // words in all
+    if (stride == 1 && n == 32 && ((uintptr_t)p & 31) == 0) {
+#pragma unroll
+        for (int w = 0; w < W; w += 8) load32b((const uint32_t*)p + w, r + w);
+    } else if (stride == 1 && n == 32 && ((uintptr_t)p & 15) == 0) {
+#pragma unroll
+        for (int w = 0; w < W; w += 4) {
+            const uint4 q = *reinterpret_cast<const uint4*>((const uint32_t*)p + w);
+            r[w] = q.x, r[w + 1] = q.y, r[w + 2] = q.z, r[w + 3] = q.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 32; e++) v[e] = e < n ? p[e * stride] : from_f32<T>(0.0f);
+    }
+}
+template <class T>
+__device__ __forceinline__ void store32(T* p, long long stride, int n, const T* v) {
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+    constexpr int W = 8 * sizeof(T);
+    if (stride == 1 && n == 32 && ((uintptr_t)p & 31) == 0) {
+#pragma unroll
+        for (int w = 0; w < W; w += 8) store32b((uint32_t*)p + w, r + w);
+    } else if (stride == 1 && n == 32 && ((uintptr_t)p & 15) == 0) {
+#pragma unroll
+        for (int w = 0; w < W; w += 4)
+            *reinterpret_cast<uint4*>((uint32_t*)p + w) = make_uint4(r[w], r[w + 1], r[w + 2], r[w + 3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 32; e++)
+            if (e < n) p[e * stride] = v[e];
+    }
+}
+
+// f with the activation as a constant
+template <class F>
+__device__ __forceinline__ void with_act(int act, F f) {
+    switch (act) {
+        case PHYZB_ACT_RELU: return f(std::integral_constant<int, PHYZB_ACT_RELU>());
+        case PHYZB_ACT_TANH: return f(std::integral_constant<int, PHYZB_ACT_TANH>());
+        case PHYZB_ACT_SILU: return f(std::integral_constant<int, PHYZB_ACT_SILU>());
+        case PHYZB_ACT_GELU: return f(std::integral_constant<int, PHYZB_ACT_GELU>());
+        default: return f(std::integral_constant<int, PHYZB_ACT_NONE>());
+    }
 }
 
 // The sigmoid by the approximate exp2 and reciprocal (2 ulp and 1 ulp each):
