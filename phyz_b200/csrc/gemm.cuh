@@ -121,8 +121,11 @@ __device__ __forceinline__ GemmUnit gemm_unit(const GemmArgs& g, int u) {
         q.i = i;
         q.j = t - W * i * (i + 1) / 2;
     } else {
-        q.i = t % g.ti;
-        q.j = t / g.ti;
+        // the side with fewer tiles first: the other operand's tile is then read by
+        // neighbours at the same time, and comes from memory once
+        const bool i_first = g.ti <= g.tj;
+        q.i = i_first ? t % g.ti : t / g.tj;
+        q.j = i_first ? t / g.ti : t % g.tj;
     }
     q.split = r % g.splits;
     q.z = r / g.splits;

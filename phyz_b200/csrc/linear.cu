@@ -497,8 +497,9 @@ struct DzArgs {
     void* dz;
     float* part;
     int act, planes;
+    int lines;  // outer lines of a block
 };
-constexpr int DZ_OUTER = 128;   // outer lines of a block
+constexpr int DZ_OUTER = 128;   // outer lines of a block, at most
 constexpr int DZ_INNER = 2048;  // inner values of a block, where it sums along them
 
 template <class T>
@@ -527,13 +528,13 @@ __global__ void __launch_bounds__(256) dz_rows_kernel(const __grid_constant__ Dz
     __shared__ float sums[8][32 * V];
     const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
     const long long i0 = ((long long)blockIdx.x * 32 + tx) * V;
-    const long long o1 = (blockIdx.y + 1) * (long long)DZ_OUTER < a.outer ? (blockIdx.y + 1) * (long long)DZ_OUTER : a.outer;
+    const long long o0 = blockIdx.y * (long long)a.lines, o1 = o0 + a.lines < a.outer ? o0 + a.lines : a.outer;
     float sum[V] = {};
     with_act(a.act, [&](auto kind) {
         if (i0 >= a.inner) return;
         constexpr int ACT = decltype(kind)::value;
 #pragma unroll 4
-        for (long long o = blockIdx.y * (long long)DZ_OUTER + ty; o < o1; o += 8) {
+        for (long long o = o0 + ty; o < o1; o += 8) {
             T d[V], z[V], out[V];
             const T *pd = (const T*)a.dy + o * a.dy_o + i0 * a.dy_i, *pz = (const T*)a.pre + o * a.pre_o + i0 * a.pre_i;
             if constexpr (V > 1) {
@@ -602,23 +603,22 @@ __global__ void __launch_bounds__(256) dz_features_kernel(const __grid_constant_
     }
 }
 
-// out[j] = sum over the blocks of part[block][j]: 8 warps take every 8th block.
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* part, long long blocks, long long n, float* out) {
-    __shared__ float sums[8][32];
+// out[j] = sum over the blocks of part[block][j]: 32 warps take every 32nd block.
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* part, long long blocks, long long n, float* out) {
+    __shared__ float sums[32][33];
     const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
     const long long j = (long long)blockIdx.x * 32 + tx;
     float v = 0.0f;
     if (j < n) {
 #pragma unroll 8
-        for (long long r = ty; r < blocks; r += 8) v += part[r * n + j];
+        for (long long r = ty; r < blocks; r += 32) v += part[r * n + j];
     }
     sums[ty][tx] = v;
     __syncthreads();
-    if (ty == 0 && j < n) {
+    v = sums[tx][ty];  // warp ty finishes column ty
 #pragma unroll
-        for (int r = 1; r < 8; r++) v += sums[r][tx];
-        out[j] = v;
-    }
+    for (int o = 16; o; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (tx == 0 && (long long)blockIdx.x * 32 + ty < n) out[(long long)blockIdx.x * 32 + ty] = v;
 }
 
 struct Backward {
@@ -626,6 +626,7 @@ struct Backward {
     bool simt_dx, simt_dw;    // f32 on the FMA units
     bool own_dz;              // dz is written (else dy is used as it is)
     int planes;               // of dz: 0 = T
+    int lines;                // of a dz_rows_kernel block
     long long outer, inner, pitch, plane, blocks;
     bool dx_rows_first;       // dx: i = rows
     bool dw_n_first;          // dw: i = n
@@ -646,7 +647,10 @@ struct Backward {
         inner = features ? a.m : a.n;
         pitch = up(inner, 8);
         plane = up(pitch * outer, 128);
-        blocks = features ? (inner + DZ_INNER - 1) / DZ_INNER : (outer + DZ_OUTER - 1) / DZ_OUTER;
+        // fewer lines to a block while blocks are fewer than four per SM
+        lines = DZ_OUTER;
+        while (lines > 16 && (outer + lines - 1) / lines * ((inner + 255) / 256) < 4 * GEMM_SMS) lines /= 2;
+        blocks = features ? (inner + DZ_INNER - 1) / DZ_INNER : (outer + lines - 1) / lines;
         // (both products of a layer have the same size: one way serves both)
         simt_dx = simt_dw = f32 && simt_is_faster((double)a.m, (double)a.n, (double)a.k);
         planes = f32 && !simt_dx ? 3 : 0;
@@ -682,7 +686,7 @@ cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st)
     const Out<T> dw{(T*)a.dw, a.dw_stride[0], a.dw_stride[1]};  // i = n
     if (a.m == 0) {  // no rows: sums of nothing
         if (a.dw) join_kernel<<<(unsigned)((a.n * a.k + 255) / 256), 256, 0, st>>>(nullptr, 0, a.n, a.k, StoreEpi<T>{dw, a.n});
-        if (a.dbias) column_sum_kernel<<<(unsigned)((a.n + 31) / 32), 256, 0, st>>>(nullptr, 0, a.n, a.dbias);
+        if (a.dbias) column_sum_kernel<<<(unsigned)((a.n + 31) / 32), 1024, 0, st>>>(nullptr, 0, a.n, a.dbias);
         return cudaGetLastError();
     }
     const Backward p(a);
@@ -703,6 +707,7 @@ cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st)
         d.part = a.dbias ? (float*)(ws + p.ws_part) : nullptr;
         d.act = a.activation;
         d.planes = p.planes;
+        d.lines = p.lines;
         constexpr int V = 16 / sizeof(T);
         auto wide = [&](const void* q, long long os, long long is) {
             return (uintptr_t)q % 16 == 0 && is == 1 && (p.outer == 1 || os % V == 0);
@@ -716,7 +721,7 @@ cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st)
             dz_rows_kernel<T, 1><<<dim3((unsigned)((p.inner + 31) / 32), (unsigned)p.blocks), 256, 0, st>>>(d);
         }
         if (a.dbias)
-            column_sum_kernel<<<(unsigned)((a.n + 31) / 32), 256, 0, st>>>(d.part, p.blocks, a.n, a.dbias);
+            column_sum_kernel<<<(unsigned)((a.n + 31) / 32), 1024, 0, st>>>(d.part, p.blocks, a.n, a.dbias);
         e = cudaGetLastError();
         if (e != cudaSuccess) return e;
     }

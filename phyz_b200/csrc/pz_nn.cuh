@@ -92,34 +92,40 @@ __device__ __forceinline__ void with_act(int act, F f) {
     }
 }
 
-// The sigmoid by the approximate exp2 and reciprocal (2 ulp and 1 ulp each):
-// within 2^-22 of itself near 1 and of e^z near 0; exactly 0 and 1 at the ends.
-__device__ __forceinline__ float sigmoid_f32(float z) {
+// sigmoid(z / log2 e) by the approximate exp2 and reciprocal (2 ulp and 1 ulp
+// each); exactly 0 and 1 at the ends.
+__device__ __forceinline__ float sigmoid2_f32(float z) {
     float e, a;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-z));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.0f + e));
     return a;
 }
+constexpr float LOG2E = 1.4426950408889634f;
+// within 2^-22 of the sigmoid near 1 and of e^z near 0
+__device__ __forceinline__ float sigmoid_f32(float z) { return sigmoid2_f32(z * LOG2E); }
 
 // tanh z = 2 sigmoid(2z) - 1; below 1/8, where that cancels, its series to z^7
 // (the next term is under 2^-29 of it).
 __device__ __forceinline__ float tanh_f32(float z) {
     const float q = z * z;
     const float s = z * fmaf(q, fmaf(q, fmaf(q, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-    const float t = fmaf(2.0f, sigmoid_f32(2.0f * z), -1.0f);
+    const float t = fmaf(2.0f, sigmoid2_f32(z * (2.0f * LOG2E)), -1.0f);
     return fabsf(z) < 0.125f ? s : t;
 }
 
 constexpr float GELU_C = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float GELU_K = 0.044715f;
+// gelu(z) = z (1 + tanh u) / 2 = z sigmoid(2u), u = C (z + K z^3)
+__device__ __forceinline__ float gelu_gate(float z, float q) {
+    return sigmoid2_f32(z * fmaf(q, 2.0f * LOG2E * GELU_C * GELU_K, 2.0f * LOG2E * GELU_C));
+}
 
 __device__ __forceinline__ float act_f32(float z, int act) {
     switch (act) {
         case PHYZB_ACT_RELU: return z > 0.0f || z != z ? z : 0.0f;
         case PHYZB_ACT_TANH: return tanh_f32(z);
         case PHYZB_ACT_SILU: return z * sigmoid_f32(z);
-        // z (1 + tanh u) / 2 = z sigmoid(2u)
-        case PHYZB_ACT_GELU: return z * sigmoid_f32(2.0f * GELU_C * (z + GELU_K * z * z * z));
+        case PHYZB_ACT_GELU: return z * gelu_gate(z, z * z);
         default: return z;
     }
 }
@@ -130,15 +136,15 @@ __device__ __forceinline__ float act_grad_f32(float z, int act) {
         case PHYZB_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
         case PHYZB_ACT_TANH: {
             const float t = tanh_f32(z);
-            return 1.0f - t * t;
+            return fmaf(-t, t, 1.0f);
         }
         case PHYZB_ACT_SILU: {
             const float s = sigmoid_f32(z);
-            return s * (1.0f + z * (1.0f - s));
+            return fmaf(fmaf(-s, s, s), z, s);
         }
         case PHYZB_ACT_GELU: {
-            const float s = sigmoid_f32(2.0f * GELU_C * (z + GELU_K * z * z * z));
-            return s + z * s * (1.0f - s) * 2.0f * GELU_C * (1.0f + 3.0f * GELU_K * z * z);
+            const float q = z * z, s = gelu_gate(z, q);
+            return fmaf(fmaf(-s, s, s), z * fmaf(q, 6.0f * GELU_C * GELU_K, 2.0f * GELU_C), s);
         }
         default: return 1.0f;
     }
