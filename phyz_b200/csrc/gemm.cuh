@@ -1,12 +1,17 @@
 // Products on the tensor cores: D[i][j] = sum_k A[i][k] B[j][k], f32 sums, for
 // bf16 or f16 operands in either order (k contiguous, or i / j contiguous).
 //
-// One persistent block per SM walks 128 x BN tiles of D. Warp 0 brings 64-deep
-// stages of both operands by TMA into 128-byte-swizzled shared memory, warp 1
-// issues tcgen05.mma into one of two accumulators in Tensor Memory, and eight
-// more warps empty the other one through the epilogue, so that the tensor cores
-// wait neither for memory nor for the epilogue. The lanes of an epilogue warp
-// are neighbours in i: the caller makes i the contiguous side of D.
+// One persistent block per SM walks tiles of D. Warp 0 brings 64-deep stages of
+// both operands by TMA into 128-byte-swizzled shared memory, warp 1 issues
+// tcgen05.mma into one of two accumulators in Tensor Memory, and eight more warps
+// empty the other one through the epilogue, so that the tensor cores wait neither
+// for memory nor for the epilogue. In the epilogue a lane has 32 neighbours in j
+// and a warp 32 in i.
+//
+// CTAS = 2: the two blocks of a cluster (the SMs of a pair) make one tile of 256 x
+// BN: each brings its 128 rows of A and half of B's, one mma reads both shared
+// memories, and each gets its rows' sums. A tile of 128 x 256 alone takes 96 bytes
+// a clock from L2 for every SM, more than it gives; the pair's takes 64.
 //
 // PL > 1: each operand is PL 16-bit planes whose sum is the value, and D is the
 // sum of the plane products that matter: two planes hi hi + (hi lo + lo hi);
@@ -29,16 +34,18 @@ constexpr int GEMM_EPI_WARPS = 8;
 constexpr int GEMM_THREADS = 32 * (2 + GEMM_EPI_WARPS);
 constexpr int GEMM_SMS = 148;
 
-template <int BN, int PL>
+template <int BN, int PL, int CTAS>
 struct GemmShape {
-    static constexpr int A_BYTES = GEMM_BM * GEMM_BK * 2, B_BYTES = BN * GEMM_BK * 2;
+    static constexpr int ROWS = GEMM_BM * CTAS;      // of a tile
+    static constexpr int BR = BN / CTAS;             // rows of B that a block brings
+    static constexpr int A_BYTES = GEMM_BM * GEMM_BK * 2, B_BYTES = BR * GEMM_BK * 2;
     static constexpr int STAGE = PL * (A_BYTES + B_BYTES);
     static constexpr int FIT = (200 * 1024) / STAGE;
     static constexpr int STAGES = FIT > 6 ? 6 : FIT;
     static constexpr int ACCS = PL > 1 ? 2 : 1;      // main, small terms
     static constexpr int COLS = 2 * ACCS * BN;       // two tiles in flight
     static constexpr int BYTES = STAGES * STAGE + 1024 + 256;
-    static_assert(COLS <= 512 && STAGES >= 2);
+    static_assert(COLS <= 512 && STAGES >= 2 && BR >= 64);
 };
 
 // An operand: R rows (i or j) by K, z matrices zs apart.
@@ -50,7 +57,7 @@ struct GemmSide {
 struct GemmArgs {
     GemmSide a, b;
     int m, n;             // rows of A, rows of B
-    int ti, tj;           // tiles of 128 and of BN
+    int ti, tj;           // tiles of ROWS and of BN
     int kblocks;          // of 64 in all
     int splits;           // ranges of k; a unit is (tile, split, batch)
     int per;              // k blocks of a split
@@ -59,25 +66,81 @@ struct GemmArgs {
     uint32_t idesc;       // instruction descriptor (types, orders, shape)
 };
 
+template <int CTAS>
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, int cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(cols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (CTAS == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
 }
+template <int CTAS>
 __device__ __forceinline__ void tmem_free(uint32_t addr, int cols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+    if constexpr (CTAS == 2)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+    else
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
 }
+template <int CTAS>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    if constexpr (CTAS == 2)
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            : "memory");
+}
+// the barrier (with two blocks, each one's) gets one arrival when every mma
+// issued so far has finished
+template <int CTAS>
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    if constexpr (CTAS == 2)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                smem_addr(bar)),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                     : "memory");
+}
+// The same place in the first block's shared memory.
+__device__ __forceinline__ uint32_t lead_addr(const void* p) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(p)));
+    return a;
+}
+// Relaxed: what it reports is Tensor Memory that has been read (and waited for);
+// a release would wait for the epilogue's stores to global memory.
+__device__ __forceinline__ void mbar_arrive_at(uint32_t addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// A box into this block's shared memory; its bytes complete on the first block's
+// barrier (address in the cluster).
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_addr(dst)),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
-// the barrier gets one arrival when every mma issued so far has finished
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
+template <int CTAS>
+__device__ __forceinline__ void block_sync() {  // of the tile's blocks
+    if constexpr (CTAS == 2) {
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
 }
 __device__ __forceinline__ void mma_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void mma_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -106,12 +169,13 @@ __device__ __forceinline__ uint64_t gemm_desc(uint32_t addr, int mn) {
 }
 
 struct GemmUnit {
-    int i, j, k0, k1, split, z;
+    int row0, j, k0, k1, split, z;  // row0: the tile's first row
+    int i;
 };
-template <int BN>
+template <int BN, int ROWS>
 __device__ __forceinline__ GemmUnit gemm_unit(const GemmArgs& g, int u) {
     GemmUnit q;
-    constexpr int W = GEMM_BM / BN > 0 ? GEMM_BM / BN : 1;  // tiles across a diagonal block
+    constexpr int W = ROWS / BN;  // tiles across a diagonal block
     const int tiles = g.symmetric ? W * g.ti * (g.ti + 1) / 2 : g.ti * g.tj;
     const int t = u % tiles, r = u / tiles;
     if (g.symmetric) {  // row i has W (i + 1) tiles
@@ -127,6 +191,7 @@ __device__ __forceinline__ GemmUnit gemm_unit(const GemmArgs& g, int u) {
         q.i = i_first ? t % g.ti : t / g.tj;
         q.j = i_first ? t / g.ti : t % g.tj;
     }
+    q.row0 = q.i * ROWS;
     q.split = r % g.splits;
     q.z = r / g.splits;
     q.k0 = q.split * g.per;
@@ -136,20 +201,24 @@ __device__ __forceinline__ GemmUnit gemm_unit(const GemmArgs& g, int u) {
 
 // wait that also ends when another role of the block has given up
 __device__ __forceinline__ bool gemm_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* gave_up) {
-    for (int i = 0; i < WAIT_TRIES; i++) {
-        if (mbar_try(bar, parity)) return true;
+    if (mbar_try(bar, parity)) return true;
+    const long long begin = clock64();
+    while (!mbar_try(bar, parity)) {
         if (*gave_up) return false;
+        if (clock64() - begin > WAIT_CLOCKS) {
+            *gave_up = 1;
+            return false;
+        }
     }
-    *gave_up = 1;
-    return false;
+    return true;
 }
 
 // Epi: void operator()(const GemmUnit&, long long i, int j0, int cols, const float* sum) const for 32 columns
 // from j0 (cols of them inside D) of row i, called by whole warps (rows past m too).
-template <int BN, int PL, class Epi>
-__global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_constant__ GemmArgs g,
-                                                               const __grid_constant__ Epi epi, unsigned int* fault) {
-    using S = GemmShape<BN, PL>;
+template <int BN, int PL, int CTAS, class Epi>
+__global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
+    gemm_kernel(const __grid_constant__ GemmArgs g, const __grid_constant__ Epi epi, unsigned int* fault) {
+    using S = GemmShape<BN, PL, CTAS>;
     extern __shared__ unsigned char raw[];
     // 128-byte swizzle repeats every 1024 bytes
     unsigned char* const sm = raw + (1024 - (smem_addr(raw) & 1023)) % 1024;
@@ -161,6 +230,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
     uint32_t* const slot = reinterpret_cast<uint32_t*>(done + 1);
     volatile uint32_t* const gave_up = slot + 1;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int rank = CTAS == 2 ? blockIdx.x % 2 : 0;  // in the cluster; the first one leads
     if (threadIdx.x == 0) {
         for (int k = 0; k < S::STAGES; k++) {
             mbar_init(&full[k], 1);
@@ -168,7 +238,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
         }
         for (int k = 0; k < 2; k++) {
             mbar_init(&acc_full[k], 1);
-            mbar_init(&acc_empty[k], GEMM_EPI_WARPS);
+            mbar_init(&acc_empty[k], CTAS * GEMM_EPI_WARPS);
         }
         mbar_init(done, 1);
         *gave_up = 0;
@@ -178,22 +248,34 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
             tma_prefetch(&g.b.map[k]);
         }
     }
-    if (warp == 1) tmem_alloc(slot, S::COLS);
-    mma_fence_before();
     __syncthreads();
+    if (warp == 1) tmem_alloc<CTAS>(slot, S::COLS);
+    mma_fence_before();
+    block_sync<CTAS>();
     mma_fence_after();
     const uint32_t tmem = *slot;
+    const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
     if (warp == 0) {
         if (lane == 0) {
             int stage = 0, phase = 0, asked = 0;
             bool ok = true;
-            for (int u = blockIdx.x; u < g.units && ok; u += gridDim.x) {
-                const GemmUnit q = gemm_unit<BN>(g, u);
+            for (int u = first; u < g.units && ok; u += step) {
+                const GemmUnit q = gemm_unit<BN, S::ROWS>(g, u);
+                const int ra = q.row0 + rank * GEMM_BM, rb = q.j * BN + rank * S::BR;
                 for (int k = q.k0; k < q.k1; k++) {
                     ok = gemm_wait(&empty[stage], phase ^ 1, gave_up);
                     if (!ok) break;
-                    mbar_expect(&full[stage], S::STAGE);
+                    const uint32_t bar = CTAS == 2 ? lead_addr(&full[stage]) : 0;
+                    // (the other block's boxes of this round may complete before this: it asks for
+                    // them when the stage is empty, so the last round is over)
+                    if (rank == 0) mbar_expect(&full[stage], CTAS * S::STAGE);
+                    auto load = [&](unsigned char* at, const CUtensorMap* map, int x, int y) {
+                        if constexpr (CTAS == 2)
+                            tma_load_pair(at, map, bar, x, y, q.z);
+                        else
+                            tma_load(at, map, &full[stage], x, y, q.z);
+                    };
                     unsigned char* const at = sm + stage * S::STAGE;
 #pragma unroll
                     for (int p = 0; p < PL; p++) {
@@ -201,31 +283,30 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
                         unsigned char* const pb = at + PL * S::A_BYTES + p * S::B_BYTES;
                         if (g.a.mn)
                             for (int h = 0; h < GEMM_BM / 64; h++)
-                                tma_load(pa + h * 8192, &g.a.map[p], &full[stage], q.i * GEMM_BM + h * 64, k * GEMM_BK,
-                                         q.z);
+                                load(pa + h * 8192, &g.a.map[p], ra + h * 64, k * GEMM_BK);
                         else
-                            tma_load(pa, &g.a.map[p], &full[stage], k * GEMM_BK, q.i * GEMM_BM, q.z);
+                            load(pa, &g.a.map[p], k * GEMM_BK, ra);
                         if (g.b.mn)
-                            for (int h = 0; h < BN / 64; h++)
-                                tma_load(pb + h * 8192, &g.b.map[p], &full[stage], q.j * BN + h * 64, k * GEMM_BK, q.z);
+                            for (int h = 0; h < S::BR / 64; h++)
+                                load(pb + h * 8192, &g.b.map[p], rb + h * 64, k * GEMM_BK);
                         else
-                            tma_load(pb, &g.b.map[p], &full[stage], k * GEMM_BK, q.j * BN, q.z);
+                            load(pb, &g.b.map[p], k * GEMM_BK, rb);
                     }
                     asked++;
                     if (++stage == S::STAGES) stage = 0, phase ^= 1;
                 }
             }
-            if (!ok)  // not before the copies asked for have come
+            if (!ok && rank == 0)  // not before the copies asked for have come
                 for (int r = asked > S::STAGES ? asked - S::STAGES : 0; r < asked; r++)
                     mbar_wait(&full[r % S::STAGES], (r / S::STAGES) & 1);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             int stage = 0, phase = 0, acc = 0, aphase = 0;
             bool ok = true;
             const int ka = g.a.mn ? 2048 >> 4 : 32 >> 4, kb = g.b.mn ? 2048 >> 4 : 32 >> 4;  // 16 k further
-            for (int u = blockIdx.x; u < g.units && ok; u += gridDim.x) {
-                const GemmUnit q = gemm_unit<BN>(g, u);
+            for (int u = first; u < g.units && ok; u += step) {
+                const GemmUnit q = gemm_unit<BN, S::ROWS>(g, u);
                 ok = gemm_wait(&acc_empty[acc], aphase ^ 1, gave_up);
                 if (!ok) break;
                 mma_fence_after();
@@ -246,16 +327,16 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
                             const bool starts = k == q.k0 && (!small || (pa == 0 && pb == 1));
 #pragma unroll
                             for (int s = 0; s < GEMM_BK / 16; s++)
-                                mma_f16(d + (small ? BN : 0), da + s * ka, db + s * kb, g.idesc, !(starts && s == 0));
+                                mma_f16<CTAS>(d + (small ? BN : 0), da + s * ka, db + s * kb, g.idesc, !(starts && s == 0));
                         }
-                    mma_commit(&empty[stage]);
+                    mma_commit<CTAS>(&empty[stage]);
                     if (++stage == S::STAGES) stage = 0, phase ^= 1;
                 }
-                if (ok) mma_commit(&acc_full[acc]);
+                if (ok) mma_commit<CTAS>(&acc_full[acc]);
                 if (++acc == 2) acc = 0, aphase ^= 1;
             }
             if (!ok) {  // not before what was issued has finished
-                mma_commit(done);
+                mma_commit<CTAS>(done);
                 mbar_wait(done, 0);
             }
         }
@@ -263,12 +344,12 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
         // lanes 32 (warp % 4) .. of the accumulator are this warp's to read
         const int quarter = warp % 4, half = (warp - 2) / 4;
         int acc = 0, aphase = 0;
-        for (int u = blockIdx.x; u < g.units; u += gridDim.x) {
-            const GemmUnit q = gemm_unit<BN>(g, u);
+        for (int u = first; u < g.units; u += step) {
+            const GemmUnit q = gemm_unit<BN, S::ROWS>(g, u);
             if (!__all_sync(0xffffffffu, gemm_wait(&acc_full[acc], aphase, gave_up))) break;
             mma_fence_after();
             const uint32_t d = tmem + acc * S::ACCS * BN + ((uint32_t)quarter * 32 << 16);
-            const long long i = (long long)q.i * GEMM_BM + quarter * 32 + lane;
+            const long long i = q.row0 + rank * GEMM_BM + quarter * 32 + lane;
             const bool any = q.k0 < q.k1;
             for (int c = half * 32; c < BN; c += 64) {
                 const int j = q.j * BN + c, cols = g.n - j < 32 ? g.n - j : 32;
@@ -292,15 +373,20 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_cons
             }
             mma_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[acc]);
+            if (lane == 0) {
+                if constexpr (CTAS == 2)
+                    mbar_arrive_at(lead_addr(&acc_empty[acc]));
+                else
+                    mbar_arrive(&acc_empty[acc]);
+            }
             if (++acc == 2) acc = 0, aphase ^= 1;
         }
     }
     __syncwarp();
     mma_fence_before();
-    __syncthreads();
+    block_sync<CTAS>();
     mma_fence_after();
-    if (warp == 1) tmem_free(tmem, S::COLS);
+    if (warp == 1) tmem_free<CTAS>(tmem, S::COLS);
     if (threadIdx.x == 0 && *gave_up) atomicAdd(fault, 1u);
 }
 
@@ -350,47 +436,90 @@ struct GemmOnce {
     }
 };
 
-// Splits of k that make `units` up to about two per SM, each of 8 blocks at least.
-inline int gemm_splits(long long tiles, long long kblocks) {
-    if (tiles >= GEMM_SMS / 2) return 1;
-    long long n = 2 * GEMM_SMS / tiles;
-    if (n > kblocks / 8) n = kblocks / 8;
-    if (n < 2) return 1;
-    const long long per = (kblocks + n - 1) / n;
-    return (int)((kblocks + per - 1) / per);
+// How a product is cut.
+struct GemmCut {
+    int ctas, bn, splits;
+};
+
+// The shape that takes least by a rough count of clocks: rounds of tiles over the
+// SMs (pairs for two blocks), each its k blocks' mma time (a lone block's are held
+// up by L2) and 1500 to fill and empty. `planes`: products per product. splits: k
+// is cut too where that fills SMs that the tiles leave empty (parts of 8 k blocks
+// at least; joining them costs about 3000 more).
+inline GemmCut gemm_cut(long long rows, long long cols, long long k, long long batch, int products, bool symmetric,
+                        bool may_split) {
+    const struct {
+        int ctas, bn;
+        double clocks;  // of a k block
+    } shapes[] = {{2, 256, 540}, {2, 128, 300}, {1, 128, 340}, {1, 64, 230}};
+    const long long kb = (k + GEMM_BK - 1) / GEMM_BK;
+    GemmCut best{};
+    double least = 0;
+    for (const auto& s : shapes) {
+        if (products > 1 && s.bn == 256) continue;  // (Tensor Memory holds two tiles of two accumulators)
+        const long long r = GEMM_BM * s.ctas, ti = (rows + r - 1) / r, tj = (cols + s.bn - 1) / s.bn;
+        const long long tiles = (symmetric ? r / s.bn * ti * (ti + 1) / 2 : ti * tj) * batch;
+        const long long slots = GEMM_SMS / s.ctas;
+        long long most = may_split && tiles < slots ? kb / 8 : 1;
+        if (most > 64) most = 64;
+        for (long long n = 1; n == 1 || n <= most; n++) {
+            const long long per = (kb + n - 1) / n;
+            if (n > 1 && (kb + per - 1) / per != n) continue;
+            const double c = (double)((tiles * n + slots - 1) / slots) * (per * s.clocks * products + 1500) +
+                             (n > 1 ? 3000 + n * 100.0 : 0);
+            if (!best.ctas || c < least) {
+                best = {s.ctas, s.bn, (int)n};
+                least = c;
+            }
+            if (tiles * n > 2 * slots) break;
+        }
+    }
+    return best;
 }
 
 // D = A B^T (rows ma of A, nb of B). a, b: PL planes each. splits > 1: the
 // epilogue gets each split's part.
-template <int BN, int PL, class Epi>
-cudaError_t gemm_launch(const GemmMat* a, const GemmMat* b, long long ma, long long nb, long long k, int batch,
-                        int splits, bool symmetric, bool bf16, const Epi& epi, unsigned int* fault, cudaStream_t st) {
-    using S = GemmShape<BN, PL>;
+template <int BN, int PL, int CTAS, class Epi>
+cudaError_t gemm_launch_as(const GemmMat* a, const GemmMat* b, long long ma, long long nb, long long k, int batch,
+                           int splits, bool symmetric, bool bf16, const Epi& epi, unsigned int* fault, cudaStream_t st) {
+    using S = GemmShape<BN, PL, CTAS>;
     GemmArgs g{};
     for (int p = 0; p < PL; p++) {
         if (!gemm_map(&g.a, p, a[p], ma, k, batch, GEMM_BM, bf16)) return cudaErrorInvalidValue;
-        if (!gemm_map(&g.b, p, b[p], nb, k, batch, BN, bf16)) return cudaErrorInvalidValue;
+        if (!gemm_map(&g.b, p, b[p], nb, k, batch, S::BR, bf16)) return cudaErrorInvalidValue;
     }
     g.m = (int)ma;
     g.n = (int)nb;
-    g.ti = (int)((ma + GEMM_BM - 1) / GEMM_BM);
+    g.ti = (int)((ma + S::ROWS - 1) / S::ROWS);
     g.tj = (int)((nb + BN - 1) / BN);
     g.kblocks = (int)((k + GEMM_BK - 1) / GEMM_BK);
     g.splits = splits;
     g.per = (g.kblocks + splits - 1) / splits;
     g.symmetric = symmetric;
-    const long long tiles =
-        symmetric ? (long long)(GEMM_BM / BN) * g.ti * (g.ti + 1) / 2 : (long long)g.ti * g.tj;
+    const long long tiles = symmetric ? (long long)(S::ROWS / BN) * g.ti * (g.ti + 1) / 2 : (long long)g.ti * g.tj;
     if (tiles * splits * batch >= 1 << 30) return cudaErrorInvalidValue;
     g.units = (int)(tiles * splits * batch);
     g.idesc = 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (uint32_t)g.a.mn << 15 |
-              (uint32_t)g.b.mn << 16 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(GEMM_BM >> 4) << 24;
-    auto kernel = gemm_kernel<BN, PL, Epi>;
+              (uint32_t)g.b.mn << 16 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(S::ROWS >> 4) << 24;
+    auto kernel = gemm_kernel<BN, PL, CTAS, Epi>;
     static GemmOnce once;
     const cudaError_t e = once.smem(kernel, S::BYTES);
     if (e != cudaSuccess) return e;
-    kernel<<<g.units < GEMM_SMS ? g.units : GEMM_SMS, GEMM_THREADS, S::BYTES, st>>>(g, epi, fault);
+    const int slots = GEMM_SMS / CTAS;
+    kernel<<<(g.units < slots ? g.units : slots) * CTAS, GEMM_THREADS, S::BYTES, st>>>(g, epi, fault);
     return cudaGetLastError();
+}
+
+template <int PL, class Epi>
+cudaError_t gemm_launch(const GemmMat* a, const GemmMat* b, long long ma, long long nb, long long k, int batch,
+                        const GemmCut& c, bool symmetric, bool bf16, const Epi& epi, unsigned int* fault,
+                        cudaStream_t st) {
+    if constexpr (PL == 1)
+        if (c.ctas == 2 && c.bn == 256)
+            return gemm_launch_as<256, PL, 2>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, epi, fault, st);
+    if (c.ctas == 2) return gemm_launch_as<128, PL, 2>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, epi, fault, st);
+    if (c.bn == 128) return gemm_launch_as<128, PL, 1>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, epi, fault, st);
+    return gemm_launch_as<64, PL, 1>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, epi, fault, st);
 }
 
 }  // namespace pz

@@ -254,34 +254,9 @@ struct Operand {
 
 // ── tensor-core products ──────────────────────────────────────────────────
 
-// How a product is cut: columns of a tile (256, 128 or 64; 128 at most for
-// planes), splits of k. The widest tile does most work per byte of shared
-// memory; narrower ones are taken where the wide ones leave SMs idle in the last
-// round (a tile costs about its width and 32 columns more).
-struct Cut {
-    int bn, splits;
-};
+using Cut = GemmCut;
 Cut cut_of(long long rows, long long cols, long long k, bool f32) {
-    const long long ti = (rows + 127) / 128;
-    Cut c{0, 1};
-    long long best = 0;
-    for (int bn = f32 ? 128 : 256; bn >= 64; bn /= 2) {
-        const long long tiles = ti * ((cols + bn - 1) / bn);
-        const long long cost = (tiles + GEMM_SMS - 1) / GEMM_SMS * (bn + 32);
-        if (!c.bn || cost < best) {
-            c.bn = bn;
-            best = cost;
-        }
-    }
-    const long long kb = (k + GEMM_BK - 1) / GEMM_BK;
-    if (ti * ((cols + 255) / 256) < GEMM_SMS / 2) {
-        // too few tiles: cut k as well, into tiles as wide as they were
-        int bn = f32 ? 128 : 256;
-        while (bn > 64 && bn / 2 >= cols) bn /= 2;
-        const int s = gemm_splits(ti * ((cols + bn - 1) / bn), kb);
-        if (s > 1) return {bn, s};
-    }
-    return c;
+    return gemm_cut(rows, cols, k, 1, f32 ? 6 : 1, false, true);
 }
 
 long long part_bytes(const Cut& c, long long rows, long long cols) {
@@ -296,10 +271,7 @@ cudaError_t multiply_cut(const GemmMat* a, const GemmMat* b, long long rows, lon
     if (!fault) return cudaErrorInvalidSymbol;
     constexpr bool bf16 = !std::is_same<T, __half>::value;
     constexpr int PL = sizeof(T) == 4 ? 3 : 1;
-    if constexpr (PL == 1)
-        if (c.bn == 256) return gemm_launch<256, PL>(a, b, rows, cols, k, 1, c.splits, false, bf16, epi, fault, st);
-    if (c.bn == 128) return gemm_launch<128, PL>(a, b, rows, cols, k, 1, c.splits, false, bf16, epi, fault, st);
-    return gemm_launch<64, PL>(a, b, rows, cols, k, 1, c.splits, false, bf16, epi, fault, st);
+    return gemm_launch<PL>(a, b, rows, cols, k, 1, c, false, bf16, epi, fault, st);
 }
 
 // D = A B^T through `epi`; part: room for the splits' parts.

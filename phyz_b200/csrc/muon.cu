@@ -209,7 +209,7 @@ struct SquareEpi {
         for (int k = 0; k < 32; k++) v[k] = g.p ? fmaf(b, v[k], c * sum[k]) : c * sum[k];
         pair_store(out, e, cols, v);
         // the tile's mirror image, unless it is inside a diagonal block
-        if (j0 < q.i * GEMM_BM) {
+        if (j0 < q.row0) {
 #pragma unroll
             for (int k = 0; k < 32; k++)
                 if (k < cols) out.put(z + (j0 + k) * out.pitch + i, v[k]);
@@ -296,8 +296,7 @@ Ws layout(long long batch, long long rows, long long cols) {
     return w;
 }
 
-// D = A B^T on pairs. BN = 128 does twice the work of 64 per byte of shared
-// memory; 64 where 128 leaves SMs idle in the only round.
+// D = A B^T on pairs.
 template <class Epi>
 cudaError_t multiply(const Pair& a, bool a_mn, const Pair& b, bool b_mn, long long rows, long long cols, long long k,
                      int batch, bool symmetric, const Epi& epi, unsigned int* fault, cudaStream_t st) {
@@ -306,11 +305,8 @@ cudaError_t multiply(const Pair& a, bool a_mn, const Pair& b, bool b_mn, long lo
         ma[h] = {a.p + h * a.lo, a_mn ? 1 : a.pitch, a_mn ? a.pitch : 1, a.zs};
         mb[h] = {b.p + h * b.lo, b_mn ? 1 : b.pitch, b_mn ? b.pitch : 1, b.zs};
     }
-    const long long ti = (rows + 127) / 128, tj = (cols + 127) / 128;
-    const long long units = (symmetric ? ti * (ti + 1) / 2 : ti * tj) * batch;
-    if (units * 2 <= GEMM_SMS)
-        return gemm_launch<64, 2>(ma, mb, rows, cols, k, batch, 1, symmetric, false, epi, fault, st);
-    return gemm_launch<128, 2>(ma, mb, rows, cols, k, batch, 1, symmetric, false, epi, fault, st);
+    const GemmCut cut = gemm_cut(rows, cols, k, batch, 3, symmetric, false);
+    return gemm_launch<2>(ma, mb, rows, cols, k, batch, cut, symmetric, false, epi, fault, st);
 }
 
 cudaError_t solve(const Problem& q, char* ws, cudaStream_t st) {

@@ -32,20 +32,21 @@ __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
     uint32_t done;
     asm volatile(
         "{\n.reg .pred p;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 10000;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
         "selp.u32 %0, 1, 0, p;\n}"
         : "=r"(done)
         : "r"(smem_addr(bar)), "r"(parity)
         : "memory");
     return done != 0;
 }
-// One try sleeps up to 10 us (the hint above), so this gives up after seconds,
-// far above any wait that ends.
-constexpr int WAIT_TRIES = 1 << 19;
+// A wait gives up after some seconds (2^33 clocks), far above any that ends.
+constexpr long long WAIT_CLOCKS = 1ll << 33;
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
-    for (int i = 0; i < WAIT_TRIES; i++)
-        if (mbar_try(bar, parity)) return true;
-    return false;
+    if (mbar_try(bar, parity)) return true;
+    const long long begin = clock64();
+    while (!mbar_try(bar, parity))
+        if (clock64() - begin > WAIT_CLOCKS) return false;
+    return true;
 }
 
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
