@@ -6,7 +6,10 @@
 // tcgen05.mma into one of two accumulators in Tensor Memory, and eight more warps
 // empty the other one through the epilogue, so that the tensor cores wait neither
 // for memory nor for the epilogue. In the epilogue a lane has 32 neighbours in j
-// and a warp 32 in i.
+// and a warp 32 in i: a chunk. Where TMA can address them, what the epilogue reads
+// comes into the warp's own slots of shared memory a chunk ahead and what it
+// writes leaves from there: a lane's own 32-byte accesses to 32 rows keep the
+// memory pipe busy for longer than the tensor cores take for a K of 1024.
 //
 // CTAS = 2: the two blocks of a cluster (the SMs of a pair) make one tile of 256 x
 // BN: each brings its 128 rows of A and half of B's, one mma reads both shared
@@ -34,17 +37,23 @@ constexpr int GEMM_EPI_WARPS = 8;
 constexpr int GEMM_THREADS = 32 * (2 + GEMM_EPI_WARPS);
 constexpr int GEMM_SMS = 148;
 
-template <int BN, int PL, int CTAS>
+// A chunk's slot: 32 rows of 32 16-bit values, one or two planes.
+constexpr int GEMM_PLANE = 32 * 64;
+
+template <int BN, int PL, int CTAS, class Epi>
 struct GemmShape {
     static constexpr int ROWS = GEMM_BM * CTAS;      // of a tile
     static constexpr int BR = BN / CTAS;             // rows of B that a block brings
     static constexpr int A_BYTES = GEMM_BM * GEMM_BK * 2, B_BYTES = BR * GEMM_BK * 2;
     static constexpr int STAGE = PL * (A_BYTES + B_BYTES);
-    static constexpr int FIT = (200 * 1024) / STAGE;
+    static constexpr int WARP_SLOTS = Epi::PLANES * Epi::SLOTS * GEMM_PLANE;
+    static constexpr int SLOTS = GEMM_EPI_WARPS * WARP_SLOTS;
+    static constexpr int FIT = (224 * 1024 - SLOTS) / STAGE;
     static constexpr int STAGES = FIT > 6 ? 6 : FIT;
     static constexpr int ACCS = PL > 1 ? 2 : 1;      // main, small terms
     static constexpr int COLS = 2 * ACCS * BN;       // two tiles in flight
-    static constexpr int BYTES = STAGES * STAGE + 1024 + 256;
+    static constexpr int BYTES = STAGES * STAGE + SLOTS + 1024 + 512;
+    static_assert(BYTES <= 227 * 1024);
     static_assert(COLS <= 512 && STAGES >= 2 && BR >= 64);
 };
 
@@ -54,8 +63,16 @@ struct GemmSide {
     int mn;  // rows contiguous instead of k
 };
 
+// What the epilogue reads and writes through slots: planes of arrays [batch][i][j]
+// (j contiguous) as tensor maps, in boxes of 32 x 32.
+struct GemmIo {
+    CUtensorMap in[2], out[2];
+    int reads, writes;  // whether through slots
+};
+
 struct GemmArgs {
     GemmSide a, b;
+    GemmIo io;
     int m, n;             // rows of A, rows of B
     int ti, tj;           // tiles of ROWS and of BN
     int kblocks;          // of 64 in all
@@ -213,21 +230,44 @@ __device__ __forceinline__ bool gemm_wait(uint64_t* bar, uint32_t parity, volati
     return true;
 }
 
-// Epi: void operator()(const GemmUnit&, long long i, int j0, int cols, const float* sum) const for 32 columns
-// from j0 (cols of them inside D) of row i, called by whole warps (rows past m too).
+// A lane's 32 16-bit values in a slot's plane (64-byte swizzle).
+__device__ __forceinline__ void slot_load(const unsigned char* plane, uint32_t* w) {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const uint4 q = *reinterpret_cast<const uint4*>(plane + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4));
+        w[4 * c] = q.x, w[4 * c + 1] = q.y, w[4 * c + 2] = q.z, w[4 * c + 3] = q.w;
+    }
+}
+__device__ __forceinline__ void slot_store(unsigned char* plane, const uint32_t* w) {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+        *reinterpret_cast<uint4*>(plane + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4)) =
+            make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+}
+// where value (row, col) of a plane is
+__device__ __forceinline__ int slot_at(int row, int col) { return row * 64 + (((col >> 3) ^ (row >> 1 & 3)) << 4) + (col & 7) * 2; }
+
+// Epi: void operator()(const GemmUnit&, long long i, int j0, int cols, float* sum, const unsigned char* in, unsigned
+// char* out) const for 32 columns from j0 (cols of them inside D) of row i, called by whole warps (rows past m too).
+// in, out: the chunk's slot where GemmIo says so (the same one), else null. PLANES of a slot, SLOTS of a warp. MIRROR:
+// where mirrored(unit, j0) says so, the chunk's mirror image is written as well, by turn(sum, slot).
 template <int BN, int PL, int CTAS, class Epi>
 __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
     gemm_kernel(const __grid_constant__ GemmArgs g, const __grid_constant__ Epi epi, unsigned int* fault) {
-    using S = GemmShape<BN, PL, CTAS>;
+    using S = GemmShape<BN, PL, CTAS, Epi>;
     extern __shared__ unsigned char raw[];
     // 128-byte swizzle repeats every 1024 bytes
     unsigned char* const sm = raw + (1024 - (smem_addr(raw) & 1023)) % 1024;
-    uint64_t* const full = reinterpret_cast<uint64_t*>(sm + S::STAGES * S::STAGE);
+    unsigned char* const slots = sm + S::STAGES * S::STAGE;
+    uint64_t* const full = reinterpret_cast<uint64_t*>(slots + S::SLOTS);
     uint64_t* const empty = full + S::STAGES;
     uint64_t* const acc_full = empty + S::STAGES;
     uint64_t* const acc_empty = acc_full + 2;
     uint64_t* const done = acc_empty + 2;
-    uint32_t* const slot = reinterpret_cast<uint32_t*>(done + 1);
+    uint64_t* const slot_full = done + 1;
+    uint32_t* const slot = reinterpret_cast<uint32_t*>(slot_full + GEMM_EPI_WARPS * Epi::SLOTS);
     volatile uint32_t* const gave_up = slot + 1;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rank = CTAS == 2 ? blockIdx.x % 2 : 0;  // in the cluster; the first one leads
@@ -241,6 +281,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
             mbar_init(&acc_empty[k], CTAS * GEMM_EPI_WARPS);
         }
         mbar_init(done, 1);
+        for (int k = 0; k < GEMM_EPI_WARPS * Epi::SLOTS; k++) mbar_init(&slot_full[k], 1);
         *gave_up = 0;
         mbar_init_fence();
         for (int k = 0; k < PL; k++) {
@@ -342,18 +383,64 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
         }
     } else {
         // lanes 32 (warp % 4) .. of the accumulator are this warp's to read
-        const int quarter = warp % 4, half = (warp - 2) / 4;
-        int acc = 0, aphase = 0;
-        for (int u = first; u < g.units; u += step) {
+        const int quarter = warp % 4, half = (warp - 2) / 4, own = rank * GEMM_BM + quarter * 32;
+        constexpr int NS = Epi::SLOTS, MOD = NS > 0 ? NS : 1;
+        unsigned char* const mine = slots + (warp - 2) * S::WARP_SLOTS;
+        uint64_t* const bars = slot_full + (warp - 2) * NS;
+        // lane 0's place in the sequence of chunks, ahead of the warp's
+        int au = first, ac = half * 32, asked = 0;
+        GemmUnit aq{};
+        if (au < g.units) aq = gemm_unit<BN, S::ROWS>(g, au);
+        auto request = [&]() {
+            while (au < g.units) {
+                const bool there = ac < BN && aq.row0 + own < g.m && aq.j * BN + ac < g.n;
+                if (there) {
+                    unsigned char* const at = mine + asked % MOD * Epi::PLANES * GEMM_PLANE;
+                    mbar_expect(&bars[asked % MOD], Epi::PLANES * GEMM_PLANE);
+#pragma unroll
+                    for (int p = 0; p < Epi::PLANES; p++)
+                        tma_load(at + p * GEMM_PLANE, &g.io.in[p], &bars[asked % MOD], aq.j * BN + ac, aq.row0 + own, aq.z);
+                    asked++;
+                    ac += 64;
+                    return;
+                }
+                ac = half * 32;
+                au += step;
+                if (au < g.units) aq = gemm_unit<BN, S::ROWS>(g, au);
+            }
+        };
+        const bool reads = Epi::PLANES && g.io.reads, writes = Epi::PLANES && g.io.writes;
+        // (a chunk's slot is asked for again two chunks after its results left, one where there are two slots)
+        if (reads && lane == 0)
+            for (int k = 0; k < (NS > 2 ? NS - 2 : 1); k++) request();
+        int acc = 0, aphase = 0, n = 0;
+        bool ok = true;
+        for (int u = first; u < g.units && ok; u += step) {
             const GemmUnit q = gemm_unit<BN, S::ROWS>(g, u);
-            if (!__all_sync(0xffffffffu, gemm_wait(&acc_full[acc], aphase, gave_up))) break;
+            ok = __all_sync(0xffffffffu, gemm_wait(&acc_full[acc], aphase, gave_up));
+            if (!ok) break;
             mma_fence_after();
             const uint32_t d = tmem + acc * S::ACCS * BN + ((uint32_t)quarter * 32 << 16);
-            const long long i = q.row0 + rank * GEMM_BM + quarter * 32 + lane;
+            const long long i = q.row0 + own + lane;
             const bool any = q.k0 < q.k1;
             for (int c = half * 32; c < BN; c += 64) {
                 const int j = q.j * BN + c, cols = g.n - j < 32 ? g.n - j : 32;
-                if (cols <= 0) break;
+                if (cols <= 0 || q.row0 + own >= g.m) break;
+                unsigned char* const at = mine + n % MOD * Epi::PLANES * GEMM_PLANE;
+                if constexpr (NS > 0) {
+                    if (writes || reads) {
+                        // the slot of a chunk ahead, or this one's, is empty again
+                        if (lane == 0) {
+                            if (reads && NS > 1) {
+                                tma_store_wait_read<(NS > 2 ? 1 : 0)>();
+                                request();
+                            } else {
+                                tma_store_wait_read<NS - 1>();
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
                 float v[32];
                 tmem_load(d + c, v);
                 if (PL > 1) {
@@ -369,7 +456,47 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
 #pragma unroll
                     for (int e = 0; e < 32; e++) v[e] = 0.0f;
                 }
-                epi(q, i, j, cols, v);
+                if constexpr (NS > 0) {
+                    if (reads) {
+                        ok = __all_sync(0xffffffffu, gemm_wait(&bars[n % NS], (n / NS) & 1, gave_up));
+                        if (!ok) break;
+                    }
+                }
+                epi(q, i, j, cols, v, reads ? at : nullptr, writes ? at : nullptr);
+                if constexpr (NS > 0) {
+                    if (writes) {
+                        fence_async();
+                        __syncwarp();
+                        if (lane == 0) {  // (past m and n nothing is written)
+#pragma unroll
+                            for (int p = 0; p < Epi::PLANES; p++)
+                                tma_store(&g.io.out[p], at + p * GEMM_PLANE, j, q.row0 + own, q.z);
+                            tma_store_commit();
+                        }
+                        if constexpr (Epi::MIRROR) {
+                            if (epi.mirrored(q, j)) {
+                                if (lane == 0) tma_store_wait_read<0>();
+                                __syncwarp();
+                                epi.turn(v, at);
+                                fence_async();
+                                __syncwarp();
+                                if (lane == 0) {
+#pragma unroll
+                                    for (int p = 0; p < Epi::PLANES; p++)
+                                        tma_store(&g.io.out[p], at + p * GEMM_PLANE, q.row0 + own, j, q.z);
+                                    tma_store_commit();
+                                }
+                            }
+                        }
+                    } else {
+                        __syncwarp();
+                    }
+                    if (NS == 1 && reads && lane == 0) {
+                        tma_store_wait_read<0>();
+                        request();
+                    }
+                }
+                n++;
             }
             mma_fence_before();
             __syncwarp();
@@ -380,6 +507,13 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
                     mbar_arrive(&acc_empty[acc]);
             }
             if (++acc == 2) acc = 0, aphase ^= 1;
+        }
+        if constexpr (NS > 0) {
+            if (lane == 0) {
+                if (!ok)  // not before the boxes asked for have come
+                    for (int r = asked > NS ? asked - NS : 0; r < asked; r++) mbar_wait(&bars[r % NS], (r / NS) & 1);
+                tma_store_wait_read<0>();
+            }
         }
     }
     __syncwarp();
@@ -406,6 +540,18 @@ inline bool gemm_tma_ok(const GemmMat& m, long long rows, long long k, long long
     if ((uintptr_t)m.p % 16 || (batch > 1 && !stride_ok(m.zs))) return false;
     if (gemm_mn(m, k)) return k == 1 || stride_ok(m.ks);
     return m.ks == 1 && (rows == 1 || stride_ok(m.rs));
+}
+
+// The tensor map of a plane that an epilogue reads or writes: [batch][rows][cols],
+// cols contiguous. False where TMA cannot address it.
+inline bool gemm_io_map(CUtensorMap* m, const void* p, long long rs, long long cs, long long zs, long long rows,
+                        long long cols, long long batch, bool bf16) {
+    if (cs != 1 || !gemm_tma_ok({p, rs, 1, zs}, rows, cols, batch)) return false;
+    const cuuint64_t size[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch};
+    const cuuint64_t stride[2] = {rows > 1 ? (cuuint64_t)rs * 2 : 16, batch > 1 ? (cuuint64_t)zs * 2 : 16};
+    const cuuint32_t box[3] = {32, 32, 1};
+    return encode_tiled(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                        const_cast<void*>(p), size, stride, box, CU_TENSOR_MAP_SWIZZLE_64B) == CUDA_SUCCESS;
 }
 
 inline bool gemm_map(GemmSide* s, int plane, const GemmMat& m, long long rows, long long k, long long batch, int tile,
@@ -481,9 +627,11 @@ inline GemmCut gemm_cut(long long rows, long long cols, long long k, long long b
 // epilogue gets each split's part.
 template <int BN, int PL, int CTAS, class Epi>
 cudaError_t gemm_launch_as(const GemmMat* a, const GemmMat* b, long long ma, long long nb, long long k, int batch,
-                           int splits, bool symmetric, bool bf16, const Epi& epi, unsigned int* fault, cudaStream_t st) {
-    using S = GemmShape<BN, PL, CTAS>;
+                           int splits, bool symmetric, bool bf16, const GemmIo& io, const Epi& epi, unsigned int* fault,
+                           cudaStream_t st) {
+    using S = GemmShape<BN, PL, CTAS, Epi>;
     GemmArgs g{};
+    g.io = io;
     for (int p = 0; p < PL; p++) {
         if (!gemm_map(&g.a, p, a[p], ma, k, batch, GEMM_BM, bf16)) return cudaErrorInvalidValue;
         if (!gemm_map(&g.b, p, b[p], nb, k, batch, S::BR, bf16)) return cudaErrorInvalidValue;
@@ -512,14 +660,14 @@ cudaError_t gemm_launch_as(const GemmMat* a, const GemmMat* b, long long ma, lon
 
 template <int PL, class Epi>
 cudaError_t gemm_launch(const GemmMat* a, const GemmMat* b, long long ma, long long nb, long long k, int batch,
-                        const GemmCut& c, bool symmetric, bool bf16, const Epi& epi, unsigned int* fault,
-                        cudaStream_t st) {
+                        const GemmCut& c, bool symmetric, bool bf16, const GemmIo& io, const Epi& epi,
+                        unsigned int* fault, cudaStream_t st) {
     if constexpr (PL == 1)
         if (c.ctas == 2 && c.bn == 256)
-            return gemm_launch_as<256, PL, 2>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, epi, fault, st);
-    if (c.ctas == 2) return gemm_launch_as<128, PL, 2>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, epi, fault, st);
-    if (c.bn == 128) return gemm_launch_as<128, PL, 1>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, epi, fault, st);
-    return gemm_launch_as<64, PL, 1>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, epi, fault, st);
+            return gemm_launch_as<256, PL, 2>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, io, epi, fault, st);
+    if (c.ctas == 2) return gemm_launch_as<128, PL, 2>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, io, epi, fault, st);
+    if (c.bn == 128) return gemm_launch_as<128, PL, 1>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, io, epi, fault, st);
+    return gemm_launch_as<64, PL, 1>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, io, epi, fault, st);
 }
 
 }  // namespace pz

@@ -77,8 +77,16 @@ __device__ __forceinline__ void store4(float* p, long long stride, int n, const 
     }
 }
 
+// 16-bit results go through slots where TMA can address them; f32 ones are few
+// beside their six products, and go straight.
 template <class T>
-struct LinearEpi {
+struct Slotted {
+    static constexpr int PLANES = sizeof(T) == 2 ? 1 : 0, SLOTS = sizeof(T) == 2 ? 4 : 0;
+    static constexpr bool MIRROR = false;
+};
+
+template <class T>
+struct LinearEpi : Slotted<T> {
     const float* bias;
     int by_i;  // bias along i
     int act;
@@ -108,12 +116,16 @@ struct LinearEpi {
             store4(y.p + i * y.is + j * y.js, along_i ? y.is : y.js, n, z);
         }
     }
-    __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, const float* sum) const {
+    __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, const float* sum,
+                                               const unsigned char* in, unsigned char* out) const {
         if (i >= m) return;
         T t[32];
         // (the residual may be y itself: all 32 are read before any is written)
         T r[32];
-        if (res.p) load32(res.p + i * res.is + j0 * res.js, res.js, cols, r);
+        if (in)
+            slot_load(in, reinterpret_cast<uint32_t*>(r));
+        else if (res.p)
+            load32(res.p + i * res.is + j0 * res.js, res.js, cols, r);
         float z[32];
         if (bias && !by_i) {
             load32(bias + j0, 1, cols, z);
@@ -135,12 +147,15 @@ struct LinearEpi {
         });
 #pragma unroll
         for (int c = 0; c < 32; c++) t[c] = from_f32<T>(res.p ? z[c] + to_f32(r[c]) : z[c]);
-        store32(y.p + i * y.is + j0 * y.js, y.js, cols, t);
+        if (out)
+            slot_store(out, reinterpret_cast<const uint32_t*>(t));
+        else
+            store32(y.p + i * y.is + j0 * y.js, y.js, cols, t);
     }
 };
 
 template <class T>
-struct StoreEpi {
+struct StoreEpi : Slotted<T> {
     Out<T> out;
     long long m;
     __device__ __forceinline__ void one(long long i, long long j, float v) const {
@@ -149,26 +164,60 @@ struct StoreEpi {
     __device__ __forceinline__ void four(int, long long i, long long j, const float* v, int n, bool along_i) const {
         if constexpr (sizeof(T) == 4) store4(out.p + i * out.is + j * out.js, along_i ? out.is : out.js, n, v);
     }
-    __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, const float* v) const {
+    __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, const float* v,
+                                               const unsigned char*, unsigned char* slot) const {
         if (i >= m) return;
         T t[32];
 #pragma unroll
         for (int c = 0; c < 32; c++) t[c] = from_f32<T>(v[c]);
-        store32(out.p + i * out.is + j0 * out.js, out.js, cols, t);
+        if (slot)
+            slot_store(slot, reinterpret_cast<const uint32_t*>(t));
+        else
+            store32(out.p + i * out.is + j0 * out.js, out.js, cols, t);
     }
 };
 
+template <class T>
+StoreEpi<T> store_epi(const Out<T>& out, long long m) {
+    StoreEpi<T> e;
+    e.out = out;
+    e.m = m;
+    return e;
+}
+
+// The slots' side of an epilogue for D [rows][cols].
+template <class T>
+GemmIo io_of(const LinearEpi<T>& e, long long rows, long long cols) {
+    GemmIo io{};
+    constexpr bool bf16 = !std::is_same<T, __half>::value;
+    if constexpr (sizeof(T) == 2) {
+        io.writes = gemm_io_map(&io.out[0], e.y.p, e.y.is, e.y.js, 0, rows, cols, 1, bf16);
+        io.reads = e.res.p && gemm_io_map(&io.in[0], e.res.p, e.res.is, e.res.js, 0, rows, cols, 1, bf16);
+    }
+    return io;
+}
+template <class T>
+GemmIo io_of(const StoreEpi<T>& e, long long rows, long long cols) {
+    GemmIo io{};
+    if constexpr (sizeof(T) == 2)
+        io.writes = gemm_io_map(&io.out[0], e.out.p, e.out.is, e.out.js, 0, rows, cols, 1, !std::is_same<T, __half>::value);
+    return io;
+}
+
 // A split's part, [split][m][n] f32.
-struct PartEpi {
+struct PartEpi : Slotted<float> {
     float* part;
     long long m, n;
     __device__ __forceinline__ void four(int split, long long i, long long j, const float* v, int k, bool along_i) const {
         store4(part + (split * m + i) * n + j, along_i ? n : 1, k, v);
     }
-    __device__ __forceinline__ void operator()(const GemmUnit& q, long long i, int j0, int cols, const float* v) const {
+    __device__ __forceinline__ void operator()(const GemmUnit& q, long long i, int j0, int cols, const float* v,
+                                               const unsigned char*, unsigned char*) const {
         if (i < m) store32(part + (q.split * m + i) * n + j0, 1, cols, v);
     }
 };
+
+inline GemmIo io_of(const PartEpi&, long long, long long) { return {}; }
 
 // The parts in order, through the epilogue; threads along D's contiguous side.
 template <class Epi>
@@ -271,7 +320,7 @@ cudaError_t multiply_cut(const GemmMat* a, const GemmMat* b, long long rows, lon
     if (!fault) return cudaErrorInvalidSymbol;
     constexpr bool bf16 = !std::is_same<T, __half>::value;
     constexpr int PL = sizeof(T) == 4 ? 3 : 1;
-    return gemm_launch<PL>(a, b, rows, cols, k, 1, c, false, bf16, epi, fault, st);
+    return gemm_launch<PL>(a, b, rows, cols, k, 1, c, false, bf16, io_of(epi, rows, cols), epi, fault, st);
 }
 
 // D = A B^T through `epi`; part: room for the splits' parts.
@@ -279,7 +328,7 @@ template <class T, class Epi>
 cudaError_t multiply(const GemmMat* a, const GemmMat* b, long long rows, long long cols, long long k, const Cut& c,
                      char* part, const Epi& epi, cudaStream_t st) {
     if (c.splits == 1) return multiply_cut<T>(a, b, rows, cols, k, c, epi, st);
-    const cudaError_t e = multiply_cut<T>(a, b, rows, cols, k, c, PartEpi{(float*)part, rows, cols}, st);
+    const cudaError_t e = multiply_cut<T>(a, b, rows, cols, k, c, PartEpi{{}, (float*)part, rows, cols}, st);
     if (e != cudaSuccess) return e;
     join_kernel<<<(unsigned)((rows * cols + 255) / 256), 256, 0, st>>>((const float*)part, c.splits, rows, cols, epi);
     return cudaGetLastError();
@@ -308,7 +357,7 @@ template <class Epi>
 cudaError_t simt_multiply(const SimtOperand& a, const SimtOperand& b, long long rows, long long cols, long long k,
                           int splits, bool along_i, char* part, const Epi& epi, cudaStream_t st) {
     if (splits == 1) return simt_gemm(a, b, rows, cols, k, 1, along_i, epi, st);
-    const cudaError_t e = simt_gemm(a, b, rows, cols, k, splits, false, PartEpi{(float*)part, rows, cols}, st);
+    const cudaError_t e = simt_gemm(a, b, rows, cols, k, splits, false, PartEpi{{}, (float*)part, rows, cols}, st);
     if (e != cudaSuccess) return e;
     join_kernel<<<(unsigned)((rows * cols + 255) / 256), 256, 0, st>>>((const float*)part, splits, rows, cols, epi);
     return cudaGetLastError();
@@ -415,7 +464,7 @@ LinearEpi<T> epilogue(const phyzb_linear_args& a, bool rows_first) {
     auto turn = [&](auto* p, const int64_t* s) {
         return Out<std::remove_pointer_t<decltype(p)>>{p, rows_first ? s[0] : s[1], rows_first ? s[1] : s[0]};
     };
-    return {a.bias, !rows_first, a.activation, turn((const T*)a.residual, a.residual_stride), turn((T*)a.y, a.y_stride),
+    return {{}, a.bias, !rows_first, a.activation, turn((const T*)a.residual, a.residual_stride), turn((T*)a.y, a.y_stride),
             turn((T*)a.pre, a.pre_stride), rows_first ? a.m : a.n};
 }
 
@@ -657,7 +706,7 @@ template <class T>
 cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st) {
     const Out<T> dw{(T*)a.dw, a.dw_stride[0], a.dw_stride[1]};  // i = n
     if (a.m == 0) {  // no rows: sums of nothing
-        if (a.dw) join_kernel<<<(unsigned)((a.n * a.k + 255) / 256), 256, 0, st>>>(nullptr, 0, a.n, a.k, StoreEpi<T>{dw, a.n});
+        if (a.dw) join_kernel<<<(unsigned)((a.n * a.k + 255) / 256), 256, 0, st>>>(nullptr, 0, a.n, a.k, store_epi<T>(dw, a.n));
         if (a.dbias) column_sum_kernel<<<(unsigned)((a.n + 31) / 32), 1024, 0, st>>>(nullptr, 0, a.n, a.dbias);
         return cudaGetLastError();
     }
@@ -713,14 +762,15 @@ cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st)
             if (p.simt_dx) {
                 e = simt_multiply({(const float*)zp, zr, zn}, {(const float*)a.w, a.w_stride[1], a.w_stride[0]}, a.m, a.k,
                                   a.n, p.split_dx, rf, part,
-                                  StoreEpi<T>{{(T*)a.dx, a.dx_stride[0], a.dx_stride[1]}, a.m}, st);
+                                  store_epi<T>({(T*)a.dx, a.dx_stride[0], a.dx_stride[1]}, a.m), st);
             }
         }
         if (!p.simt_dx) {
             GemmMat w[3];
             e = Backward::w_of(a).ready(ws + p.ws_w, w, st);
             if (e != cudaSuccess) return e;
-            const StoreEpi<T> epi{{(T*)a.dx, a.dx_stride[rf ? 0 : 1], a.dx_stride[rf ? 1 : 0]}, rf ? a.m : a.k};
+            const StoreEpi<T> epi =
+                store_epi<T>({(T*)a.dx, a.dx_stride[rf ? 0 : 1], a.dx_stride[rf ? 1 : 0]}, rf ? a.m : a.k);
             e = multiply<T>(rf ? dz : w, rf ? w : dz, rf ? a.m : a.k, rf ? a.k : a.m, a.n, p.cut_dx, part, epi, st);
         }
         if (e != cudaSuccess) return e;
@@ -730,15 +780,15 @@ cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st)
             if (p.simt_dw)
                 return simt_multiply({(const float*)zp, zn, zr}, {(const float*)a.x, a.x_stride[1], a.x_stride[0]}, a.n,
                                      a.k, a.m, p.split_dw, false, part,
-                                     StoreEpi<T>{dw, a.n}, st);
+                                     store_epi<T>(dw, a.n), st);
         }
         GemmMat x[3];
         e = Backward::x_of(a).ready(ws + p.ws_x, x, st);
         if (e != cudaSuccess) return e;
         if (p.dw_n_first)
-            e = multiply<T>(dzt, x, a.n, a.k, a.m, p.cut_dw, part, StoreEpi<T>{dw, a.n}, st);
+            e = multiply<T>(dzt, x, a.n, a.k, a.m, p.cut_dw, part, store_epi<T>(dw, a.n), st);
         else
-            e = multiply<T>(x, dzt, a.k, a.n, a.m, p.cut_dw, part, StoreEpi<T>{{dw.p, dw.js, dw.is}, a.k}, st);
+            e = multiply<T>(x, dzt, a.k, a.n, a.m, p.cut_dw, part, store_epi<T>({dw.p, dw.js, dw.is}, a.k), st);
     }
     return e;
 }

@@ -60,11 +60,6 @@ __device__ __forceinline__ float load_as(const void* p, long long e, int dtype) 
 struct Pair {
     __half* p = nullptr;
     long long lo = 0, zs = 0, pitch = 0;  // offset of the low plane; strides
-    __device__ __forceinline__ void put(long long e, float v) const {
-        const __half h = __float2half_rn(v);
-        p[e] = h;
-        p[e + lo] = __float2half_rn(v - __half2float(h));
-    }
 };
 
 // V neighbours of row r from column c: momentum advanced (ADVANCE) or as it is,
@@ -176,65 +171,74 @@ __global__ void __launch_bounds__(256) normalize_kernel(const __grid_constant__ 
 
 // ── epilogues: D is at SCALE^2 ────────────────────────────────────────────
 
-// 32 neighbours of a pair's row
-__device__ __forceinline__ void pair_load(const Pair& x, long long e, int n, float* v) {
+// a lane's 32 values of a slot's pair
+__device__ __forceinline__ void pair_load(const unsigned char* in, float* v) {
     __half h[32], l[32];
-    load32(x.p + e, 1, n, h);
-    load32(x.p + x.lo + e, 1, n, l);
+    slot_load(in, reinterpret_cast<uint32_t*>(h));
+    slot_load(in + GEMM_PLANE, reinterpret_cast<uint32_t*>(l));
 #pragma unroll
     for (int k = 0; k < 32; k++) v[k] = __half2float(h[k]) + __half2float(l[k]);
 }
-__device__ __forceinline__ void pair_store(const Pair& x, long long e, int n, const float* v) {
-    __half h[32], l[32];
+__device__ __forceinline__ void split(const float* v, __half* h, __half* l) {
 #pragma unroll
     for (int k = 0; k < 32; k++) {
         h[k] = __float2half_rn(v[k]);
         l[k] = __float2half_rn(v[k] - __half2float(h[k]));
     }
-    store32(x.p + e, 1, n, h);
-    store32(x.p + x.lo + e, 1, n, l);
 }
 
-// G = sum, or b G + c sum, and its mirror image: D[i][j] = D[j][i].
+// G = sum, or b G + c sum, and its mirror image: D[i][j] = D[j][i]. (The pairs are
+// in the workspace: all of this goes through slots.)
 struct SquareEpi {
-    Pair out, g;
+    static constexpr int PLANES = 2, SLOTS = 1;
+    static constexpr bool MIRROR = true;
     float b, c;  // c / SCALE
-    int s;
-    __device__ __forceinline__ void operator()(const GemmUnit& q, long long i, int j0, int cols, const float* sum) const {
-        if (i >= s) return;
-        const long long z = q.z * out.zs, e = z + i * out.pitch + j0;
+    // the tile's mirror image is another one, unless it is inside a diagonal block
+    __device__ __forceinline__ bool mirrored(const GemmUnit& q, int j0) const { return j0 < q.row0; }
+    __device__ __forceinline__ void operator()(const GemmUnit& q, long long i, int j0, int cols, float* sum,
+                                               const unsigned char* in, unsigned char* out) const {
         float v[32];
-        if (g.p) pair_load(g, e, cols, v);
+        if (in) pair_load(in, v);
 #pragma unroll
-        for (int k = 0; k < 32; k++) v[k] = g.p ? fmaf(b, v[k], c * sum[k]) : c * sum[k];
-        pair_store(out, e, cols, v);
-        // the tile's mirror image, unless it is inside a diagonal block
-        if (j0 < q.row0) {
+        for (int k = 0; k < 32; k++) sum[k] = in ? fmaf(b, v[k], c * sum[k]) : c * sum[k];
+        __half h[32], l[32];
+        split(sum, h, l);
+        slot_store(out, reinterpret_cast<const uint32_t*>(h));
+        slot_store(out + GEMM_PLANE, reinterpret_cast<const uint32_t*>(l));
+    }
+    __device__ __forceinline__ void turn(const float* v, unsigned char* out) const {
+        __half h[32], l[32];
+        split(v, h, l);
+        const int lane = threadIdx.x % 32;
 #pragma unroll
-            for (int k = 0; k < 32; k++)
-                if (k < cols) out.put(z + (j0 + k) * out.pitch + i, v[k]);
+        for (int k = 0; k < 32; k++) {
+            *reinterpret_cast<__half*>(out + slot_at(k, lane)) = h[k];
+            *reinterpret_cast<__half*>(out + GEMM_PLANE + slot_at(k, lane)) = l[k];
         }
     }
 };
 
 // a X + sum; i along the rows of X, j along its columns.
 struct StepEpi {
-    Pair x, out;
-    int rows;
-    __device__ __forceinline__ void operator()(const GemmUnit& q, long long i, int j0, int cols, const float* sum) const {
-        if (i >= rows) return;
-        const long long e = q.z * x.zs + i * x.pitch + j0;
+    static constexpr int PLANES = 2, SLOTS = 1;
+    static constexpr bool MIRROR = false;
+    __device__ __forceinline__ void operator()(const GemmUnit&, long long, int, int, const float* sum,
+                                               const unsigned char* in, unsigned char* out) const {
         float v[32];
-        pair_load(x, e, cols, v);
+        pair_load(in, v);
 #pragma unroll
         for (int k = 0; k < 32; k++) v[k] = fmaf(NS_A, v[k], sum[k] * (1.0f / SCALE));
-        pair_store(out, e, cols, v);
+        __half h[32], l[32];
+        split(v, h, l);
+        slot_store(out, reinterpret_cast<const uint32_t*>(h));
+        slot_store(out + GEMM_PLANE, reinterpret_cast<const uint32_t*>(l));
     }
 };
 
 // The last a X + sum, into the weights or the result.
 struct LastEpi {
-    Pair x;
+    static constexpr int PLANES = 2, SLOTS = 1;
+    static constexpr bool MIRROR = false;
     Problem q;
     template <class T>
     __device__ __forceinline__ static void write(const View& o, long long z, long long i, int j0, int cols,
@@ -250,10 +254,11 @@ struct LastEpi {
         if (dtype == PHYZB_DT_BF16) return write<__nv_bfloat16>(o, z, i, j0, cols, v);
         return write<__half>(o, z, i, j0, cols, v);
     }
-    __device__ __forceinline__ void operator()(const GemmUnit& u, long long i, int j0, int cols, const float* sum) const {
+    __device__ __forceinline__ void operator()(const GemmUnit& u, long long i, int j0, int cols, float* sum,
+                                               const unsigned char* in, unsigned char*) const {
         if (i >= q.rows) return;
         float v[32];
-        pair_load(x, u.z * x.zs + i * x.pitch + j0, cols, v);
+        pair_load(in, v);
 #pragma unroll
         for (int k = 0; k < 32; k++) v[k] = fmaf(NS_A, v[k], sum[k] * (1.0f / SCALE)) * (1.0f / SCALE);
         if (q.out.p) return write(q.out, q.out_dtype, u.z, i, j0, cols, v);
@@ -296,17 +301,26 @@ Ws layout(long long batch, long long rows, long long cols) {
     return w;
 }
 
-// D = A B^T on pairs.
+// D = A B^T on pairs; the epilogue reads `in` and writes `out` (either may be
+// absent), pairs of D's shape.
 template <class Epi>
 cudaError_t multiply(const Pair& a, bool a_mn, const Pair& b, bool b_mn, long long rows, long long cols, long long k,
-                     int batch, bool symmetric, const Epi& epi, unsigned int* fault, cudaStream_t st) {
+                     int batch, bool symmetric, const Pair& in, const Pair& out, const Epi& epi, unsigned int* fault,
+                     cudaStream_t st) {
     GemmMat ma[2], mb[2];
+    GemmIo io{};
     for (int h = 0; h < 2; h++) {
         ma[h] = {a.p + h * a.lo, a_mn ? 1 : a.pitch, a_mn ? a.pitch : 1, a.zs};
         mb[h] = {b.p + h * b.lo, b_mn ? 1 : b.pitch, b_mn ? b.pitch : 1, b.zs};
+        if (in.p && !gemm_io_map(&io.in[h], in.p + h * in.lo, in.pitch, 1, in.zs, rows, cols, batch, false))
+            return cudaErrorInvalidValue;
+        if (out.p && !gemm_io_map(&io.out[h], out.p + h * out.lo, out.pitch, 1, out.zs, rows, cols, batch, false))
+            return cudaErrorInvalidValue;
     }
+    io.reads = in.p != nullptr;
+    io.writes = out.p != nullptr;
     const GemmCut cut = gemm_cut(rows, cols, k, batch, 3, symmetric, false);
-    return gemm_launch<2>(ma, mb, rows, cols, k, batch, cut, symmetric, false, epi, fault, st);
+    return gemm_launch<2>(ma, mb, rows, cols, k, batch, cut, symmetric, false, io, epi, fault, st);
 }
 
 cudaError_t solve(const Problem& q, char* ws, cudaStream_t st) {
@@ -338,16 +352,16 @@ cudaError_t solve(const Problem& q, char* ws, cudaStream_t st) {
     Pair x = o.x, y = o.y;
     for (int k = 0; k < q.steps && e == cudaSuccess; k++) {
         // G: the short side's products along the long one
-        e = multiply(x, tall, x, tall, s, s, l, q.batch, true, SquareEpi{o.g, Pair{}, 0.0f, 1.0f / SCALE, s}, fault, st);
+        e = multiply(x, tall, x, tall, s, s, l, q.batch, true, Pair{}, o.g, SquareEpi{0.0f, 1.0f / SCALE}, fault, st);
         if (e != cudaSuccess) break;
-        e = multiply(o.g, false, o.g, false, s, s, s, q.batch, true, SquareEpi{o.p, o.g, NS_B, NS_C / SCALE, s}, fault, st);
+        e = multiply(o.g, false, o.g, false, s, s, s, q.batch, true, o.g, o.p, SquareEpi{NS_B, NS_C / SCALE}, fault, st);
         if (e != cudaSuccess) break;
         // i = rows of X, j = columns. Wide: P's rows by X^T's; tall: X's rows by P's
         const Pair &a = tall ? x : o.p, &b = tall ? o.p : x;
         if (k + 1 < q.steps)
-            e = multiply(a, false, b, !tall, q.rows, q.cols, s, q.batch, false, StepEpi{x, y, q.rows}, fault, st);
+            e = multiply(a, false, b, !tall, q.rows, q.cols, s, q.batch, false, x, y, StepEpi{}, fault, st);
         else
-            e = multiply(a, false, b, !tall, q.rows, q.cols, s, q.batch, false, LastEpi{x, q}, fault, st);
+            e = multiply(a, false, b, !tall, q.rows, q.cols, s, q.batch, false, x, Pair{}, LastEpi{q}, fault, st);
         const Pair t = x;
         x = y;
         y = t;
