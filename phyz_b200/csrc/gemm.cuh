@@ -3,8 +3,8 @@
 //
 // One persistent block per SM walks tiles of D. Warp 0 brings 64-deep stages of
 // both operands by TMA into 128-byte-swizzled shared memory, warp 1 issues
-// tcgen05.mma into one of two accumulators in Tensor Memory, and eight more warps
-// empty the other one through the epilogue, so that the tensor cores wait neither
+// tcgen05.mma into one of two accumulators in Tensor Memory, and eight or
+// sixteen more warps empty the other one through the epilogue, so that the tensor cores wait neither
 // for memory nor for the epilogue. In the epilogue a lane has 32 neighbours in j
 // and a warp 32 in i: a chunk. Where TMA can address them, what the epilogue reads
 // comes into the warp's own slots of shared memory a chunk ahead and what it
@@ -33,8 +33,6 @@
 namespace pz {
 
 constexpr int GEMM_BM = 128, GEMM_BK = 64;
-constexpr int GEMM_EPI_WARPS = 8;
-constexpr int GEMM_THREADS = 32 * (2 + GEMM_EPI_WARPS);
 constexpr int GEMM_SMS = 148;
 
 // A chunk's slot: 32 rows of 32 16-bit values, one or two planes.
@@ -47,11 +45,13 @@ struct GemmShape {
     static constexpr int A_BYTES = GEMM_BM * GEMM_BK * 2, B_BYTES = BR * GEMM_BK * 2;
     static constexpr int STAGE = PL * (A_BYTES + B_BYTES);
     static constexpr int WARP_SLOTS = Epi::PLANES * Epi::SLOTS * GEMM_PLANE;
-    static constexpr int SLOTS = GEMM_EPI_WARPS * WARP_SLOTS;
+    static constexpr int THREADS = 32 * (2 + Epi::WARPS);
+    static constexpr int SLOTS = Epi::WARPS * WARP_SLOTS;
     static constexpr int FIT = (224 * 1024 - SLOTS) / STAGE;
     static constexpr int STAGES = FIT > 6 ? 6 : FIT;
     static constexpr int ACCS = PL > 1 ? 2 : 1;      // main, small terms
-    static constexpr int COLS = 2 * ACCS * BN;       // two tiles in flight
+    static constexpr int BUFS = 2 * ACCS * BN <= 512 ? 2 : 1;  // tiles in Tensor Memory
+    static constexpr int COLS = BUFS * ACCS * BN;
     static constexpr int BYTES = STAGES * STAGE + SLOTS + 1024 + 512;
     static_assert(BYTES <= 227 * 1024);
     static_assert(COLS <= 512 && STAGES >= 2 && BR >= 64);
@@ -194,7 +194,7 @@ __device__ __forceinline__ GemmUnit gemm_unit(const GemmArgs& g, int u) {
     GemmUnit q;
     constexpr int W = ROWS / BN;  // tiles across a diagonal block
     const int tiles = g.symmetric ? W * g.ti * (g.ti + 1) / 2 : g.ti * g.tj;
-    const int t = u % tiles, r = u / tiles;
+    const int r = u < tiles ? 0 : u / tiles, t = u - r * tiles;
     if (g.symmetric) {  // row i has W (i + 1) tiles
         int i = (int)((sqrtf(8.0f * (t / W) + 1.0f) - 1.0f) * 0.5f);
         while (W * (i + 1) * (i + 2) / 2 <= t) i++;
@@ -205,12 +205,13 @@ __device__ __forceinline__ GemmUnit gemm_unit(const GemmArgs& g, int u) {
         // the side with fewer tiles first: the other operand's tile is then read by
         // neighbours at the same time, and comes from memory once
         const bool i_first = g.ti <= g.tj;
-        q.i = i_first ? t % g.ti : t / g.tj;
-        q.j = i_first ? t / g.ti : t % g.tj;
+        const int fast = i_first ? g.ti : g.tj, slow = t / fast;
+        q.i = i_first ? t - slow * fast : slow;
+        q.j = i_first ? slow : t - slow * fast;
     }
     q.row0 = q.i * ROWS;
-    q.split = r % g.splits;
-    q.z = r / g.splits;
+    q.z = r < g.splits ? 0 : r / g.splits;
+    q.split = r - q.z * g.splits;
     q.k0 = q.split * g.per;
     q.k1 = q.k0 + g.per < g.kblocks ? q.k0 + g.per : g.kblocks;
     return q;
@@ -251,10 +252,10 @@ __device__ __forceinline__ int slot_at(int row, int col) { return row * 64 + (((
 
 // Epi: void operator()(const GemmUnit&, long long i, int j0, int cols, float* sum, const unsigned char* in, unsigned
 // char* out) const for 32 columns from j0 (cols of them inside D) of row i, called by whole warps (rows past m too).
-// in, out: the chunk's slot where GemmIo says so (the same one), else null. PLANES of a slot, SLOTS of a warp. MIRROR:
+// in, out: the chunk's slot where GemmIo says so (the same one), else null. PLANES of a slot, SLOTS of a warp, 4 to 16 WARPS. MIRROR:
 // where mirrored(unit, j0) says so, the chunk's mirror image is written as well, by turn(sum, slot).
 template <int BN, int PL, int CTAS, class Epi>
-__global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
+__global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL, CTAS, Epi>::THREADS), 1)
     gemm_kernel(const __grid_constant__ GemmArgs g, const __grid_constant__ Epi epi, unsigned int* fault) {
     using S = GemmShape<BN, PL, CTAS, Epi>;
     extern __shared__ unsigned char raw[];
@@ -267,7 +268,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
     uint64_t* const acc_empty = acc_full + 2;
     uint64_t* const done = acc_empty + 2;
     uint64_t* const slot_full = done + 1;
-    uint32_t* const slot = reinterpret_cast<uint32_t*>(slot_full + GEMM_EPI_WARPS * Epi::SLOTS);
+    uint32_t* const slot = reinterpret_cast<uint32_t*>(slot_full + Epi::WARPS * Epi::SLOTS);
     volatile uint32_t* const gave_up = slot + 1;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rank = CTAS == 2 ? blockIdx.x % 2 : 0;  // in the cluster; the first one leads
@@ -278,10 +279,10 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
         }
         for (int k = 0; k < 2; k++) {
             mbar_init(&acc_full[k], 1);
-            mbar_init(&acc_empty[k], CTAS * GEMM_EPI_WARPS);
+            mbar_init(&acc_empty[k], CTAS * Epi::WARPS);
         }
         mbar_init(done, 1);
-        for (int k = 0; k < GEMM_EPI_WARPS * Epi::SLOTS; k++) mbar_init(&slot_full[k], 1);
+        for (int k = 0; k < Epi::WARPS * Epi::SLOTS; k++) mbar_init(&slot_full[k], 1);
         *gave_up = 0;
         mbar_init_fence();
         for (int k = 0; k < PL; k++) {
@@ -374,7 +375,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
                     if (++stage == S::STAGES) stage = 0, phase ^= 1;
                 }
                 if (ok) mma_commit<CTAS>(&acc_full[acc]);
-                if (++acc == 2) acc = 0, aphase ^= 1;
+                if (++acc == S::BUFS) acc = 0, aphase ^= 1;
             }
             if (!ok) {  // not before what was issued has finished
                 mma_commit<CTAS>(done);
@@ -383,12 +384,13 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
         }
     } else {
         // lanes 32 (warp % 4) .. of the accumulator are this warp's to read
-        const int quarter = warp % 4, half = (warp - 2) / 4, own = rank * GEMM_BM + quarter * 32;
+        const int quarter = warp % 4, from = (warp - 2) / 4 * 32, own = rank * GEMM_BM + quarter * 32;
+        constexpr int EVERY = Epi::WARPS * 8;  // columns from one of a warp's chunks to the next
         constexpr int NS = Epi::SLOTS, MOD = NS > 0 ? NS : 1;
         unsigned char* const mine = slots + (warp - 2) * S::WARP_SLOTS;
         uint64_t* const bars = slot_full + (warp - 2) * NS;
         // lane 0's place in the sequence of chunks, ahead of the warp's
-        int au = first, ac = half * 32, asked = 0;
+        int au = first, ac = from, asked = 0;
         GemmUnit aq{};
         if (au < g.units) aq = gemm_unit<BN, S::ROWS>(g, au);
         auto request = [&]() {
@@ -401,10 +403,10 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
                     for (int p = 0; p < Epi::PLANES; p++)
                         tma_load(at + p * GEMM_PLANE, &g.io.in[p], &bars[asked % MOD], aq.j * BN + ac, aq.row0 + own, aq.z);
                     asked++;
-                    ac += 64;
+                    ac += EVERY;
                     return;
                 }
-                ac = half * 32;
+                ac = from;
                 au += step;
                 if (au < g.units) aq = gemm_unit<BN, S::ROWS>(g, au);
             }
@@ -423,7 +425,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
             const uint32_t d = tmem + acc * S::ACCS * BN + ((uint32_t)quarter * 32 << 16);
             const long long i = q.row0 + own + lane;
             const bool any = q.k0 < q.k1;
-            for (int c = half * 32; c < BN; c += 64) {
+            for (int c = from; c < BN; c += EVERY) {
                 const int j = q.j * BN + c, cols = g.n - j < 32 ? g.n - j : 32;
                 if (cols <= 0 || q.row0 + own >= g.m) break;
                 unsigned char* const at = mine + n % MOD * Epi::PLANES * GEMM_PLANE;
@@ -506,7 +508,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
                 else
                     mbar_arrive(&acc_empty[acc]);
             }
-            if (++acc == 2) acc = 0, aphase ^= 1;
+            if (++acc == S::BUFS) acc = 0, aphase ^= 1;
         }
         if constexpr (NS > 0) {
             if (lane == 0) {
@@ -602,7 +604,7 @@ inline GemmCut gemm_cut(long long rows, long long cols, long long k, long long b
     GemmCut best{};
     double least = 0;
     for (const auto& s : shapes) {
-        if (products > 1 && s.bn == 256) continue;  // (Tensor Memory holds two tiles of two accumulators)
+        if (products > 3 && s.bn == 256) continue;  // (three planes of it do not fit shared memory twice)
         const long long r = GEMM_BM * s.ctas, ti = (rows + r - 1) / r, tj = (cols + s.bn - 1) / s.bn;
         const long long tiles = (symmetric ? r / s.bn * ti * (ti + 1) / 2 : ti * tj) * batch;
         const long long slots = GEMM_SMS / s.ctas;
@@ -654,7 +656,7 @@ cudaError_t gemm_launch_as(const GemmMat* a, const GemmMat* b, long long ma, lon
     const cudaError_t e = once.smem(kernel, S::BYTES);
     if (e != cudaSuccess) return e;
     const int slots = GEMM_SMS / CTAS;
-    kernel<<<(g.units < slots ? g.units : slots) * CTAS, GEMM_THREADS, S::BYTES, st>>>(g, epi, fault);
+    kernel<<<(g.units < slots ? g.units : slots) * CTAS, S::THREADS, S::BYTES, st>>>(g, epi, fault);
     return cudaGetLastError();
 }
 
@@ -662,7 +664,7 @@ template <int PL, class Epi>
 cudaError_t gemm_launch(const GemmMat* a, const GemmMat* b, long long ma, long long nb, long long k, int batch,
                         const GemmCut& c, bool symmetric, bool bf16, const GemmIo& io, const Epi& epi,
                         unsigned int* fault, cudaStream_t st) {
-    if constexpr (PL == 1)
+    if constexpr (PL <= 2)
         if (c.ctas == 2 && c.bn == 256)
             return gemm_launch_as<256, PL, 2>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, io, epi, fault, st);
     if (c.ctas == 2) return gemm_launch_as<128, PL, 2>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, io, epi, fault, st);

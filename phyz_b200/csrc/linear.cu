@@ -81,7 +81,7 @@ __device__ __forceinline__ void store4(float* p, long long stride, int n, const 
 // beside their six products, and go straight.
 template <class T>
 struct Slotted {
-    static constexpr int PLANES = sizeof(T) == 2 ? 1 : 0, SLOTS = sizeof(T) == 2 ? 4 : 0;
+    static constexpr int PLANES = sizeof(T) == 2 ? 1 : 0, SLOTS = sizeof(T) == 2 ? 4 : 0, WARPS = 8;
     static constexpr bool MIRROR = false;
 };
 

@@ -190,7 +190,7 @@ __device__ __forceinline__ void split(const float* v, __half* h, __half* l) {
 // G = sum, or b G + c sum, and its mirror image: D[i][j] = D[j][i]. (The pairs are
 // in the workspace: all of this goes through slots.)
 struct SquareEpi {
-    static constexpr int PLANES = 2, SLOTS = 1;
+    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8;
     static constexpr bool MIRROR = true;
     float b, c;  // c / SCALE
     // the tile's mirror image is another one, unless it is inside a diagonal block
@@ -220,7 +220,7 @@ struct SquareEpi {
 
 // a X + sum; i along the rows of X, j along its columns.
 struct StepEpi {
-    static constexpr int PLANES = 2, SLOTS = 1;
+    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8;
     static constexpr bool MIRROR = false;
     __device__ __forceinline__ void operator()(const GemmUnit&, long long, int, int, const float* sum,
                                                const unsigned char* in, unsigned char* out) const {
@@ -237,7 +237,7 @@ struct StepEpi {
 
 // The last a X + sum, into the weights or the result.
 struct LastEpi {
-    static constexpr int PLANES = 2, SLOTS = 1;
+    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8;
     static constexpr bool MIRROR = false;
     Problem q;
     template <class T>
