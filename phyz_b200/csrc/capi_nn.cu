@@ -3,6 +3,7 @@
 // device memory or waits for the device.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <exception>
 #include <string>
@@ -68,10 +69,14 @@ int check_array(const void* p, const int64_t* stride, const int64_t* size, int n
 int esize(int dtype) { return dtype == PHYZB_DT_F32 ? 4 : 2; }
 
 int check_device(int device) {
-    int ndev = 0;
-    if (cudaGetDeviceCount(&ndev) != cudaSuccess || ndev < 1) {
-        cudaGetLastError();
-        return fail(PHYZB_ERR_NO_DEVICE, "no CUDA device");
+    static std::atomic<int> count{0};  // devices do not come and go in a process
+    int ndev = count.load(std::memory_order_relaxed);
+    if (ndev < 1) {
+        if (cudaGetDeviceCount(&ndev) != cudaSuccess || ndev < 1) {
+            cudaGetLastError();
+            return fail(PHYZB_ERR_NO_DEVICE, "no CUDA device");
+        }
+        count.store(ndev, std::memory_order_relaxed);
     }
     if (device < 0 || device >= ndev) return bad("device " + std::to_string(device) + " out of range");
     return PHYZB_OK;

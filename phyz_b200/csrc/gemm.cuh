@@ -178,9 +178,9 @@ __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::l
 
 // Shared-memory descriptor of a 128-byte-swizzled operand stage. k contiguous:
 // rows of 128 bytes, groups of eight 1024 bytes apart. Rows contiguous: blocks
-// of 64 rows (64 k lines of 128 bytes) 8192 bytes apart, eight k lines 1024.
-__device__ __forceinline__ uint64_t gemm_desc(uint32_t addr, int mn) {
-    const uint64_t lead = mn ? 8192 >> 4 : 1;
+// of 64 rows (k lines of 128 bytes) `block` bytes apart, eight k lines 1024.
+__device__ __forceinline__ uint64_t gemm_desc(uint32_t addr, int mn, int block = 8192) {
+    const uint64_t lead = mn ? block >> 4 : 1;
     return (uint64_t)((addr >> 4) & 0x3fff) | lead << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
            (uint64_t)2 << 61;
 }

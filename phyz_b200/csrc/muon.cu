@@ -241,18 +241,32 @@ struct LastEpi {
     static constexpr bool MIRROR = false;
     Problem q;
     template <class T>
-    __device__ __forceinline__ static void write(const View& o, long long z, long long i, int j0, int cols,
-                                                 const float* v) {
+    __device__ __forceinline__ static void write(const View& o, long long at, long long stride, int n, const float* v) {
         T t[32];
 #pragma unroll
         for (int k = 0; k < 32; k++) t[k] = from_f32<T>(v[k]);
-        store32((T*)o.p + z * o.zs + i * o.rs + j0 * o.cs, o.cs, cols, t);
+        store32((T*)o.p + at, stride, n, t);
     }
-    __device__ __forceinline__ static void write(const View& o, int dtype, long long z, long long i, int j0, int cols,
+    __device__ __forceinline__ static void write(const View& o, int dtype, long long at, long long stride, int n,
                                                  const float* v) {
-        if (dtype == PHYZB_DT_F32) return write<float>(o, z, i, j0, cols, v);
-        if (dtype == PHYZB_DT_BF16) return write<__nv_bfloat16>(o, z, i, j0, cols, v);
-        return write<__half>(o, z, i, j0, cols, v);
+        if (dtype == PHYZB_DT_F32) return write<float>(o, at, stride, n, v);
+        if (dtype == PHYZB_DT_BF16) return write<__nv_bfloat16>(o, at, stride, n, v);
+        return write<__half>(o, at, stride, n, v);
+    }
+    // n values (at SCALE) of matrix z from (r, c) along c, or down r
+    __device__ __forceinline__ void finish(long long z, long long r, long long c, bool down, int n, float* v) const {
+        auto at = [&](const View& o) { return z * o.zs + r * o.rs + c * o.cs; };
+        auto stride = [&](const View& o) { return down ? o.rs : o.cs; };
+#pragma unroll
+        for (int k = 0; k < 32; k++) v[k] *= 1.0f / SCALE;
+        if (q.out.p) return write(q.out, q.out_dtype, at(q.out), stride(q.out), n, v);
+        float old[32];
+        float* w = (float*)q.w.p + at(q.w);
+        load32(w, stride(q.w), n, old);
+#pragma unroll
+        for (int k = 0; k < 32; k++) v[k] = fmaf(-q.lr, v[k], q.decay * old[k]);
+        store32(w, stride(q.w), n, v);
+        if (q.copy.p) write(q.copy, q.copy_dtype, at(q.copy), stride(q.copy), n, v);
     }
     __device__ __forceinline__ void operator()(const GemmUnit& u, long long i, int j0, int cols, float* sum,
                                                const unsigned char* in, unsigned char*) const {
@@ -260,17 +274,183 @@ struct LastEpi {
         float v[32];
         pair_load(in, v);
 #pragma unroll
-        for (int k = 0; k < 32; k++) v[k] = fmaf(NS_A, v[k], sum[k] * (1.0f / SCALE)) * (1.0f / SCALE);
-        if (q.out.p) return write(q.out, q.out_dtype, u.z, i, j0, cols, v);
-        float old[32];
-        float* w = (float*)q.w.p + u.z * q.w.zs + i * q.w.rs + j0 * q.w.cs;
-        load32(w, q.w.cs, cols, old);
-#pragma unroll
-        for (int k = 0; k < 32; k++) v[k] = fmaf(-q.lr, v[k], q.decay * old[k]);
-        store32(w, q.w.cs, cols, v);
-        if (q.copy.p) write(q.copy, q.copy_dtype, u.z, i, j0, cols, v);
+        for (int k = 0; k < 32; k++) v[k] = fmaf(NS_A, v[k], sum[k] * (1.0f / SCALE));
+        finish(u.z, i, j0, false, cols, v);
     }
 };
+
+// ── small matrices: all of it in one block ───────────────────────────────
+
+// s <= 128 and l <= LB: X, G and P stay in shared memory as f16 pairs, the
+// accumulators in Tensor Memory, and one launch does the whole update. X is
+// [128 rows][l] in blocks of 64 columns, 128-byte swizzled: as it lies it is the
+// operand with k along l (X X^T) and the one with k along its rows (P X). What is
+// left of five iterations is latency: three products of a microsecond and their
+// epilogues each, against five launches' worth of it for every product.
+constexpr int SMALL_THREADS = 512;
+constexpr int SMALL_BLOCK = 128 * 128;  // bytes of 128 rows of 64 values
+
+template <int LB>
+struct Small {
+    static constexpr int X = LB / 64 * SMALL_BLOCK, G = 2 * SMALL_BLOCK;  // bytes of a plane
+    static constexpr int BYTES = 2 * X + 2 * G + 1024 + 128;
+};
+
+// bytes of value (row, col) in a plane
+__device__ __forceinline__ int small_at(int row, int col) {
+    return (col >> 6) * SMALL_BLOCK + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2;
+}
+// 32 columns from c (a multiple of 32) of a lane's row
+__device__ __forceinline__ void small_load(const unsigned char* hi, int lo, int row, int c, float* v) {
+#pragma unroll
+    for (int p = 0; p < 2; p++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            __half t[8];
+            *(uint4*)t = *(const uint4*)(hi + p * lo + small_at(row, c + q * 8));
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[q * 8 + e] = p ? v[q * 8 + e] + __half2float(t[e]) : __half2float(t[e]);
+        }
+}
+__device__ __forceinline__ void small_store(unsigned char* hi, int lo, int row, int c, const float* v) {
+    __half h[32], l[32];
+    split(v, h, l);
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        *(uint4*)(hi + small_at(row, c + q * 8)) = *(const uint4*)(h + q * 8);
+        *(uint4*)(hi + lo + small_at(row, c + q * 8)) = *(const uint4*)(l + q * 8);
+    }
+}
+// the sum of an accumulator and its small terms
+__device__ __forceinline__ void small_sum(uint32_t main, uint32_t small, float* v) {
+    float w[32];
+    tmem_load(main, v);
+    tmem_load(small, w);
+    tmem_load_wait();
+#pragma unroll
+    for (int e = 0; e < 32; e++) v[e] += w[e];
+}
+
+template <int LB, int V>
+__global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_constant__ Problem q, unsigned int* fault) {
+    using C = Small<LB>;
+    extern __shared__ unsigned char raw[];
+    __shared__ float sums[SMALL_THREADS / 32];
+    unsigned char* const X = raw + (1024 - (smem_addr(raw) & 1023)) % 1024;
+    unsigned char* const G = X + 2 * C::X;
+    uint64_t* const bar = reinterpret_cast<uint64_t*>(G + 2 * C::G);
+    uint32_t* const slot = reinterpret_cast<uint32_t*>(bar + 1);
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, z = blockIdx.x;
+    const bool tall = q.rows > q.cols;
+    const int s = tall ? q.cols : q.rows, l = tall ? q.rows : q.cols;
+    if (tid == 0) {
+        mbar_init(bar, 1);
+        mbar_init_fence();
+    }
+    if (warp == 0) tmem_alloc<1>(slot, 512);
+    // momentum and |u|^2, then X = u / |u| as pairs, zeros around it
+    const int per = q.cols / V, n = per * q.rows;
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int e = tid; e < n; e += SMALL_THREADS) {
+        const int r = e / per, c = (e - r * per) * V;
+        float u[V];
+        direction<V, true>(q, z, r, c, u);
+#pragma unroll
+        for (int v = 0; v < V; v++) sum = fmaf(u[v], u[v], sum);
+    }
+    for (int e = tid; e < 2 * C::X / 16; e += SMALL_THREADS) reinterpret_cast<uint4*>(X)[e] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int o = 16; o; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sums[warp] = sum;
+    mma_fence_before();
+    __syncthreads();
+    mma_fence_after();
+    const uint32_t tmem = *slot;
+    float norm = 0.0f;
+#pragma unroll
+    for (int w = 0; w < SMALL_THREADS / 32; w++) norm += sums[w];
+    const float scale = SCALE / (sqrtf(norm) + NS_EPS);
+#pragma unroll 4
+    for (int e = tid; e < n; e += SMALL_THREADS) {
+        const int r = e / per, c = (e - r * per) * V;
+        float u[V];
+        direction<V, false>(q, z, r, c, u);
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const float x = u[v] * scale;
+            const __half h = __float2half_rn(x);
+            unsigned char* const at = X + (tall ? small_at(c + v, r) : small_at(r, c + v));
+            *(__half*)at = h;
+            *(__half*)(at + C::X) = __float2half_rn(x - __half2float(h));
+        }
+    }
+    const int quarter = warp % 4, from = warp / 4 * 32, row = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)quarter * 32 << 16);
+    const int ns = (s + 15) / 16 * 16, nl = (l + 15) / 16 * 16;
+    constexpr uint32_t GS = 128, P = 256, PS = 384, XS = 256;  // columns: G at 0, its small terms, P's, X's small terms
+    int phase = 0;
+    bool ok = true;
+    // D (main, small) = A B^T on pairs, K in steps of 16; then every thread waits
+    auto product = [&](uint32_t main, uint32_t small, const unsigned char* A, int a_lo, const unsigned char* B, int b_lo,
+                       bool b_mn, int cols, int ksteps) {
+        fence_async();
+        mma_fence_before();
+        ok = __syncthreads_and(ok);
+        mma_fence_after();
+        if (!ok) return;
+        if (tid == 0) {
+            const uint32_t idesc = 1u << 4 | (uint32_t)b_mn << 16 | (uint32_t)(cols >> 3) << 17 | (128u >> 4) << 24;
+            for (int k = 0; k < ksteps; k++)
+#pragma unroll
+                for (int p = 0; p < 3; p++) {  // hi hi; hi lo, lo hi
+                    const uint32_t a = smem_addr(A) + (p == 2 ? a_lo : 0) + (k >> 2) * SMALL_BLOCK + (k & 3) * 32;
+                    const uint32_t b = smem_addr(B) + (p == 1 ? b_lo : 0) +
+                                       (b_mn ? k * 2048 : (k >> 2) * SMALL_BLOCK + (k & 3) * 32);
+                    mma_f16<1>(tmem + (p ? small : main), gemm_desc(a, 0), gemm_desc(b, b_mn, SMALL_BLOCK), idesc,
+                               k > 0 || p == 2);
+                }
+            mma_commit<1>(bar);
+        }
+        ok = mbar_wait(bar, phase);
+        phase ^= 1;
+        mma_fence_after();
+    };
+    for (int k = 0; k < q.steps; k++) {
+        float v[32], g[32];
+        product(0, GS, X, C::X, X, C::X, false, ns, (l + 15) / 16);
+        if (from < ns) {
+            small_sum(lanes + from, lanes + GS + from, v);
+#pragma unroll
+            for (int e = 0; e < 32; e++) v[e] *= 1.0f / SCALE;
+            small_store(G, C::G, row, from, v);
+        }
+        product(P, PS, G, C::G, G, C::G, false, ns, ns / 16);
+        if (from < ns) {
+            small_sum(lanes + from, lanes + GS + from, g);
+            small_sum(lanes + P + from, lanes + PS + from, v);
+#pragma unroll
+            for (int e = 0; e < 32; e++) v[e] = fmaf(NS_B / SCALE, g[e], NS_C / SCALE * v[e]);
+            small_store(G, C::G, row, from, v);
+        }
+        product(0, XS, G, C::G, X, C::X, true, nl, ns / 16);
+        for (int c = from; c < nl; c += 128) {
+            small_sum(lanes + c, lanes + XS + c, v);
+            small_load(X, C::X, row, c, g);
+#pragma unroll
+            for (int e = 0; e < 32; e++) v[e] = fmaf(NS_A, g[e], v[e] * (1.0f / SCALE));
+            if (k + 1 < q.steps)
+                small_store(X, C::X, row, c, v);
+            else if (ok && row < s && c < l)
+                LastEpi{q}.finish(z, tall ? c : row, tall ? row : c, tall, l - c < 32 ? l - c : 32, v);
+        }
+    }
+    mma_fence_before();
+    __syncthreads();
+    mma_fence_after();
+    if (warp == 0) tmem_free<1>(tmem, 512);
+    if (!ok && tid == 0) atomicAdd(fault, 1u);
+}
 
 // ── host side ─────────────────────────────────────────────────────────────
 
@@ -301,6 +481,21 @@ Ws layout(long long batch, long long rows, long long cols) {
     return w;
 }
 
+bool is_small(long long rows, long long cols) {
+    const long long s = rows < cols ? rows : cols, l = rows < cols ? cols : rows;
+    return s <= 128 && l <= 256;
+}
+
+template <int LB, int V>
+cudaError_t run_small(const Problem& q, unsigned int* fault, cudaStream_t st) {
+    auto kernel = small_kernel<LB, V>;
+    static GemmOnce once;
+    const cudaError_t e = once.smem(kernel, Small<LB>::BYTES);
+    if (e != cudaSuccess) return e;
+    kernel<<<q.batch, SMALL_THREADS, Small<LB>::BYTES, st>>>(q, fault);
+    return cudaGetLastError();
+}
+
 // D = A B^T on pairs; the epilogue reads `in` and writes `out` (either may be
 // absent), pairs of D's shape.
 template <class Epi>
@@ -326,6 +521,15 @@ cudaError_t multiply(const Pair& a, bool a_mn, const Pair& b, bool b_mn, long lo
 cudaError_t solve(const Problem& q, char* ws, cudaStream_t st) {
     unsigned int* fault = fault_word();
     if (!fault) return cudaErrorInvalidSymbol;
+    auto wide = [&](const View& v, int e) {
+        return !v.p || ((uintptr_t)v.p % (4 * e) == 0 && v.cs == 1 && v.rs % 4 == 0 && (q.batch == 1 || v.zs % 4 == 0));
+    };
+    const bool by4 = q.cols % 4 == 0 && wide(q.g, q.dtype == PHYZB_DT_F32 ? 4 : 2) && wide(q.m, 4);
+    if (is_small(q.rows, q.cols)) {
+        const bool narrow = q.rows <= 128 && q.cols <= 128;
+        if (by4) return narrow ? run_small<128, 4>(q, fault, st) : run_small<256, 4>(q, fault, st);
+        return narrow ? run_small<128, 1>(q, fault, st) : run_small<256, 1>(q, fault, st);
+    }
     Ws o = layout(q.batch, q.rows, q.cols);
     o.x.p = (__half*)(ws + o.x_at);
     o.y.p = (__half*)(ws + o.y_at);
@@ -334,10 +538,6 @@ cudaError_t solve(const Problem& q, char* ws, cudaStream_t st) {
     float* part = (float*)(ws + o.part_at);
     const bool tall = q.rows > q.cols;
     const int s = tall ? q.cols : q.rows, l = tall ? q.rows : q.cols;
-    auto wide = [&](const View& v, int e) {
-        return !v.p || ((uintptr_t)v.p % (4 * e) == 0 && v.cs == 1 && v.rs % 4 == 0 && v.zs % 4 == 0);
-    };
-    const bool by4 = q.cols % 4 == 0 && wide(q.g, q.dtype == PHYZB_DT_F32 ? 4 : 2) && wide(q.m, 4);
     // blocks of a few stretches, at most NORM_BLOCKS
     const long long stretches = q.rows * ((q.cols + (by4 ? 1023 : 255)) / (by4 ? 1024 : 256));
     const dim3 grid((unsigned)(stretches < NORM_BLOCKS ? stretches : NORM_BLOCKS), (unsigned)q.batch);
@@ -373,7 +573,9 @@ View view(const void* p, const int64_t* st) { return {(void*)p, st[0], st[1], st
 
 }  // namespace
 
-long long muon_workspace(const phyzb_muon_args& a) { return layout(a.batch, a.rows, a.cols).total; }
+long long muon_workspace(const phyzb_muon_args& a) {
+    return is_small(a.rows, a.cols) ? 0 : layout(a.batch, a.rows, a.cols).total;
+}
 
 cudaError_t muon_update(const phyzb_muon_args& a, void* ws, cudaStream_t s) {
     Problem q{};
@@ -394,7 +596,9 @@ cudaError_t muon_update(const phyzb_muon_args& a, void* ws, cudaStream_t s) {
     return solve(q, (char*)ws, s);
 }
 
-long long orthogonalize_workspace(const phyzb_orthogonalize_args& a) { return layout(a.batch, a.rows, a.cols).total; }
+long long orthogonalize_workspace(const phyzb_orthogonalize_args& a) {
+    return is_small(a.rows, a.cols) ? 0 : layout(a.batch, a.rows, a.cols).total;
+}
 
 cudaError_t orthogonalize(const phyzb_orthogonalize_args& a, void* ws, cudaStream_t s) {
     Problem q{};

@@ -45,19 +45,22 @@ def _dtype(t: torch.Tensor, name: str) -> int:
     return d
 
 
-def _arr(t, name: str, shape: tuple, dtype, device, none=None) -> tuple:
+def _arr(t, name: str, shape, dtype, dev: int, none=None) -> tuple:
     """(address, strides) of a tensor that must have this shape, type and device."""
     if t is None:
         _need(none is not None, f"{name} is missing")
         return none
-    if t.shape != shape or t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}: {tuple(shape)} {dtype} on {device} is wanted")
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != dev:
+        raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}: {tuple(shape)} {dtype} on cuda:{dev} "
+                         "is wanted")
     return t.data_ptr(), t.stride()
 
 
 def _device(t: torch.Tensor, name: str) -> int:
-    _need(t.is_cuda, f"{name} is on {t.device}: a CUDA device is wanted")
-    return t.device.index
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"{name} is on {t.device}: a CUDA device is wanted")
+    return dev
 
 
 def _activation(name: str) -> int:
@@ -66,13 +69,34 @@ def _activation(name: str) -> int:
     return a
 
 
-def _call(op: str, query: str, args: bytes, device: torch.device) -> None:
-    lib = _lib.load()
-    need = C.c_int64(0)
-    _lib.check(getattr(lib, query)(args, C.byref(need)))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    _lib.check(getattr(lib, op)(args, ws.data_ptr() if ws is not None else None, need.value, stream))
+class _Op:
+    """One operator of the library: asks for its workspace, then runs on the current stream of a device."""
+
+    def __init__(self, run: str, query: str):
+        self._names, self._fns = (run, query), None
+
+    def __call__(self, args: bytes, dev: int) -> None:
+        if self._fns is None:
+            lib = _lib.load()
+            self._fns = tuple(getattr(lib, n) for n in self._names)
+        run, query = self._fns
+        need = C.c_int64()
+        code = query(args, C.byref(need))
+        if code:
+            _lib.check(code)
+        n = need.value
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        code = run(args, ws.data_ptr() if n else None, n, torch._C._cuda_getCurrentRawStream(dev))
+        if code:
+            _lib.check(code)
+
+
+_linear = _Op("phyzb_linear", "phyzb_linear_workspace")
+_linear_grad = _Op("phyzb_linear_grad", "phyzb_linear_grad_workspace")
+_scan = _Op("phyzb_gated_scan", "phyzb_gated_scan_workspace")
+_scan_grad = _Op("phyzb_gated_scan_grad", "phyzb_gated_scan_grad_workspace")
+_muon = _Op("phyzb_muon_update", "phyzb_muon_workspace")
+_orth = _Op("phyzb_orthogonalize", "phyzb_orthogonalize_workspace")
 
 
 def _like(x: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
@@ -92,17 +116,17 @@ def linear(x, weight, bias=None, *, activation: str = "none", residual=None, sav
     dt, dev, act = _dtype(x, "x"), _device(x, "x"), _activation(activation)
     y = _like(x, m, n) if out is None else out
     pre = _like(x, m, n) if save_pre else None
-    d, t = x.device, x.dtype
-    pw, sw = _arr(weight, "weight", (n, k), t, d)
-    py, sy = _arr(y, "out", (m, n), t, d)
-    pr, sr = _arr(residual, "residual", (m, n), t, d, _NO2)
-    pp, sp = _arr(pre, "pre", (m, n), t, d, _NO2)
+    t = x.dtype
+    pw, sw = _arr(weight, "weight", (n, k), t, dev)
+    py, sy = (y.data_ptr(), y.stride()) if out is None else _arr(out, "out", (m, n), t, dev)
+    pr, sr = _arr(residual, "residual", (m, n), t, dev, _NO2)
+    pp, sp = (pre.data_ptr(), pre.stride()) if save_pre else _NO2
     pb = 0
     if bias is not None:
-        pb, sb = _arr(bias, "bias", (n,), torch.float32, d)
+        pb, sb = _arr(bias, "bias", (n,), torch.float32, dev)
         _need(sb[0] == 1 or n == 1, "bias must be contiguous")
     args = _LINEAR.pack(dt, act, dev, m, k, n, x.data_ptr(), *x.stride(), pw, *sw, pb, pr, *sr, py, *sy, pp, *sp)
-    _call("phyzb_linear", "phyzb_linear_workspace", args, d)
+    _linear(args, dev)
     return (y, pre) if save_pre else y
 
 
@@ -115,29 +139,30 @@ def linear_backward(dy, x, weight, pre=None, *, activation: str = "none", bias: 
     m, k = x.shape
     n = weight.shape[0]
     dt, dev, act = _dtype(x, "x"), _device(x, "x"), _activation(activation)
-    d, t = x.device, x.dtype
-    pw, sw = _arr(weight, "weight", (n, k), t, d)
-    pd, sd = _arr(dy, "dy", (m, n), t, d)
-    pp, sp = _arr(pre, "pre", (m, n), t, d, _NO2 if act == 0 else None)
+    t = x.dtype
+    pw, sw = _arr(weight, "weight", (n, k), t, dev)
+    pd, sd = _arr(dy, "dy", (m, n), t, dev)
+    pp, sp = _arr(pre, "pre", (m, n), t, dev, _NO2 if act == 0 else None)
     dx = _like(x, m, k) if need_dx else None
-    dw = torch.empty((n, k), dtype=t, device=d) if need_dw else None
-    db = torch.empty(n, dtype=torch.float32, device=d) if bias else None
+    dw = torch.empty((n, k), dtype=t, device=x.device) if need_dw else None
+    db = torch.empty(n, dtype=torch.float32, device=x.device) if bias else None
     px, sx = (dx.data_ptr(), dx.stride()) if need_dx else _NO2
     pg, sg = (dw.data_ptr(), dw.stride()) if need_dw else _NO2
     args = _LINEAR_GRAD.pack(dt, act, dev, m, k, n, pd, *sd, pp, *sp, x.data_ptr(), *x.stride(), pw, *sw, px, *sx,
                              pg, *sg, db.data_ptr() if bias else 0)
-    _call("phyzb_linear_grad", "phyzb_linear_grad_workspace", args, d)
+    _linear_grad(args, dev)
     return dx, dw, db
 
 
-def _reset(reset, shape, device) -> tuple:
+def _reset(reset, shape, dev: int) -> tuple:
     if reset is None:
         return _NO3
-    if reset.dtype == torch.bool:
-        reset = reset.view(torch.uint8)
+    if reset.dtype is not torch.uint8 and reset.dtype is not torch.bool or reset.get_device() != dev:
+        raise ValueError(f"reset is {reset.dtype} on {reset.device}: uint8 or bool on cuda:{dev} is wanted")
+    if reset.shape == shape:
+        return reset.data_ptr(), reset.stride()
     if reset.dim() == 2:
         reset = reset.unsqueeze(2)
-    _need(reset.dtype == torch.uint8 and reset.device == device, f"reset must be uint8 or bool on {device}")
     return reset.data_ptr(), reset.expand(shape).stride()
 
 
@@ -147,16 +172,16 @@ def gated_scan(x, gate, h0=None, reset=None, *, out=None):
     dropped. Returns (h in x's type and order, the last state [b, c] in float32)."""
     _need(x.dim() == 3, "x must be [b, t, c]")
     b, t, c = shape = x.shape
-    dt, dev, d = _dtype(x, "x"), _device(x, "x"), x.device
+    dt, dev = _dtype(x, "x"), _device(x, "x")
     h = torch.empty_like(x) if out is None else out
-    last = torch.empty((b, c), dtype=torch.float32, device=d)
-    pg, sg = _arr(gate, "gate", shape, x.dtype, d)
-    p0, s0 = _arr(h0, "h0", (b, c), torch.float32, d, _NO2)
-    pr, sr = _reset(reset, shape, d)
-    ph, sh = _arr(h, "out", shape, x.dtype, d)
+    last = torch.empty((b, c), dtype=torch.float32, device=x.device)
+    pg, sg = _arr(gate, "gate", shape, x.dtype, dev)
+    p0, s0 = _arr(h0, "h0", (b, c), torch.float32, dev, _NO2)
+    pr, sr = _reset(reset, shape, dev)
+    ph, sh = (h.data_ptr(), h.stride()) if out is None else _arr(out, "out", shape, x.dtype, dev)
     args = _SCAN.pack(dt, dev, b, t, c, x.data_ptr(), *x.stride(), pg, *sg, p0, *s0, pr, *sr, ph, *sh,
                       last.data_ptr())
-    _call("phyzb_gated_scan", "phyzb_gated_scan_workspace", args, d)
+    _scan(args, dev)
     return h, last
 
 
@@ -165,18 +190,18 @@ def gated_scan_backward(dh, x, gate, h, h0=None, reset=None, dh_last=None):
     inputs and its h."""
     _need(x.dim() == 3, "x must be [b, t, c]")
     b, t, c = shape = x.shape
-    dt, dev, d = _dtype(x, "x"), _device(x, "x"), x.device
+    dt, dev = _dtype(x, "x"), _device(x, "x")
+    pd, sd = _arr(dh, "dh", shape, x.dtype, dev)
+    pg, sg = _arr(gate, "gate", shape, x.dtype, dev)
+    ph, sh = _arr(h, "h", shape, x.dtype, dev)
+    p0, s0 = _arr(h0, "h0", (b, c), torch.float32, dev, _NO2)
+    pr, sr = _reset(reset, shape, dev)
+    pl, sl = _arr(dh_last, "dh_last", (b, c), torch.float32, dev, _NO2)
     dx, dg = torch.empty_like(x), torch.empty_like(gate)
-    dh0 = torch.empty((b, c), dtype=torch.float32, device=d)
-    pd, sd = _arr(dh, "dh", shape, x.dtype, d)
-    pg, sg = _arr(gate, "gate", shape, x.dtype, d)
-    ph, sh = _arr(h, "h", shape, x.dtype, d)
-    p0, s0 = _arr(h0, "h0", (b, c), torch.float32, d, _NO2)
-    pr, sr = _reset(reset, shape, d)
-    pl, sl = _arr(dh_last, "dh_last", (b, c), torch.float32, d, _NO2)
+    dh0 = torch.empty((b, c), dtype=torch.float32, device=x.device)
     args = _SCAN_GRAD.pack(dt, dev, b, t, c, pd, *sd, x.data_ptr(), *x.stride(), pg, *sg, ph, *sh, p0, *s0, pr, *sr,
                            pl, *sl, dx.data_ptr(), *dx.stride(), dg.data_ptr(), *dg.stride(), dh0.data_ptr())
-    _call("phyzb_gated_scan_grad", "phyzb_gated_scan_grad_workspace", args, d)
+    _scan_grad(args, dev)
     return dx, dg, dh0
 
 
@@ -195,22 +220,22 @@ def muon_update(weight, grad, momentum, *, lr: float, mu: float = 0.95, nesterov
     float32, grad any type, scale sqrt(max(1, rows / cols)) unless given; `copy` (bfloat16 or float16) gets the new
     weights too."""
     w = _matrices(weight, "weight")
-    shape, d = w.shape, w.device
+    shape = w.shape
     g = _matrices(grad, "grad", shape)
     dt, dev = _dtype(g, "grad"), _device(w, "weight")
     b, r, c = shape
-    pw, sw = _arr(w, "weight", shape, torch.float32, d)
-    pg, sg = _arr(g, "grad", shape, g.dtype, d)
-    pm, sm = _arr(_matrices(momentum, "momentum", shape), "momentum", shape, torch.float32, d)
+    pw, sw = _arr(w, "weight", shape, torch.float32, dev)
+    pg, sg = _arr(g, "grad", shape, g.dtype, dev)
+    pm, sm = _arr(_matrices(momentum, "momentum", shape), "momentum", shape, torch.float32, dev)
     pc, sc, cdt = 0, (0, 0, 0), 0
     if copy is not None:
         _need(copy.dtype in (torch.bfloat16, torch.float16), f"copy is {copy.dtype}: bfloat16 or float16 is wanted")
-        pc, sc = _arr(_matrices(copy, "copy", shape), "copy", shape, copy.dtype, d)
+        pc, sc = _arr(_matrices(copy, "copy", shape), "copy", shape, copy.dtype, dev)
         cdt = _DT[copy.dtype]
     scale = math.sqrt(max(1.0, r / c)) if scale is None else scale
     args = _MUON.pack(dt, dev, int(bool(nesterov)), steps, b, r, c, pg, *sg, pm, *sm, pw, *sw, cdt, 0, pc, *sc,
                       lr, mu, weight_decay, scale)
-    _call("phyzb_muon_update", "phyzb_muon_workspace", args, d)
+    _muon(args, dev)
 
 
 def orthogonalize(x, *, steps: int = 5):
@@ -220,5 +245,5 @@ def orthogonalize(x, *, steps: int = 5):
     dt, dev = _dtype(v, "x"), _device(v, "x")
     out = torch.empty_like(v, memory_format=torch.contiguous_format)
     args = _ORTH.pack(dt, dev, steps, 0, *v.shape, v.data_ptr(), *v.stride(), out.data_ptr(), *out.stride())
-    _call("phyzb_orthogonalize", "phyzb_orthogonalize_workspace", args, v.device)
+    _orth(args, dev)
     return out if x.dim() == 3 else out[0]

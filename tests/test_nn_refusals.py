@@ -88,12 +88,13 @@ def test_null_arguments_and_small_workspaces():
     for op in _lib.NN_OPS:
         assert getattr(lib, f"phyzb_{op}")(None, None, 0, None) == _lib.ERR_INVALID
     need = C.c_int64(-1)
-    assert lib.phyzb_muon_workspace(muon_args(), None) == _lib.ERR_INVALID
-    assert lib.phyzb_muon_workspace(muon_args(), C.byref(need)) == 0 and need.value > 0
-    assert lib.phyzb_muon_update(muon_args(), C.c_void_p(256), need.value - 1, None) == _lib.ERR_INVALID
+    big = muon_args(r=300, c=400, s=(120000, 400, 1))  # (small matrices need no workspace)
+    assert lib.phyzb_muon_workspace(big, None) == _lib.ERR_INVALID
+    assert lib.phyzb_muon_workspace(big, C.byref(need)) == 0 and need.value > 0
+    assert lib.phyzb_muon_update(big, C.c_void_p(256), need.value - 1, None) == _lib.ERR_INVALID
     assert "smaller" in lib.phyzb_last_error().decode()
-    assert lib.phyzb_muon_update(muon_args(), None, need.value, None) == _lib.ERR_INVALID
-    assert lib.phyzb_muon_update(muon_args(), C.c_void_p(16), need.value, None) == _lib.ERR_INVALID
+    assert lib.phyzb_muon_update(big, None, need.value, None) == _lib.ERR_INVALID
+    assert lib.phyzb_muon_update(big, C.c_void_p(16), need.value, None) == _lib.ERR_INVALID
     assert "256" in lib.phyzb_last_error().decode()
 
 
