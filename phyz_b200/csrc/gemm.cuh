@@ -272,6 +272,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
     volatile uint32_t* const gave_up = slot + 1;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rank = CTAS == 2 ? blockIdx.x % 2 : 0;  // in the cluster; the first one leads
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (int k = 0; k < S::STAGES; k++) {
             mbar_init(&full[k], 1);
@@ -296,6 +297,9 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
     block_sync<CTAS>();
     mma_fence_after();
     const uint32_t tmem = *slot;
+    // launched ahead of the end of the kernel before it (gemm_launch_as): what that
+    // one wrote is there from here on
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
     if (warp == 0) {
@@ -656,8 +660,18 @@ cudaError_t gemm_launch_as(const GemmMat* a, const GemmMat* b, long long ma, lon
     const cudaError_t e = once.smem(kernel, S::BYTES);
     if (e != cudaSuccess) return e;
     const int slots = GEMM_SMS / CTAS;
-    kernel<<<(g.units < slots ? g.units : slots) * CTAS, S::THREADS, S::BYTES, st>>>(g, epi, fault);
-    return cudaGetLastError();
+    // The next product's launch, barriers and Tensor Memory overlap this one's end.
+    cudaLaunchAttribute ahead{};
+    ahead.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    ahead.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3((unsigned)((g.units < slots ? g.units : slots) * CTAS));
+    c.blockDim = dim3(S::THREADS);
+    c.dynamicSmemBytes = S::BYTES;
+    c.stream = st;
+    c.attrs = &ahead;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, g, epi, fault);
 }
 
 template <int PL, class Epi>
