@@ -101,18 +101,28 @@ struct LinearEpi : Slotted<T> {
         if (res.p) v += to_f32(res.p[i * res.is + j * res.js]);
         y.p[i * y.is + j * y.js] = from_f32<T>(v);
     }
-    __device__ __forceinline__ void four(int, long long i, long long j, const float* sum, int n, bool along_i) const {
+    // f once with the activation as a constant
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        with_act(act, f);
+    }
+    template <class K>
+    __device__ __forceinline__ void four(K, int, long long i, long long j, const float* sum, int n, bool along_i) const {
         if constexpr (sizeof(T) == 4) {
             float z[4], r[4] = {};
+            if (bias) {
+                const bool runs = (by_i != 0) == along_i;  // along with the four values
+                const float* p = bias + (by_i ? i : j);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                z[e] = sum[e];
-                if (bias && e < n) z[e] += bias[(by_i != 0) == along_i ? (along_i ? i : j) + e : by_i ? i : j];
+                for (int e = 0; e < 4; e++) z[e] = sum[e] + (e < n ? p[runs ? e : 0] : 0.0f);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) z[e] = sum[e];
             }
             if (pre.p) store4(pre.p + i * pre.is + j * pre.js, along_i ? pre.is : pre.js, n, z);
             if (res.p) load4(res.p + i * res.is + j * res.js, along_i ? res.is : res.js, n, r);
 #pragma unroll
-            for (int e = 0; e < 4; e++) z[e] = act_f32(z[e], act) + r[e];
+            for (int e = 0; e < 4; e++) z[e] = act_f32(z[e], K::value) + r[e];
             store4(y.p + i * y.is + j * y.js, along_i ? y.is : y.js, n, z);
         }
     }
@@ -161,7 +171,11 @@ struct StoreEpi : Slotted<T> {
     __device__ __forceinline__ void one(long long i, long long j, float v) const {
         out.p[i * out.is + j * out.js] = from_f32<T>(v);
     }
-    __device__ __forceinline__ void four(int, long long i, long long j, const float* v, int n, bool along_i) const {
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        f(0);
+    }
+    __device__ __forceinline__ void four(int, int, long long i, long long j, const float* v, int n, bool along_i) const {
         if constexpr (sizeof(T) == 4) store4(out.p + i * out.is + j * out.js, along_i ? out.is : out.js, n, v);
     }
     __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, const float* v,
@@ -208,7 +222,11 @@ GemmIo io_of(const StoreEpi<T>& e, long long rows, long long cols) {
 struct PartEpi : Slotted<float> {
     float* part;
     long long m, n;
-    __device__ __forceinline__ void four(int split, long long i, long long j, const float* v, int k, bool along_i) const {
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        f(0);
+    }
+    __device__ __forceinline__ void four(int, int split, long long i, long long j, const float* v, int k, bool along_i) const {
         store4(part + (split * m + i) * n + j, along_i ? n : 1, k, v);
     }
     __device__ __forceinline__ void operator()(const GemmUnit& q, long long i, int j0, int cols, const float* v,

@@ -17,7 +17,8 @@ struct SimtOperand {
 // stage is loaded into registers while the current one is multiplied. blockIdx
 // = (tiles of i, tiles of j, split of the k range). ALONG_I: D is contiguous in
 // i; lanes then run along i, and the epilogue gets four values along it.
-// Epi: void four(int split, long long i, long long j, const float* v, int n, bool along_i)
+// Epi: each(f) calls f(kind) once, and f void four(kind, int split, long long i, long long j, const float* v, int n,
+// bool along_i)
 template <bool ALONG_I, class Epi>
 __global__ void __launch_bounds__(256) simt_gemm_kernel(SimtOperand A, SimtOperand B, long long M, long long N,
                                                         long long K, long long per, Epi epi) {
@@ -27,34 +28,42 @@ __global__ void __launch_bounds__(256) simt_gemm_kernel(SimtOperand A, SimtOpera
     const long long i0 = (long long)blockIdx.x * TM, j0 = (long long)blockIdx.y * TN;
     const long long k0 = blockIdx.z * per, k1 = k0 + per < K ? k0 + per : K;
     const int t = threadIdx.x, tj = ALONG_I ? t / 16 : t % 16, ti = ALONG_I ? t % 16 : t / 16;
-    // consecutive threads walk the operand's unit stride
+    // consecutive threads walk the operand's unit stride: a thread's elements of a
+    // stage are one column (or row) apart by a fixed step
     const bool ak = A.ks == 1, bk = B.ks == 1;
     float acc[8][4] = {};
     float ra[8], rb[4];
+    const int ai = ak ? t / TK : t % TM, akk = ak ? t % TK : t / TM;
+    const int bj = bk ? t / TK : t % TN, bkk = bk ? t % TK : t / TN;
+    const float* pa = A.p + (i0 + ai) * A.is + (k0 + akk) * A.ks;
+    const float* pb = B.p + (j0 + bj) * B.is + (k0 + bkk) * B.ks;
+    const long long sa = ak ? 16 * A.is : 2 * A.ks, sb = bk ? 16 * B.is : 4 * B.ks;
+    const int mleft = M - i0 < TM ? (int)(M - i0) : TM, nleft = N - j0 < TN ? (int)(N - j0) : TN;
     auto load = [&](long long k) {
+        const int kleft = k1 - k < TK ? (int)(k1 - k) : TK;
+        const float* p = pa;
 #pragma unroll
         for (int u = 0; u < 8; u++) {
-            const int e = t + u * 256, ii = ak ? e / TK : e % TM, kk = ak ? e % TK : e / TM;
-            ra[u] = i0 + ii < M && k + kk < k1 ? A.p[(i0 + ii) * A.is + (k + kk) * A.ks] : 0.0f;
+            const bool on = ak ? akk < kleft && ai + 16 * u < mleft : ai < mleft && akk + 2 * u < kleft;
+            ra[u] = on ? *p : 0.0f;
+            p += sa;
         }
+        p = pb;
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const int e = t + u * 256, jj = bk ? e / TK : e % TN, kk = bk ? e % TK : e / TN;
-            rb[u] = j0 + jj < N && k + kk < k1 ? B.p[(j0 + jj) * B.is + (k + kk) * B.ks] : 0.0f;
+            const bool on = bk ? bkk < kleft && bj + 16 * u < nleft : bj < nleft && bkk + 4 * u < kleft;
+            rb[u] = on ? *p : 0.0f;
+            p += sb;
         }
+        pa += TK * A.ks;
+        pb += TK * B.ks;
     };
     if (k0 < k1) load(k0);
     for (long long k = k0; k < k1; k += TK) {
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
-            const int e = t + u * 256;
-            As[ak ? e % TK : e / TM][ak ? e / TK : e % TM] = ra[u];
-        }
+        for (int u = 0; u < 8; u++) As[ak ? akk : akk + 2 * u][ak ? ai + 16 * u : ai] = ra[u];
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int e = t + u * 256;
-            Bs[bk ? e % TK : e / TN][bk ? e / TK : e % TN] = rb[u];
-        }
+        for (int u = 0; u < 4; u++) Bs[bk ? bkk : bkk + 4 * u][bk ? bj + 16 * u : bj] = rb[u];
         __syncthreads();
         if (k + TK < k1) load(k + TK);
 #pragma unroll
@@ -70,25 +79,28 @@ __global__ void __launch_bounds__(256) simt_gemm_kernel(SimtOperand A, SimtOpera
         }
         __syncthreads();
     }
-    auto left = [](long long n) { return n < 4 ? (int)n : 4; };
-    const long long jj = j0 + tj * 4;
-    if (ALONG_I) {
+    auto left = [](int n) { return n < 4 ? n : 4; };
+    const int jj = tj * 4;
+    epi.each([&](auto kind) {
+        if (ALONG_I) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const long long ii = i0 + h * 64 + ti * 4;
+            for (int h = 0; h < 2; h++) {
+                const int ii = h * 64 + ti * 4;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float v[4] = {acc[h * 4][j], acc[h * 4 + 1][j], acc[h * 4 + 2][j], acc[h * 4 + 3][j]};
-                if (ii < M && jj + j < N) epi.four(blockIdx.z, ii, jj + j, v, left(M - ii), true);
+                for (int j = 0; j < 4; j++) {
+                    const float v[4] = {acc[h * 4][j], acc[h * 4 + 1][j], acc[h * 4 + 2][j], acc[h * 4 + 3][j]};
+                    if (ii < mleft && jj + j < nleft)
+                        epi.four(kind, blockIdx.z, i0 + ii, j0 + jj + j, v, left(mleft - ii), true);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int ii = (i / 4) * 64 + ti * 4 + i % 4;
+                if (ii < mleft && jj < nleft) epi.four(kind, blockIdx.z, i0 + ii, j0 + jj, acc[i], left(nleft - jj), false);
             }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const long long ii = i0 + (i / 4) * 64 + ti * 4 + i % 4;
-            if (ii < M && jj < N) epi.four(blockIdx.z, ii, jj, acc[i], left(N - jj), false);
-        }
-    }
+    });
 }
 
 template <class Epi>
