@@ -270,6 +270,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* src, long long os, l
                                                    long long inner, long long pitch, uint16_t* dst, long long plane) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= inner) return;
+#pragma unroll 4
     for (long long o = blockIdx.y; o < outer; o += gridDim.y) {
         const T v = src[o * os + i * is];
         if constexpr (sizeof(T) == 2) {
@@ -308,7 +309,8 @@ struct Operand {
         }
         const bool mn = gemm_mn(mat, k);
         const long long outer = mn ? k : rows, inner = mn ? rows : k, os = mn ? mat.ks : mat.rs, is = mn ? 1 : mat.ks;
-        const dim3 grid((unsigned)((inner + 255) / 256), (unsigned)(outer < 65535 ? outer : 65535));
+        const long long across = (inner + 255) / 256, down = 8 * GEMM_SMS / across + 1;  // eight blocks to an SM
+        const dim3 grid((unsigned)across, (unsigned)(outer < down ? outer : down));
         if (dtype == PHYZB_DT_F32)
             pack_kernel<<<grid, 256, 0, st>>>((const float*)mat.p, os, is, outer, inner, pitch, (uint16_t*)ws, plane);
         else
@@ -563,7 +565,7 @@ __device__ __forceinline__ void dz_store(const DzArgs& a, long long o, long long
 // inner = features. V neighbours per thread, 256 threads = 32 along the features
 // x 8 rows.
 template <class T, int V>
-__global__ void __launch_bounds__(256) dz_rows_kernel(const __grid_constant__ DzArgs a) {
+__global__ void __launch_bounds__(256, 4) dz_rows_kernel(const __grid_constant__ DzArgs a) {
     __shared__ float sums[8][32 * V];
     const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
     const long long i0 = ((long long)blockIdx.x * 32 + tx) * V;
@@ -572,7 +574,7 @@ __global__ void __launch_bounds__(256) dz_rows_kernel(const __grid_constant__ Dz
     with_act(a.act, [&](auto kind) {
         if (i0 >= a.inner) return;
         constexpr int ACT = decltype(kind)::value;
-#pragma unroll 4
+#pragma unroll 2
         for (long long o = o0 + ty; o < o1; o += 8) {
             T d[V], z[V], out[V];
             const T *pd = (const T*)a.dy + o * a.dy_o + i0 * a.dy_i, *pz = (const T*)a.pre + o * a.pre_o + i0 * a.pre_i;
