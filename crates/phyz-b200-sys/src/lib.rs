@@ -555,6 +555,7 @@ extern "C" {
     pub fn phyzb_orthogonalize_workspace(a: *const phyzb_orthogonalize_args, bytes: *mut i64) -> c_int;
     pub fn phyzb_orthogonalize(a: *const phyzb_orthogonalize_args, workspace: *mut c_void,
                                workspace_bytes: i64, stream: *mut c_void) -> c_int;
+    pub fn phyzb_nn_status(device: i32) -> c_int;
 
     // measurement and kernel selection
     pub fn phyzb_flops_per_world_step(sim: *const phyzb_sim, flops: *mut f64, transcendentals: *mut f64) -> c_int;

@@ -654,8 +654,9 @@ int phyzb_get_world_lanes(phyzb_sim* sim, int32_t* lanes, int32_t* active);
  * with its epilogue, a gated recurrence over the control steps of a rollout,
  * and the Muon update of the layers' matrices. They work on caller-owned
  * device memory, allocate nothing, keep nothing between calls and run on
- * `stream` (a cudaStream_t, NULL = the default stream) of the current context
- * of `device`, asynchronously. Strides count elements and may take any order;
+ * `stream` (a cudaStream_t, NULL = the default stream) of `device`,
+ * asynchronously; the first call of each kind on a device sets its kernels up
+ * and belongs before any stream capture. Strides count elements and may take any order;
  * outputs must not overlap each other or the inputs, except where said.
  * `workspace` is device memory of at least the bytes that the matching
  * phyzb_*_workspace reports for the same arguments (256-byte aligned; NULL when it reports
@@ -677,8 +678,8 @@ int phyzb_get_world_lanes(phyzb_sim* sim, int32_t* lanes, int32_t* active);
  * `pre` is given, pre = x w^T + bias [m][n] for the backward pass. Every array
  * but bias is of `dtype`; sums are f32 and rounded once. f32 operands are
  * multiplied at f32 accuracy: on the FMA units where the layer is small, else
- * as three bf16 terms each, six products (an infinity there gives NaN). m may
- * be 0. */
+ * as three bf16 terms each, six products (an infinity may then give NaN where
+ * f32 arithmetic keeps it). m may be 0. */
 typedef struct {
     int32_t dtype, activation, device;
     int64_t m, k, n;
@@ -821,6 +822,12 @@ typedef struct {
 } phyzb_orthogonalize_args;
 int phyzb_orthogonalize_workspace(const phyzb_orthogonalize_args* a, int64_t* bytes);
 int phyzb_orthogonalize(const phyzb_orthogonalize_args* a, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Whether every wait inside the operators' kernels on `device` has ended in
+ * time since the library was loaded (each gives up after some seconds, its
+ * kernel then leaves its outputs unfinished): PHYZB_OK, or PHYZB_ERR_CUDA with
+ * the kernels and their counts in the message. Waits for the device. */
+int phyzb_nn_status(int32_t device);
 
 #ifdef __cplusplus
 }

@@ -253,6 +253,7 @@ SIGNATURES = {
     "phyzb_comm_destroy": (C.c_int, [_P]),
     "phyzb_reduce_objective": (C.c_int, [_P, _P, C.c_int, C.c_double, C.POINTER(C.c_double)]),
     "phyzb_measure_fma_peak": (C.c_int, [C.c_int, _D]),
+    "phyzb_nn_status": (C.c_int, [C.c_int32]),
     # recurrent-block operators: the argument structs are packed by nn.py
     **{f"phyzb_{op}": (C.c_int, [C.c_char_p, _P, C.c_int64, _P]) for op in NN_OPS},
     **{f"phyzb_{op}_workspace": (C.c_int, [C.c_char_p, C.POINTER(C.c_int64)]) for op in NN_WORKSPACES},

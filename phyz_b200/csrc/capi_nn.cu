@@ -291,4 +291,19 @@ int phyzb_orthogonalize(const phyzb_orthogonalize_args* a, void* ws, int64_t ws_
     return call(a, ws, ws_bytes, stream, pz::orthogonalize_workspace, pz::orthogonalize);
 }
 
+int phyzb_nn_status(int32_t device) {
+    return guarded([&] {
+        PZ_TRY(check_device(device));
+        DeviceGuard g(device);
+        unsigned int linear = 0, scan = 0, muon = 0;
+        PZ_CUDA(pz::linear_faults(&linear));
+        PZ_CUDA(pz::scan_faults(&scan));
+        PZ_CUDA(pz::muon_faults(&muon));
+        if (linear + scan + muon)
+            return fail(PHYZB_ERR_CUDA, "waits that ran out: linear " + std::to_string(linear) + ", scan " +
+                                            std::to_string(scan) + ", muon " + std::to_string(muon));
+        return (int)PHYZB_OK;
+    });
+}
+
 }  // extern "C"

@@ -36,4 +36,9 @@ cudaError_t muon_update(const phyzb_muon_args& a, void* ws, cudaStream_t s);
 long long orthogonalize_workspace(const phyzb_orthogonalize_args& a);
 cudaError_t orthogonalize(const phyzb_orthogonalize_args& a, void* ws, cudaStream_t s);
 
+// Waits of each file's kernels on the current device that ran out.
+cudaError_t linear_faults(unsigned int* n);
+cudaError_t scan_faults(unsigned int* n);
+cudaError_t muon_faults(unsigned int* n);
+
 }  // namespace pz

@@ -2,7 +2,8 @@
 //
 // Every wait is bounded. A wait that runs out returns false; the kernel then
 // leaves its loop, waits once more for its own copies (bounded again), gives
-// back what it holds and sets nn_fault, which phyzb_nn_status reports.
+// back what it holds and counts it in its file's fault word, which
+// phyzb_nn_status reports.
 #pragma once
 
 #include <cuda.h>

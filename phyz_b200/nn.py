@@ -185,9 +185,9 @@ def gated_scan(x, gate, h0=None, reset=None, *, out=None):
     return h, last
 
 
-def gated_scan_backward(dh, x, gate, h, h0=None, reset=None, dh_last=None):
+def gated_scan_backward(dh, x, gate, h, h0=None, reset=None, dh_last=None, *, out=None):
     """Gradients (dx, dgate, dh0) of `gated_scan` from dh [b, t, c] and dh_last [b, c] (float32), with the forward's
-    inputs and its h."""
+    inputs and its h. `out`: the tensors (dx, dgate) to write, such as the halves of one projection's gradient."""
     _need(x.dim() == 3, "x must be [b, t, c]")
     b, t, c = shape = x.shape
     dt, dev = _dtype(x, "x"), _device(x, "x")
@@ -197,10 +197,12 @@ def gated_scan_backward(dh, x, gate, h, h0=None, reset=None, dh_last=None):
     p0, s0 = _arr(h0, "h0", (b, c), torch.float32, dev, _NO2)
     pr, sr = _reset(reset, shape, dev)
     pl, sl = _arr(dh_last, "dh_last", (b, c), torch.float32, dev, _NO2)
-    dx, dg = torch.empty_like(x), torch.empty_like(gate)
+    dx, dg = (torch.empty_like(x), torch.empty_like(gate)) if out is None else out
+    px, sx = _arr(dx, "dx", shape, x.dtype, dev)
+    pq, sq = _arr(dg, "dgate", shape, x.dtype, dev)
     dh0 = torch.empty((b, c), dtype=torch.float32, device=x.device)
     args = _SCAN_GRAD.pack(dt, dev, b, t, c, pd, *sd, x.data_ptr(), *x.stride(), pg, *sg, ph, *sh, p0, *s0, pr, *sr,
-                           pl, *sl, dx.data_ptr(), *dx.stride(), dg.data_ptr(), *dg.stride(), dh0.data_ptr())
+                           pl, *sl, px, *sx, pq, *sq, dh0.data_ptr())
     _scan_grad(args, dev)
     return dx, dg, dh0
 
@@ -247,3 +249,9 @@ def orthogonalize(x, *, steps: int = 5):
     args = _ORTH.pack(dt, dev, steps, 0, *v.shape, v.data_ptr(), *v.stride(), out.data_ptr(), *out.stride())
     _orth(args, dev)
     return out if x.dim() == 3 else out[0]
+
+
+def status(device: int = 0) -> None:
+    """Raises PhyzbError if a wait inside an operator's kernel on `device` ever ran out (phyzb_nn_status). Waits for the
+    device."""
+    _lib.check(_lib.load().phyzb_nn_status(int(device)))
