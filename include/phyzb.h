@@ -791,8 +791,8 @@ int phyzb_gated_scan_grad(const phyzb_scan_grad_args* a, void* workspace, int64_
  * grad is of `dtype`, momentum and weight are f32. copy (may be NULL) gets the
  * new weights in `copy_dtype` (bf16 or f16: what phyzb_linear reads). Every
  * array is [batch][rows][cols] with strides. steps = 1..16, sides at most
- * 16384. The products take f16 pairs (high and low part) and sum in f32: as
- * near the f64 result as f32 products are. */
+ * 16384. The products take f16 pairs (high and low part) and sum in f32: X is
+ * within about 1e-5 of its 64-bit value. */
 #define PHYZB_MUON_MAX_SIDE 16384
 typedef struct {
     int32_t dtype, device, nesterov, steps;
@@ -811,7 +811,8 @@ typedef struct {
 int phyzb_muon_workspace(const phyzb_muon_args* a, int64_t* bytes);
 int phyzb_muon_update(const phyzb_muon_args* a, void* workspace, int64_t workspace_bytes, void* stream);
 /* The orthogonalised direction alone: out = X after `steps` iterations from
- * X = x / (|x|_F + 1e-7); x and out of `dtype`. */
+ * X = x / (|x|_F + 1e-7); x and out of `dtype`. As near the 64-bit result as f32
+ * products are. */
 typedef struct {
     int32_t dtype, device, steps, reserved;
     int64_t batch, rows, cols;

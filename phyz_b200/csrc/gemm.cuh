@@ -21,7 +21,9 @@
 // three planes the six products down to 2^-16 of the first. The small ones go
 // to an accumulator of their own: the tensor cores cut each addition off at the
 // accumulator's last bit, and the main sum should not pay for that two to five
-// times more often.
+// times more often. With Epi::FLUSH the accumulators are emptied every so many k
+// blocks into f32 registers of the epilogue's warps, whose additions round: the
+// cut ends, all towards zero, then stay few.
 #pragma once
 
 #include "pz_nn.cuh"
@@ -50,11 +52,13 @@ struct GemmShape {
     static constexpr int FIT = (224 * 1024 - SLOTS) / STAGE;
     static constexpr int STAGES = FIT > 6 ? 6 : FIT;
     static constexpr int ACCS = PL > 1 ? 2 : 1;      // main, small terms
+    static constexpr int FLUSH = PL > 1 ? Epi::FLUSH : 0;
+    static constexpr int CHUNKS = BN / (Epi::WARPS * 8);  // of a warp in a tile
     static constexpr int BUFS = 2 * ACCS * BN <= 512 ? 2 : 1;  // tiles in Tensor Memory
     static constexpr int COLS = BUFS * ACCS * BN;
     static constexpr int BYTES = STAGES * STAGE + SLOTS + 1024 + 512;
     static_assert(BYTES <= 227 * 1024);
-    static_assert(COLS <= 512 && STAGES >= 2 && BR >= 64);
+    static_assert(COLS <= 512 && STAGES >= 2 && BR >= 64 && (!FLUSH || BN <= 128));
 };
 
 // An operand: R rows (i or j) by K, z matrices zs apart.
@@ -253,7 +257,7 @@ __device__ __forceinline__ int slot_at(int row, int col) { return row * 64 + (((
 // Epi: void operator()(const GemmUnit&, long long i, int j0, int cols, float* sum, const unsigned char* in, unsigned
 // char* out) const for 32 columns from j0 (cols of them inside D) of row i, called by whole warps (rows past m too).
 // in, out: the chunk's slot where GemmIo says so (the same one), else null. PLANES of a slot, SLOTS of a warp, 4 to 16 WARPS. MIRROR:
-// where mirrored(unit, j0) says so, the chunk's mirror image is written as well, by turn(sum, slot).
+// where mirrored(unit, j0) says so, the chunk's mirror image is written as well, by turn(sum, slot). FLUSH: k blocks to a sum of the tensor cores, where a product has planes (0: all).
 template <int BN, int PL, int CTAS, class Epi>
 __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL, CTAS, Epi>::THREADS), 1)
     gemm_kernel(const __grid_constant__ GemmArgs g, const __grid_constant__ Epi epi, unsigned int* fault) {
@@ -353,11 +357,26 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
             const int ka = g.a.mn ? 2048 >> 4 : 32 >> 4, kb = g.b.mn ? 2048 >> 4 : 32 >> 4;  // 16 k further
             for (int u = first; u < g.units && ok; u += step) {
                 const GemmUnit q = gemm_unit<BN, S::ROWS>(g, u);
-                ok = gemm_wait(&acc_empty[acc], aphase ^ 1, gave_up);
+                uint32_t d = 0;
+                int begin = q.k0;  // of what the accumulator holds
+                auto next = [&]() {
+                    ok = gemm_wait(&acc_empty[acc], aphase ^ 1, gave_up);
+                    mma_fence_after();
+                    d = tmem + acc * S::ACCS * BN;
+                };
+                auto hand_over = [&]() {
+                    mma_commit<CTAS>(&acc_full[acc]);
+                    if (++acc == S::BUFS) acc = 0, aphase ^= 1;
+                };
+                next();
                 if (!ok) break;
-                mma_fence_after();
-                const uint32_t d = tmem + acc * S::ACCS * BN;
                 for (int k = q.k0; k < q.k1; k++) {
+                    if (S::FLUSH && k - begin == S::FLUSH) {
+                        hand_over();
+                        begin = k;
+                        next();
+                        if (!ok) break;
+                    }
                     ok = gemm_wait(&full[stage], phase, gave_up);
                     if (!ok) break;
                     mma_fence_after();
@@ -370,7 +389,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
                             const uint64_t db = gemm_desc(at + PL * S::A_BYTES + pb * S::B_BYTES, g.b.mn);
                             const bool small = pa + pb > 0;
                             // the first product into an accumulator starts it: (0, 0), and (0, 1) of the small ones
-                            const bool starts = k == q.k0 && (!small || (pa == 0 && pb == 1));
+                            const bool starts = k == begin && (!small || (pa == 0 && pb == 1));
 #pragma unroll
                             for (int s = 0; s < GEMM_BK / 16; s++)
                                 mma_f16<CTAS>(d + (small ? BN : 0), da + s * ka, db + s * kb, g.idesc, !(starts && s == 0));
@@ -378,8 +397,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
                     mma_commit<CTAS>(&empty[stage]);
                     if (++stage == S::STAGES) stage = 0, phase ^= 1;
                 }
-                if (ok) mma_commit<CTAS>(&acc_full[acc]);
-                if (++acc == S::BUFS) acc = 0, aphase ^= 1;
+                if (ok) hand_over();
             }
             if (!ok) {  // not before what was issued has finished
                 mma_commit<CTAS>(done);
@@ -423,13 +441,63 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
         bool ok = true;
         for (int u = first; u < g.units && ok; u += step) {
             const GemmUnit q = gemm_unit<BN, S::ROWS>(g, u);
-            ok = __all_sync(0xffffffffu, gemm_wait(&acc_full[acc], aphase, gave_up));
-            if (!ok) break;
-            mma_fence_after();
-            const uint32_t d = tmem + acc * S::ACCS * BN + ((uint32_t)quarter * 32 << 16);
+            uint32_t d = 0;
+            auto take = [&]() {
+                ok = __all_sync(0xffffffffu, gemm_wait(&acc_full[acc], aphase, gave_up));
+                mma_fence_after();
+                d = tmem + acc * S::ACCS * BN + ((uint32_t)quarter * 32 << 16);
+            };
+            auto give_back = [&]() {
+                mma_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CTAS == 2)
+                        mbar_arrive_at(lead_addr(&acc_empty[acc]));
+                    else
+                        mbar_arrive(&acc_empty[acc]);
+                }
+                if (++acc == S::BUFS) acc = 0, aphase ^= 1;
+            };
+            // 32 columns from c of the accumulator, small terms and all
+            auto sum_of = [&](int c, float* v) {
+                tmem_load(d + c, v);
+                if constexpr (PL > 1) {
+                    float w[32];
+                    tmem_load(d + BN + c, w);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int e = 0; e < 32; e++) v[e] += w[e];
+                } else {
+                    tmem_load_wait();
+                }
+            };
             const long long i = q.row0 + own + lane;
             const bool any = q.k0 < q.k1;
-            for (int c = from; c < BN; c += EVERY) {
+            float held[S::FLUSH ? S::CHUNKS : 1][32];  // FLUSH: the sums so far
+            if constexpr (S::FLUSH > 0) {
+#pragma unroll
+                for (int m = 0; m < S::CHUNKS; m++)
+#pragma unroll
+                    for (int e = 0; e < 32; e++) held[m][e] = 0.0f;
+                for (int k = q.k0; k < q.k1 && ok; k += S::FLUSH) {
+                    take();
+                    if (!ok) break;
+#pragma unroll
+                    for (int m = 0; m < S::CHUNKS; m++) {
+                        float v[32];
+                        sum_of(from + m * EVERY, v);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) held[m][e] += v[e];
+                    }
+                    give_back();
+                }
+            } else {
+                take();
+            }
+            if (!ok) break;
+#pragma unroll
+            for (int m = 0; m < S::CHUNKS; m++) {
+                const int c = from + m * EVERY;
                 const int j = q.j * BN + c, cols = g.n - j < 32 ? g.n - j : 32;
                 if (cols <= 0 || q.row0 + own >= g.m) break;
                 unsigned char* const at = mine + n % MOD * Epi::PLANES * GEMM_PLANE;
@@ -448,19 +516,15 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
                     }
                 }
                 float v[32];
-                tmem_load(d + c, v);
-                if (PL > 1) {
-                    float w[32];
-                    tmem_load(d + BN + c, w);
-                    tmem_load_wait();
+                if constexpr (S::FLUSH > 0) {
 #pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] += w[e];
+                    for (int e = 0; e < 32; e++) v[e] = held[m][e];
                 } else {
-                    tmem_load_wait();
-                }
-                if (!any) {
+                    sum_of(c, v);
+                    if (!any) {
 #pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] = 0.0f;
+                        for (int e = 0; e < 32; e++) v[e] = 0.0f;
+                    }
                 }
                 if constexpr (NS > 0) {
                     if (reads) {
@@ -504,15 +568,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
                 }
                 n++;
             }
-            mma_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (CTAS == 2)
-                    mbar_arrive_at(lead_addr(&acc_empty[acc]));
-                else
-                    mbar_arrive(&acc_empty[acc]);
-            }
-            if (++acc == S::BUFS) acc = 0, aphase ^= 1;
+            if (!S::FLUSH) give_back();
         }
         if constexpr (NS > 0) {
             if (lane == 0) {
@@ -599,7 +655,7 @@ struct GemmCut {
 // is cut too where that fills SMs that the tiles leave empty (parts of 8 k blocks
 // at least; joining them costs about 3000 more).
 inline GemmCut gemm_cut(long long rows, long long cols, long long k, long long batch, int products, bool symmetric,
-                        bool may_split) {
+                        bool may_split, bool flush) {
     const struct {
         int ctas, bn;
         double clocks;  // of a k block
@@ -608,7 +664,7 @@ inline GemmCut gemm_cut(long long rows, long long cols, long long k, long long b
     GemmCut best{};
     double least = 0;
     for (const auto& s : shapes) {
-        if (products > 3 && s.bn == 256) continue;  // (three planes of it do not fit shared memory twice)
+        if (flush && s.bn == 256) continue;  // (its sums do not fit the epilogue's registers)
         const long long r = GEMM_BM * s.ctas, ti = (rows + r - 1) / r, tj = (cols + s.bn - 1) / s.bn;
         const long long tiles = (symmetric ? r / s.bn * ti * (ti + 1) / 2 : ti * tj) * batch;
         const long long slots = GEMM_SMS / s.ctas;
@@ -678,7 +734,7 @@ template <int PL, class Epi>
 cudaError_t gemm_launch(const GemmMat* a, const GemmMat* b, long long ma, long long nb, long long k, int batch,
                         const GemmCut& c, bool symmetric, bool bf16, const GemmIo& io, const Epi& epi,
                         unsigned int* fault, cudaStream_t st) {
-    if constexpr (PL <= 2)
+    if constexpr (PL == 1 || Epi::FLUSH == 0)
         if (c.ctas == 2 && c.bn == 256)
             return gemm_launch_as<256, PL, 2>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, io, epi, fault, st);
     if (c.ctas == 2) return gemm_launch_as<128, PL, 2>(a, b, ma, nb, k, batch, c.splits, symmetric, bf16, io, epi, fault, st);

@@ -81,7 +81,7 @@ __device__ __forceinline__ void store4(float* p, long long stride, int n, const 
 // beside their six products, and go straight.
 template <class T>
 struct Slotted {
-    static constexpr int PLANES = sizeof(T) == 2 ? 1 : 0, SLOTS = sizeof(T) == 2 ? 4 : 0, WARPS = 8;
+    static constexpr int PLANES = sizeof(T) == 2 ? 1 : 0, SLOTS = sizeof(T) == 2 ? 4 : 0, WARPS = 8, FLUSH = 4;
     static constexpr bool MIRROR = false;
 };
 
@@ -325,7 +325,7 @@ struct Operand {
 
 using Cut = GemmCut;
 Cut cut_of(long long rows, long long cols, long long k, bool f32) {
-    return gemm_cut(rows, cols, k, 1, f32 ? 6 : 1, false, true);
+    return gemm_cut(rows, cols, k, 1, f32 ? 6 : 1, false, true, f32);
 }
 
 long long part_bytes(const Cut& c, long long rows, long long cols) {

@@ -12,6 +12,12 @@
 // 11500 (f16 ends at 65504), and what is lost below lo is 2^-25 2^-12 of one.
 // Three products of the tensor cores to a product (gemm.cuh), f32 sums; G and
 // b G + c G G are symmetric and only half their tiles are computed.
+//
+// The tensor cores cut their sums' additions off towards zero, and five
+// iterations make 1.3e-5 of it at 515 x 1030 (f32 products: 2.9e-6). That is far
+// below what an update by lr X shows, so the update takes it. orthogonalize,
+// whose result is X itself, has the sums flushed every 128 of k (FLUSH = 2):
+// 3.3e-6, for 4 % more time.
 #include "gemm.cuh"
 
 namespace pz {
@@ -189,8 +195,9 @@ __device__ __forceinline__ void split(const float* v, __half* h, __half* l) {
 
 // G = sum, or b G + c sum, and its mirror image: D[i][j] = D[j][i]. (The pairs are
 // in the workspace: all of this goes through slots.)
+template <int F>  // k blocks to a sum of the tensor cores (0: all)
 struct SquareEpi {
-    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8;
+    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8, FLUSH = F;
     static constexpr bool MIRROR = true;
     float b, c;  // c / SCALE
     // the tile's mirror image is another one, unless it is inside a diagonal block
@@ -219,8 +226,9 @@ struct SquareEpi {
 };
 
 // a X + sum; i along the rows of X, j along its columns.
+template <int F>
 struct StepEpi {
-    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8;
+    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8, FLUSH = F;
     static constexpr bool MIRROR = false;
     __device__ __forceinline__ void operator()(const GemmUnit&, long long, int, int, const float* sum,
                                                const unsigned char* in, unsigned char* out) const {
@@ -236,8 +244,9 @@ struct StepEpi {
 };
 
 // The last a X + sum, into the weights or the result.
+template <int F>
 struct LastEpi {
-    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8;
+    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8, FLUSH = F;
     static constexpr bool MIRROR = false;
     Problem q;
     template <class T>
@@ -442,7 +451,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) small_kernel(const __grid_co
             if (k + 1 < q.steps)
                 small_store(X, C::X, row, c, v);
             else if (ok && row < s && c < l)
-                LastEpi{q}.finish(z, tall ? c : row, tall ? row : c, tall, l - c < 32 ? l - c : 32, v);
+                LastEpi<0>{q}.finish(z, tall ? c : row, tall ? row : c, tall, l - c < 32 ? l - c : 32, v);
         }
     }
     mma_fence_before();
@@ -514,10 +523,11 @@ cudaError_t multiply(const Pair& a, bool a_mn, const Pair& b, bool b_mn, long lo
     }
     io.reads = in.p != nullptr;
     io.writes = out.p != nullptr;
-    const GemmCut cut = gemm_cut(rows, cols, k, batch, 3, symmetric, false);
+    const GemmCut cut = gemm_cut(rows, cols, k, batch, 3, symmetric, false, Epi::FLUSH > 0);
     return gemm_launch<2>(ma, mb, rows, cols, k, batch, cut, symmetric, false, io, epi, fault, st);
 }
 
+template <int F>
 cudaError_t solve(const Problem& q, char* ws, cudaStream_t st) {
     unsigned int* fault = fault_word();
     if (!fault) return cudaErrorInvalidSymbol;
@@ -552,16 +562,16 @@ cudaError_t solve(const Problem& q, char* ws, cudaStream_t st) {
     Pair x = o.x, y = o.y;
     for (int k = 0; k < q.steps && e == cudaSuccess; k++) {
         // G: the short side's products along the long one
-        e = multiply(x, tall, x, tall, s, s, l, q.batch, true, Pair{}, o.g, SquareEpi{0.0f, 1.0f / SCALE}, fault, st);
+        e = multiply(x, tall, x, tall, s, s, l, q.batch, true, Pair{}, o.g, SquareEpi<F>{0.0f, 1.0f / SCALE}, fault, st);
         if (e != cudaSuccess) break;
-        e = multiply(o.g, false, o.g, false, s, s, s, q.batch, true, o.g, o.p, SquareEpi{NS_B, NS_C / SCALE}, fault, st);
+        e = multiply(o.g, false, o.g, false, s, s, s, q.batch, true, o.g, o.p, SquareEpi<F>{NS_B, NS_C / SCALE}, fault, st);
         if (e != cudaSuccess) break;
         // i = rows of X, j = columns. Wide: P's rows by X^T's; tall: X's rows by P's
         const Pair &a = tall ? x : o.p, &b = tall ? o.p : x;
         if (k + 1 < q.steps)
-            e = multiply(a, false, b, !tall, q.rows, q.cols, s, q.batch, false, x, y, StepEpi{}, fault, st);
+            e = multiply(a, false, b, !tall, q.rows, q.cols, s, q.batch, false, x, y, StepEpi<F>{}, fault, st);
         else
-            e = multiply(a, false, b, !tall, q.rows, q.cols, s, q.batch, false, x, Pair{}, LastEpi{q}, fault, st);
+            e = multiply(a, false, b, !tall, q.rows, q.cols, s, q.batch, false, x, Pair{}, LastEpi<F>{q}, fault, st);
         const Pair t = x;
         x = y;
         y = t;
@@ -593,7 +603,7 @@ cudaError_t muon_update(const phyzb_muon_args& a, void* ws, cudaStream_t s) {
     q.mu = (float)a.mu;
     q.decay = (float)(1.0 - a.lr * a.weight_decay);
     q.lr = (float)(a.lr * a.scale);
-    return solve(q, (char*)ws, s);
+    return solve<0>(q, (char*)ws, s);
 }
 
 long long orthogonalize_workspace(const phyzb_orthogonalize_args& a) {
@@ -609,7 +619,7 @@ cudaError_t orthogonalize(const phyzb_orthogonalize_args& a, void* ws, cudaStrea
     q.g = view(a.x, a.x_stride);
     q.out = view(a.out, a.out_stride);
     q.dtype = q.out_dtype = a.dtype;
-    return solve(q, (char*)ws, s);
+    return solve<2>(q, (char*)ws, s);
 }
 
 cudaError_t muon_faults(unsigned int* n) { return cudaMemcpyFromSymbol(n, g_muon_fault, sizeof(*n)); }

@@ -507,6 +507,30 @@ def test_orthogonalize(dt, b, r, c):
     assert (t.transpose(1, 2).double() - want).norm() <= (NS_TOL + U[dt]) * want.norm()
 
 
+@pytest.mark.parametrize("r,c", [(128, 128), (100, 256), (300, 300), (515, 1030), (1024, 512)])
+def test_orthogonalize_is_as_near_as_f32_products(r, c):
+    """The header's claim: the error against 64 bits is that of the same iteration in f32 products, give or take the
+    chance in both (a factor of two) and a floor of 2^-20."""
+    x = rnd(gen(20), 1, r, c)
+    want, y = ns64(x), x / x.norm()
+    y = y.mT if r > c else y
+    for _ in range(5):
+        g = y @ y.mT
+        y = 3.4445 * y + (-4.7750 * g + 2.0315 * g @ g) @ y
+    y = y.mT if r > c else y
+    got, plain = ((v.double() - want).norm() / want.norm() for v in (nn.orthogonalize(x), y))
+    assert got <= 2 * plain + 2.0 ** -20
+
+
+@pytest.mark.parametrize("m,k,n", [(1000, 512, 512), (700, 2040, 1000)])
+def test_linear_f32_is_as_near_as_f32_products(m, k, n):
+    g = gen(21)
+    x, w = rnd(g, m, k), rnd(g, n, k, std=1 / math.sqrt(k))
+    want = x.double() @ w.double().t()
+    got, plain = ((v.double() - want).norm() / want.norm() for v in (nn.linear(x, w), x @ w.t()))
+    assert got <= 2 * plain
+
+
 @pytest.mark.parametrize("steps", [1, 2, 8])
 @pytest.mark.parametrize("r,c", [(48, 96), (300, 200)])
 def test_orthogonalize_steps(steps, r, c):
