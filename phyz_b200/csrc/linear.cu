@@ -81,7 +81,8 @@ __device__ __forceinline__ void store4(float* p, long long stride, int n, const 
 // beside their six products, and go straight.
 template <class T>
 struct Slotted {
-    static constexpr int PLANES = sizeof(T) == 2 ? 1 : 0, SLOTS = sizeof(T) == 2 ? 4 : 0, WARPS = 8, FLUSH = 4;
+    static constexpr int PLANES = sizeof(T) == 2 ? 1 : 0, SLOTS = sizeof(T) == 2 ? 2 : 0, WARPS = 8, FLUSH = 4;
+    static constexpr int WIDTH = sizeof(T) == 2 ? 64 : 32;
     static constexpr bool MIRROR = false;
 };
 
@@ -127,16 +128,19 @@ struct LinearEpi : Slotted<T> {
         }
     }
     __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, const float* sum,
-                                               const unsigned char* in, unsigned char* out) const {
+                                               const unsigned char* in, unsigned char* out, int h) const {
         if (i >= m) return;
-        T t[32];
+        constexpr int W = 8 * sizeof(T);  // words of 32 values
+        uint32_t w[W];
+        float z[32], r[32];
         // (the residual may be y itself: all 32 are read before any is written)
-        T r[32];
-        if (in)
-            slot_load(in, reinterpret_cast<uint32_t*>(r));
-        else if (res.p)
-            load32(res.p + i * res.is + j0 * res.js, res.js, cols, r);
-        float z[32];
+        if (in) {
+            slot_load<Slotted<T>::WIDTH>(in, h, w);
+            unpack32(w, r, T());
+        } else if (res.p) {
+            load32(res.p + i * res.is + j0 * res.js, res.js, cols, reinterpret_cast<T*>(w));
+            unpack32(w, r, T());
+        }
         if (bias && !by_i) {
             load32(bias + j0, 1, cols, z);
 #pragma unroll
@@ -147,20 +151,22 @@ struct LinearEpi : Slotted<T> {
             for (int c = 0; c < 32; c++) z[c] = sum[c] + b;
         }
         if (pre.p) {
-#pragma unroll
-            for (int c = 0; c < 32; c++) t[c] = from_f32<T>(z[c]);
-            store32(pre.p + i * pre.is + j0 * pre.js, pre.js, cols, t);
+            pack32(z, w, T());
+            store32(pre.p + i * pre.is + j0 * pre.js, pre.js, cols, reinterpret_cast<const T*>(w));
         }
         with_act(act, [&](auto kind) {
 #pragma unroll
             for (int c = 0; c < 32; c++) z[c] = act_f32(z[c], decltype(kind)::value);
         });
+        if (res.p) {
 #pragma unroll
-        for (int c = 0; c < 32; c++) t[c] = from_f32<T>(res.p ? z[c] + to_f32(r[c]) : z[c]);
+            for (int c = 0; c < 32; c++) z[c] += r[c];
+        }
+        pack32(z, w, T());
         if (out)
-            slot_store(out, reinterpret_cast<const uint32_t*>(t));
+            slot_store<Slotted<T>::WIDTH>(out, h, w);
         else
-            store32(y.p + i * y.is + j0 * y.js, y.js, cols, t);
+            store32(y.p + i * y.is + j0 * y.js, y.js, cols, reinterpret_cast<const T*>(w));
     }
 };
 
@@ -179,15 +185,14 @@ struct StoreEpi : Slotted<T> {
         if constexpr (sizeof(T) == 4) store4(out.p + i * out.is + j * out.js, along_i ? out.is : out.js, n, v);
     }
     __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, const float* v,
-                                               const unsigned char*, unsigned char* slot) const {
+                                               const unsigned char*, unsigned char* slot, int h) const {
         if (i >= m) return;
-        T t[32];
-#pragma unroll
-        for (int c = 0; c < 32; c++) t[c] = from_f32<T>(v[c]);
+        uint32_t w[8 * sizeof(T)];
+        pack32(v, w, T());
         if (slot)
-            slot_store(slot, reinterpret_cast<const uint32_t*>(t));
+            slot_store<Slotted<T>::WIDTH>(slot, h, w);
         else
-            store32(out.p + i * out.is + j0 * out.js, out.js, cols, t);
+            store32(out.p + i * out.is + j0 * out.js, out.js, cols, reinterpret_cast<const T*>(w));
     }
 };
 
@@ -205,8 +210,8 @@ GemmIo io_of(const LinearEpi<T>& e, long long rows, long long cols) {
     GemmIo io{};
     constexpr bool bf16 = !std::is_same<T, __half>::value;
     if constexpr (sizeof(T) == 2) {
-        io.writes = gemm_io_map(&io.out[0], e.y.p, e.y.is, e.y.js, 0, rows, cols, 1, bf16);
-        io.reads = e.res.p && gemm_io_map(&io.in[0], e.res.p, e.res.is, e.res.js, 0, rows, cols, 1, bf16);
+        io.writes = gemm_io_map(&io.out[0], e.y.p, e.y.is, e.y.js, 0, rows, cols, 1, bf16, Slotted<T>::WIDTH);
+        io.reads = e.res.p && gemm_io_map(&io.in[0], e.res.p, e.res.is, e.res.js, 0, rows, cols, 1, bf16, Slotted<T>::WIDTH);
     }
     return io;
 }
@@ -214,7 +219,8 @@ template <class T>
 GemmIo io_of(const StoreEpi<T>& e, long long rows, long long cols) {
     GemmIo io{};
     if constexpr (sizeof(T) == 2)
-        io.writes = gemm_io_map(&io.out[0], e.out.p, e.out.is, e.out.js, 0, rows, cols, 1, !std::is_same<T, __half>::value);
+        io.writes = gemm_io_map(&io.out[0], e.out.p, e.out.is, e.out.js, 0, rows, cols, 1, !std::is_same<T, __half>::value,
+                                Slotted<T>::WIDTH);
     return io;
 }
 
@@ -230,7 +236,7 @@ struct PartEpi : Slotted<float> {
         store4(part + (split * m + i) * n + j, along_i ? n : 1, k, v);
     }
     __device__ __forceinline__ void operator()(const GemmUnit& q, long long i, int j0, int cols, const float* v,
-                                               const unsigned char*, unsigned char*) const {
+                                               const unsigned char*, unsigned char*, int) const {
         if (i < m) store32(part + (q.split * m + i) * n + j0, 1, cols, v);
     }
 };

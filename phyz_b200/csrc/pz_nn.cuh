@@ -80,6 +80,45 @@ __device__ __forceinline__ void store32(T* p, long long stride, int n, const T* 
     }
 }
 
+// 32 values as 16 words of pairs, and back
+__device__ __forceinline__ void pack32(const float* v, uint32_t* w, __nv_bfloat16) {
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&p);
+    }
+}
+__device__ __forceinline__ void pack32(const float* v, uint32_t* w, __half) {
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const __half2 p = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&p);
+    }
+}
+__device__ __forceinline__ void pack32(const float* v, uint32_t* w, float) {
+#pragma unroll
+    for (int k = 0; k < 32; k++) w[k] = __float_as_uint(v[k]);
+}
+__device__ __forceinline__ void unpack32(const uint32_t* w, float* v, __nv_bfloat16) {
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        v[2 * k] = __uint_as_float(w[k] << 16);
+        v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void unpack32(const uint32_t* w, float* v, __half) {
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+        v[2 * k] = f.x;
+        v[2 * k + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void unpack32(const uint32_t* w, float* v, float) {
+#pragma unroll
+    for (int k = 0; k < 32; k++) v[k] = __uint_as_float(w[k]);
+}
+
 // f with the activation as a constant
 template <class F>
 __device__ __forceinline__ void with_act(int act, F f) {
