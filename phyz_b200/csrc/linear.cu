@@ -81,8 +81,8 @@ __device__ __forceinline__ void store4(float* p, long long stride, int n, const 
 // beside their six products, and go straight.
 template <class T>
 struct Slotted {
-    static constexpr int PLANES = sizeof(T) == 2 ? 1 : 0, SLOTS = sizeof(T) == 2 ? 2 : 0, WARPS = 8, FLUSH = 4;
-    static constexpr int WIDTH = sizeof(T) == 2 ? 64 : 32;
+    static constexpr int PLANES = sizeof(T) == 2 ? 1 : 0, SLOTS = sizeof(T) == 2 ? 2 : 0, WARPS = sizeof(T) == 2 ? 16 : 8, FLUSH = 4;
+    static constexpr int WIDTH = sizeof(T) == 2 ? 32 : 32;
     static constexpr bool MIRROR = false;
 };
 
@@ -98,7 +98,8 @@ struct LinearEpi : Slotted<T> {
     __device__ __forceinline__ void one(long long i, long long j, float z) const {
         if (bias) z += bias[by_i ? i : j];
         if (pre.p) pre.p[i * pre.is + j * pre.js] = from_f32<T>(z);
-        float v = act_f32(z, act);
+        float v = z, unused = 0.0f;
+        with_act(act, [&](auto kind) { act_pair<decltype(kind)::value>(v, unused); });
         if (res.p) v += to_f32(res.p[i * res.is + j * res.js]);
         y.p[i * y.is + j * y.js] = from_f32<T>(v);
     }
@@ -123,32 +124,30 @@ struct LinearEpi : Slotted<T> {
             if (pre.p) store4(pre.p + i * pre.is + j * pre.js, along_i ? pre.is : pre.js, n, z);
             if (res.p) load4(res.p + i * res.is + j * res.js, along_i ? res.is : res.js, n, r);
 #pragma unroll
-            for (int e = 0; e < 4; e++) z[e] = act_f32(z[e], K::value) + r[e];
+            for (int e = 0; e < 4; e += 2) act_pair<K::value>(z[e], z[e + 1]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) z[e] += r[e];
             store4(y.p + i * y.is + j * y.js, along_i ? y.is : y.js, n, z);
         }
     }
-    __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, const float* sum,
+    __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, float* z,
                                                const unsigned char* in, unsigned char* out, int h) const {
         if (i >= m) return;
-        constexpr int W = 8 * sizeof(T);  // words of 32 values
-        uint32_t w[W];
-        float z[32], r[32];
-        // (the residual may be y itself: all 32 are read before any is written)
-        if (in) {
-            slot_load<Slotted<T>::WIDTH>(in, h, w);
-            unpack32(w, r, T());
-        } else if (res.p) {
-            load32(res.p + i * res.is + j0 * res.js, res.js, cols, reinterpret_cast<T*>(w));
-            unpack32(w, r, T());
-        }
-        if (bias && !by_i) {
-            load32(bias + j0, 1, cols, z);
+        uint32_t w[8 * sizeof(T)];  // 32 values
+        if (bias) {
+            if (by_i) {
+                const float b = bias[i];
 #pragma unroll
-            for (int c = 0; c < 32; c++) z[c] += sum[c];
-        } else {
-            const float b = bias ? bias[i] : 0.0f;
+                for (int c = 0; c < 32; c++) z[c] += b;
+            } else {
 #pragma unroll
-            for (int c = 0; c < 32; c++) z[c] = sum[c] + b;
+                for (int c = 0; c < 32; c += 8) {
+                    float b[8];
+                    load8(bias + j0 + c, cols - c, b);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) z[c + e] += b[e];
+                }
+            }
         }
         if (pre.p) {
             pack32(z, w, T());
@@ -156,11 +155,14 @@ struct LinearEpi : Slotted<T> {
         }
         with_act(act, [&](auto kind) {
 #pragma unroll
-            for (int c = 0; c < 32; c++) z[c] = act_f32(z[c], decltype(kind)::value);
+            for (int c = 0; c < 32; c += 2) act_pair<decltype(kind)::value>(z[c], z[c + 1]);
         });
-        if (res.p) {
-#pragma unroll
-            for (int c = 0; c < 32; c++) z[c] += r[c];
+        if (res.p) {  // (the residual may be y itself: a lane's are read before they are written)
+            if (in)
+                slot_load<Slotted<T>::WIDTH>(in, h, w);
+            else
+                load32(res.p + i * res.is + j0 * res.js, res.js, cols, reinterpret_cast<T*>(w));
+            add32(w, z, T());
         }
         pack32(z, w, T());
         if (out)
@@ -552,7 +554,11 @@ constexpr int DZ_INNER = 2048;  // inner values of a block, where it sums along 
 template <class T>
 __device__ __forceinline__ float dz_value(const DzArgs& a, long long o, long long i) {
     float v = to_f32(((const T*)a.dy)[o * a.dy_o + i * a.dy_i]);
-    if (a.act != PHYZB_ACT_NONE) v *= act_grad_f32(to_f32(((const T*)a.pre)[o * a.pre_o + i * a.pre_i]), a.act);
+    if (a.act != PHYZB_ACT_NONE) {
+        float z = to_f32(((const T*)a.pre)[o * a.pre_o + i * a.pre_i]), unused = 0.0f;
+        with_act(a.act, [&](auto kind) { act_grad_pair<decltype(kind)::value>(z, unused); });
+        v *= z;
+    }
     return v;
 }
 template <class T>
@@ -593,9 +599,19 @@ __global__ void __launch_bounds__(256, 4) dz_rows_kernel(const __grid_constant__
             }
             float v[V];
 #pragma unroll
-            for (int e = 0; e < V; e++) {
+            for (int e = 0; e < V; e += 2) {
+                const int f = V > 1 ? e + 1 : 0;
                 v[e] = to_f32(d[e]);
-                if (ACT != PHYZB_ACT_NONE) v[e] *= act_grad_f32(to_f32(z[e]), ACT);
+                v[f] = to_f32(d[f]);
+                if (ACT != PHYZB_ACT_NONE) {
+                    float p = to_f32(z[e]), q = to_f32(z[f]);
+                    act_grad_pair<ACT>(p, q);
+                    v[e] *= p;
+                    if (V > 1) v[f] *= q;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < V; e++) {
                 sum[e] += v[e];
                 out[e] = from_f32<T>(v[e]);
             }

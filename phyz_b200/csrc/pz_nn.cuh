@@ -99,13 +99,6 @@ __device__ __forceinline__ void pack32(const float* v, uint32_t* w, float) {
 #pragma unroll
     for (int k = 0; k < 32; k++) w[k] = __float_as_uint(v[k]);
 }
-__device__ __forceinline__ void unpack32(const uint32_t* w, float* v, __nv_bfloat16) {
-#pragma unroll
-    for (int k = 0; k < 16; k++) {
-        v[2 * k] = __uint_as_float(w[k] << 16);
-        v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-    }
-}
 __device__ __forceinline__ void unpack32(const uint32_t* w, float* v, __half) {
 #pragma unroll
     for (int k = 0; k < 16; k++) {
@@ -114,9 +107,35 @@ __device__ __forceinline__ void unpack32(const uint32_t* w, float* v, __half) {
         v[2 * k + 1] = f.y;
     }
 }
-__device__ __forceinline__ void unpack32(const uint32_t* w, float* v, float) {
+// v += the values
+__device__ __forceinline__ void add32(const uint32_t* w, float* v, __nv_bfloat16) {
 #pragma unroll
-    for (int k = 0; k < 32; k++) v[k] = __uint_as_float(w[k]);
+    for (int k = 0; k < 16; k++) {
+        v[2 * k] += __uint_as_float(w[k] << 16);
+        v[2 * k + 1] += __uint_as_float(w[k] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void add32(const uint32_t* w, float* v, __half) {
+#pragma unroll
+    for (int k = 0; k < 16; k++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+        v[2 * k] += f.x;
+        v[2 * k + 1] += f.y;
+    }
+}
+__device__ __forceinline__ void add32(const uint32_t* w, float* v, float) {
+#pragma unroll
+    for (int k = 0; k < 32; k++) v[k] += __uint_as_float(w[k]);
+}
+// 8 neighbours, n of them there
+__device__ __forceinline__ void load8(const float* p, int n, float* v) {
+    if (n >= 8 && ((uintptr_t)p & 15) == 0) {
+        *(float4*)v = *(const float4*)p;
+        *(float4*)(v + 4) = *(const float4*)(p + 4);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = e < n ? p[e] : 0.0f;
+    }
 }
 
 // f with the activation as a constant
@@ -143,50 +162,79 @@ constexpr float LOG2E = 1.4426950408889634f;
 // within 2^-22 of the sigmoid near 1 and of e^z near 0
 __device__ __forceinline__ float sigmoid_f32(float z) { return sigmoid2_f32(z * LOG2E); }
 
-// tanh z = 2 sigmoid(2z) - 1; below 1/8, where that cancels, its series to z^7
-// (the next term is under 2^-29 of it).
-__device__ __forceinline__ float tanh_f32(float z) {
+// Two of them by one reciprocal, 1 / (a b): the exp and reciprocal unit is what an
+// epilogue or a gradient pass with an activation waits for (two of them a value
+// took 146 of 478 us at 262144 x 1024 values). Arguments are cut at -60, where
+// a sigmoid of 2^-60 stands for less, so that a b stays finite.
+__device__ __forceinline__ void sigmoid2_pair(float x, float y, float& s, float& t) {
+    float e, f, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(-x, 60.0f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(fminf(-y, 60.0f)));
+    e += 1.0f;
+    f += 1.0f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e * f));
+    s = r * f;
+    t = r * e;
+}
+
+// tanh z = 2 sigmoid(2z) - 1 = 2 s - 1; below 1/8, where that cancels, its series to
+// z^7 (the next term is under 2^-29 of it).
+__device__ __forceinline__ float tanh_of(float z, float s) {
     const float q = z * z;
-    const float s = z * fmaf(q, fmaf(q, fmaf(q, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-    const float t = fmaf(2.0f, sigmoid2_f32(z * (2.0f * LOG2E)), -1.0f);
-    return fabsf(z) < 0.125f ? s : t;
+    const float p = z * fmaf(q, fmaf(q, fmaf(q, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    return fabsf(z) < 0.125f ? p : fmaf(2.0f, s, -1.0f);
 }
 
 constexpr float GELU_C = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float GELU_K = 0.044715f;
-// gelu(z) = z (1 + tanh u) / 2 = z sigmoid(2u), u = C (z + K z^3)
-__device__ __forceinline__ float gelu_gate(float z, float q) {
-    return sigmoid2_f32(z * fmaf(q, 2.0f * LOG2E * GELU_C * GELU_K, 2.0f * LOG2E * GELU_C));
-}
 
-__device__ __forceinline__ float act_f32(float z, int act) {
-    switch (act) {
-        case PHYZB_ACT_RELU: return z > 0.0f || z != z ? z : 0.0f;
-        case PHYZB_ACT_TANH: return tanh_f32(z);
-        case PHYZB_ACT_SILU: return z * sigmoid_f32(z);
-        case PHYZB_ACT_GELU: return z * gelu_gate(z, z * z);
-        default: return z;
-    }
+// What an activation's sigmoid is of, over log2 e: gelu(z) = z (1 + tanh u) / 2 =
+// z sigmoid(2u), u = C (z + K z^3).
+template <int ACT>
+__device__ __forceinline__ float act_inner(float z) {
+    if (ACT == PHYZB_ACT_TANH) return z * (2.0f * LOG2E);
+    if (ACT == PHYZB_ACT_SILU) return z * LOG2E;
+    return z * fmaf(z * z, 2.0f * LOG2E * GELU_C * GELU_K, 2.0f * LOG2E * GELU_C);
 }
-
-// d act / dz
-__device__ __forceinline__ float act_grad_f32(float z, int act) {
-    switch (act) {
-        case PHYZB_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
-        case PHYZB_ACT_TANH: {
-            const float t = tanh_f32(z);
-            return fmaf(-t, t, 1.0f);
-        }
-        case PHYZB_ACT_SILU: {
-            const float s = sigmoid_f32(z);
-            return fmaf(fmaf(-s, s, s), z, s);
-        }
-        case PHYZB_ACT_GELU: {
-            const float q = z * z, s = gelu_gate(z, q);
-            return fmaf(fmaf(-s, s, s), z * fmaf(q, 6.0f * GELU_C * GELU_K, 2.0f * GELU_C), s);
-        }
-        default: return 1.0f;
+// two values through the activation, in place (a NaN stays a NaN)
+template <int ACT>
+__device__ __forceinline__ void act_pair(float& x, float& y) {
+    if (ACT == PHYZB_ACT_NONE) return;
+    if (ACT == PHYZB_ACT_RELU) {
+        x = x > 0.0f || x != x ? x : 0.0f;
+        y = y > 0.0f || y != y ? y : 0.0f;
+        return;
     }
+    float s, t;
+    sigmoid2_pair(act_inner<ACT>(x), act_inner<ACT>(y), s, t);
+    x = ACT == PHYZB_ACT_TANH ? (x == x ? tanh_of(x, s) : x) : x * s;
+    y = ACT == PHYZB_ACT_TANH ? (y == y ? tanh_of(y, t) : y) : y * t;
+}
+// d act / dz of two values
+template <int ACT>
+__device__ __forceinline__ void act_grad_pair(float& x, float& y) {
+    if (ACT == PHYZB_ACT_NONE) {
+        x = y = 1.0f;
+        return;
+    }
+    if (ACT == PHYZB_ACT_RELU) {
+        x = x > 0.0f ? 1.0f : 0.0f;
+        y = y > 0.0f ? 1.0f : 0.0f;
+        return;
+    }
+    float s, t;
+    sigmoid2_pair(act_inner<ACT>(x), act_inner<ACT>(y), s, t);
+    auto slope = [](float z, float s) {
+        if (ACT == PHYZB_ACT_TANH) {
+            const float t = tanh_of(z, s);
+            return z == z ? fmaf(-t, t, 1.0f) : z;
+        }
+        const float q = fmaf(-s, s, s);  // s (1 - s)
+        if (ACT == PHYZB_ACT_SILU) return fmaf(q, z, s);
+        return fmaf(q, z * fmaf(z * z, 6.0f * GELU_C * GELU_K, 2.0f * GELU_C), s);
+    };
+    x = slope(x, s);
+    y = slope(y, t);
 }
 
 }  // namespace pz
