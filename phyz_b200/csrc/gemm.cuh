@@ -14,7 +14,10 @@
 // CTAS = 2: the two blocks of a cluster (the SMs of a pair) make one tile of 256 x
 // BN: each brings its 128 rows of A and half of B's, one mma reads both shared
 // memories, and each gets its rows' sums. A tile of 128 x 256 alone takes 96 bytes
-// a clock from L2 for every SM, more than it gives; the pair's takes 64.
+// a clock from L2 for every SM, more than it gives (13.8 TB/s were measured, about
+// 50); the pair's takes 64. Measured without an epilogue, 262144 x 1024 x 1024
+// bf16: pairs of 256 columns 390 us (1.41 PFLOP/s), of 128 637, lone blocks of 128
+// 620.
 //
 // PL > 1: each operand is PL 16-bit planes whose sum is the value, and D is the
 // sum of the plane products that matter: two planes hi hi + (hi lo + lo hi);

@@ -395,7 +395,8 @@ cudaError_t simt_multiply(const SimtOperand& a, const SimtOperand& b, long long 
 
 constexpr int FEW = 8;
 
-// A warp takes a feature: its weights once, 16 bytes a lane where V > 1, against
+// Bound by the weights' bytes, or by latency: one row of 512 to 1024 features, 1 MB
+// of bf16 weights, 2.7 us. A warp takes a feature: its weights once, 16 bytes a lane where V > 1, against
 // M rows of x (which stay in the caches), sums in f32, joined by shuffles; lane r
 // finishes row r.
 template <class T, int M, int V>
@@ -575,7 +576,8 @@ __device__ __forceinline__ void dz_store(const DzArgs& a, long long o, long long
 }
 
 // inner = features. V neighbours per thread, 256 threads = 32 along the features
-// x 8 rows.
+// x 8 rows. Bound by memory, and by the slope's instructions: 65536 x 1024 bf16
+// with gelu, 403 MB, 86 us (4.7 TB/s).
 template <class T, int V>
 __global__ void __launch_bounds__(256, 4) dz_rows_kernel(const __grid_constant__ DzArgs a) {
     __shared__ float sums[8][32 * V];

@@ -162,10 +162,11 @@ constexpr float LOG2E = 1.4426950408889634f;
 // within 2^-22 of the sigmoid near 1 and of e^z near 0
 __device__ __forceinline__ float sigmoid_f32(float z) { return sigmoid2_f32(z * LOG2E); }
 
-// Two of them by one reciprocal, 1 / (a b): the exp and reciprocal unit is what an
-// epilogue or a gradient pass with an activation waits for (two of them a value
-// took 146 of 478 us at 262144 x 1024 values). Arguments are cut at -60, where
-// a sigmoid of 2^-60 stands for less, so that a b stays finite.
+// Two of them by one reciprocal, 1 / (a b): exp and reciprocal share a unit of a
+// quarter of the lanes, and activations are what an epilogue takes longest over
+// (146 of 478 us at 262144 x 1024 values, before it had sixteen warps).
+// Arguments are cut at -60, where a sigmoid of 2^-60 stands for less, so that
+// a b stays finite.
 __device__ __forceinline__ void sigmoid2_pair(float x, float y, float& s, float& t) {
     float e, f, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(-x, 60.0f)));

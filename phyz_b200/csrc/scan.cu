@@ -47,6 +47,8 @@ struct alignas(16) Bytes16 {
 };
 
 // V = 1: any strides. V = 16 bytes of values: channels contiguous and aligned.
+// Bound by memory and by a launch's own two microseconds: 4096 x 256 f32, 21 MB,
+// 4.6 us.
 template <class T, int V>
 __global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ phyzb_scan_args a) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -141,7 +143,13 @@ __device__ __forceinline__ void finish(const Side& s, long long b, long long c, 
 constexpr int NT = 128;  // threads of a block; its chains in lane_kernel: cw along c x NT / cw rows of b
 
 // Boxes of 4 KB, two stages ahead and two behind: 24 KB a block forward, 48
-// backward (six and four blocks to an SM).
+// backward (six and four blocks to an SM). Measured: 64 x 64 x 16384 f32 in the
+// history's order with resets 131 us, 6.2 TB/s or 95 % of a plain copy; backward 64 x
+// 1024 x 1024 bf16 141 us, 5.7 TB/s; 2 x 32769 x 512 bf16, cut in 108, 64 us with
+// its first launch's 27. Longer boxes or a third stage leave room for fewer
+// blocks: 188 us instead of 149 backward. Blocks of 64 threads: the same. Eight
+// warps to 32 chains, each with a run of the steps and a join a tile, took 32
+// instructions a value and 86 us where this takes 64.
 template <class T, bool BWD, bool OUT>
 struct Lane {
     static constexpr int S = 32 / (int)sizeof(T);  // steps of a tile

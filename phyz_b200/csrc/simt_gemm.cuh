@@ -15,7 +15,8 @@ struct SimtOperand {
 // 256 threads compute a 128 x 64 tile, 8 x 4 values each (two groups of four
 // rows 64 apart, four columns), from stages of 16 k in shared memory; the next
 // stage is loaded into registers while the current one is multiplied. blockIdx
-// = (tiles of i, tiles of j, split of the k range). ALONG_I: D is contiguous in
+// = (tiles of i, tiles of j, split of the k range). Bound by instructions: 65536 x
+// 30 x 64 with bias, tanh and pre-activations, 41 MB, 18.5 us. ALONG_I: D is contiguous in
 // i; lanes then run along i, and the epilogue gets four values along it.
 // Epi: each(f) calls f(kind) once, and f void four(kind, int split, long long i, long long j, const float* v, int n,
 // bool along_i)
