@@ -29,7 +29,7 @@ int guarded(F f) {
 
 int bad(const std::string& msg) { return fail(PHYZB_ERR_INVALID, msg); }
 
-constexpr int64_t MAX_SIDE = (int64_t)1 << 31;   // one side of an array
+constexpr int64_t MAX_SIDE = ((int64_t)1 << 31) - 1024;  // one side of an array (32-bit tile coordinates)
 constexpr int64_t MAX_SPAN = (int64_t)1 << 46;   // elements that an array spans
 
 int check_dtype(int dtype, const char* what) {
@@ -43,7 +43,7 @@ int check_sides(const int64_t* v, const char* const* names, int n, int64_t lo) {
     for (int i = 0; i < n; i++)
         if (v[i] < lo || v[i] >= MAX_SIDE)
             return bad(std::string(names[i]) + " = " + std::to_string(v[i]) + " not in " + std::to_string(lo) +
-                       "..2^31-1");
+                       ".." + std::to_string(MAX_SIDE - 1));
     return PHYZB_OK;
 }
 
@@ -141,7 +141,7 @@ int check(const phyzb_scan_args* a) {
     const int64_t n[] = {a->b, a->t, a->c}, bc[] = {a->b, a->c};
     const char* names[] = {"b", "t", "c"};
     PZ_TRY(check_sides(n, names, 3, 0));
-    if (a->b && a->c && a->b > MAX_SIDE * 64 / a->c) return bad("b * c exceeds 2^37 chains");
+    if (a->c && a->b > ((int64_t)1 << 37) / a->c) return bad("b * c exceeds 2^37 chains");
     if (a->b == 0 || a->c == 0) return PHYZB_OK;
     const int e = esize(a->dtype);
     if (a->h0) PZ_TRY(check_array(a->h0, a->h0_stride, bc, 2, 4, false, "h0"));
@@ -159,7 +159,7 @@ int check(const phyzb_scan_grad_args* a) {
     const int64_t n[] = {a->b, a->t, a->c}, bc[] = {a->b, a->c};
     const char* names[] = {"b", "t", "c"};
     PZ_TRY(check_sides(n, names, 3, 0));
-    if (a->b && a->c && a->b > MAX_SIDE * 64 / a->c) return bad("b * c exceeds 2^37 chains");
+    if (a->c && a->b > ((int64_t)1 << 37) / a->c) return bad("b * c exceeds 2^37 chains");
     if (a->b == 0 || a->c == 0) return PHYZB_OK;
     const int e = esize(a->dtype);
     if (a->h0) PZ_TRY(check_array(a->h0, a->h0_stride, bc, 2, 4, false, "h0"));

@@ -33,8 +33,6 @@
 #include "pz_tma.cuh"
 #include "pz_tma.h"
 
-#include <atomic>
-
 namespace pz {
 
 constexpr int GEMM_BM = 128, GEMM_BK = 64;
@@ -644,21 +642,6 @@ inline bool gemm_map(GemmSide* s, int plane, const GemmMat& m, long long rows, l
            CUDA_SUCCESS;
 }
 
-// A kernel's shared memory, set once per device (two threads that both do so
-// set the same).
-struct GemmOnce {
-    std::atomic<bool> ready[64];
-    template <class F>
-    cudaError_t smem(F* kernel, int bytes) {
-        int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
-        if (e != cudaSuccess || (dev < 64 && ready[dev].load(std::memory_order_acquire))) return e;
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e == cudaSuccess && dev < 64) ready[dev].store(true, std::memory_order_release);
-        return e;
-    }
-};
-
 // How a product is cut.
 struct GemmCut {
     int ctas, bn, splits;
@@ -727,7 +710,7 @@ cudaError_t gemm_launch_as(const GemmMat* a, const GemmMat* b, long long ma, lon
     g.idesc = 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (uint32_t)g.a.mn << 15 |
               (uint32_t)g.b.mn << 16 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(S::ROWS >> 4) << 24;
     auto kernel = gemm_kernel<BN, PL, CTAS, Epi>;
-    static GemmOnce once;
+    static SmemOnce once;
     const cudaError_t e = once.smem(kernel, S::BYTES);
     if (e != cudaSuccess) return e;
     const int slots = GEMM_SMS / CTAS;

@@ -26,19 +26,9 @@ namespace {
 
 __device__ unsigned int g_linear_fault;  // waits that ran out (pz_tma.cuh)
 
-// Each device's address of g_linear_fault (a kernel of another file's template
-// gets it as an argument).
 unsigned int* fault_word() {
-    static std::atomic<unsigned int*> at[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return nullptr;
-    unsigned int* p = at[dev].load(std::memory_order_acquire);
-    if (!p) {
-        void* q = nullptr;
-        if (cudaGetSymbolAddress(&q, g_linear_fault) != cudaSuccess) return nullptr;
-        at[dev].store(p = (unsigned int*)q, std::memory_order_release);
-    }
-    return p;
+    static FaultWord word;
+    return word.get(g_linear_fault);
 }
 
 long long up(long long v, long long to = 256) { return (v + to - 1) / to * to; }
@@ -396,9 +386,9 @@ cudaError_t simt_multiply(const SimtOperand& a, const SimtOperand& b, long long 
 constexpr int FEW = 8;
 
 // Bound by the weights' bytes, or by latency: one row of 512 to 1024 features, 1 MB
-// of bf16 weights, 2.7 us. A warp takes a feature: its weights once, 16 bytes a lane where V > 1, against
-// M rows of x (which stay in the caches), sums in f32, joined by shuffles; lane r
-// finishes row r.
+// of bf16 weights, 2.7 us. A warp takes a feature: its weights once, 16 bytes a lane
+// where V > 1, against M rows of x (which stay in the caches), sums in f32, joined
+// by shuffles; lane r finishes row r.
 template <class T, int M, int V>
 __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ phyzb_linear_args a, LinearEpi<T> epi) {
     const int lane = threadIdx.x % 32;
@@ -645,26 +635,30 @@ __global__ void __launch_bounds__(256, 4) dz_rows_kernel(const __grid_constant__
 template <class T>
 __global__ void __launch_bounds__(256) dz_features_kernel(const __grid_constant__ DzArgs a) {
     __shared__ float sums[8];
-    const long long i0 = (long long)blockIdx.x * DZ_INNER, o = blockIdx.y;
-    float sum = 0.0f;
+    const long long i0 = (long long)blockIdx.x * DZ_INNER;
+    for (long long o = blockIdx.y; o < a.outer; o += gridDim.y) {
+        float sum = 0.0f;
 #pragma unroll
-    for (int u = 0; u < DZ_INNER / 256; u++) {
-        const long long i = i0 + u * 256 + threadIdx.x;
-        if (i < a.inner) {
-            const float v = dz_value<T>(a, o, i);
-            dz_store<T>(a, o, i, v);
-            sum += v;
+        for (int u = 0; u < DZ_INNER / 256; u++) {
+            const long long i = i0 + u * 256 + threadIdx.x;
+            if (i < a.inner) {
+                const float v = dz_value<T>(a, o, i);
+                dz_store<T>(a, o, i, v);
+                sum += v;
+            }
         }
-    }
+        if (!a.part) continue;
 #pragma unroll
-    for (int s = 16; s; s /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-    if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0 && a.part) {
-        float s = 0.0f;
+        for (int s = 16; s; s /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            float s = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 8; w++) s += sums[w];
-        a.part[blockIdx.x * a.outer + o] = s;
+            for (int w = 0; w < 8; w++) s += sums[w];
+            a.part[blockIdx.x * a.outer + o] = s;
+        }
+        __syncthreads();
     }
 }
 
@@ -714,6 +708,7 @@ struct Backward {
         plane = up(pitch * outer, 128);
         // fewer lines to a block while blocks are fewer than four per SM
         lines = DZ_OUTER;
+        while (outer / lines >= 65535) lines *= 2;
         while (lines > 16 && (outer + lines - 1) / lines * ((inner + 255) / 256) < 4 * GEMM_SMS) lines /= 2;
         blocks = features ? (inner + DZ_INNER - 1) / DZ_INNER : (outer + lines - 1) / lines;
         // (both products of a layer have the same size: one way serves both)
@@ -778,7 +773,7 @@ cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st)
             return (uintptr_t)q % 16 == 0 && is == 1 && (p.outer == 1 || os % V == 0);
         };
         if (p.features) {
-            dz_features_kernel<T><<<dim3((unsigned)p.blocks, (unsigned)p.outer), 256, 0, st>>>(d);
+            dz_features_kernel<T><<<dim3((unsigned)p.blocks, (unsigned)(p.outer < 65535 ? p.outer : 65535)), 256, 0, st>>>(d);
         } else if (p.inner % V == 0 && wide(d.dy, d.dy_o, d.dy_i) &&
                    (a.activation == PHYZB_ACT_NONE || wide(d.pre, d.pre_o, d.pre_i))) {
             dz_rows_kernel<T, V><<<dim3((unsigned)((p.inner + 32 * V - 1) / (32 * V)), (unsigned)p.blocks), 256, 0, st>>>(d);

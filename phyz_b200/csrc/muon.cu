@@ -31,16 +31,8 @@ constexpr int NORM_BLOCKS = 512;  // partial sums of a matrix's |u|^2, at most
 __device__ unsigned int g_muon_fault;  // waits that ran out (pz_tma.cuh)
 
 unsigned int* fault_word() {
-    static std::atomic<unsigned int*> at[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return nullptr;
-    unsigned int* p = at[dev].load(std::memory_order_acquire);
-    if (!p) {
-        void* q = nullptr;
-        if (cudaGetSymbolAddress(&q, g_muon_fault) != cudaSuccess) return nullptr;
-        at[dev].store(p = (unsigned int*)q, std::memory_order_release);
-    }
-    return p;
+    static FaultWord word;
+    return word.get(g_muon_fault);
 }
 
 // A stack of matrices: element (z, r, c) at p[z * zs + r * rs + c * cs].
@@ -502,7 +494,7 @@ bool is_small(long long rows, long long cols) {
 template <int LB, int V>
 cudaError_t run_small(const Problem& q, unsigned int* fault, cudaStream_t st) {
     auto kernel = small_kernel<LB, V>;
-    static GemmOnce once;
+    static SmemOnce once;
     const cudaError_t e = once.smem(kernel, Small<LB>::BYTES);
     if (e != cudaSuccess) return e;
     kernel<<<q.batch, SMALL_THREADS, Small<LB>::BYTES, st>>>(q, fault);

@@ -22,7 +22,6 @@
 #include "pz_tma.cuh"
 #include "pz_tma.h"
 
-#include <atomic>
 #include <type_traits>
 
 namespace pz {
@@ -504,21 +503,6 @@ Plan plan_of(const int64_t* n, int dtype, bool bwd, bool tma) {
     return cut(LOOSE, 1, (b * c + NT - 1) / NT, t, bwd ? loose_steps<true, true> : loose_steps<false, true>);
 }
 
-// A kernel's shared memory, set once per device (two threads that both do so
-// set the same).
-struct Once {
-    std::atomic<bool> ready[64];
-    template <class F>
-    cudaError_t smem(F* kernel, int bytes) {
-        int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
-        if (e != cudaSuccess || (dev < 64 && ready[dev].load(std::memory_order_acquire))) return e;
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e == cudaSuccess && dev < 64) ready[dev].store(true, std::memory_order_release);
-        return e;
-    }
-};
-
 // The tensor map of an array as (c, b, t), in boxes of `rows` rows of cw chains
 // at `steps` steps.
 template <class T>
@@ -535,7 +519,7 @@ template <class T, bool RESET, bool BWD, bool OUT>
 cudaError_t run_lanes(LaneArgs& a, cudaStream_t st) {
     using C = Lane<T, BWD, OUT>;
     auto kernel = lane_kernel<T, RESET, BWD, OUT>;
-    static Once once;
+    static SmemOnce once;
     const cudaError_t e = once.smem(kernel, C::BYTES);
     if (e != cudaSuccess) return e;
     a.units = a.ctiles * a.btiles * (OUT ? a.s.splits : a.s.splits - 1);

@@ -110,6 +110,29 @@ def test_linear_layouts(dt, how, m, k, n):
     check_forward(dt, m, k, n, "tanh", True, True, how)
 
 
+@pytest.mark.parametrize("k,n", [(30, 64), (1, 1), (64, 100), (300, 33), (37, 128)])
+@pytest.mark.parametrize("act", ["tanh", "none"])
+def test_linear_many_feature_major_rows(k, n, act):
+    """The policy history's shape: rows enough to fill the GPU, feature-major."""
+    check_forward(torch.float32, 19001, k, n, act, True, True, "features")
+    check_forward(torch.float32, 19001, k, n, act, False, False, "features")
+
+
+@pytest.mark.parametrize("how", ["rows", "features"])
+def test_linear_backward_more_rows_than_a_grid_side(how):
+    """9 million rows: more blocks of rows than a launch has along its second axis. With x = 1 and w = 1 the gradients
+    are sums of dy, whole numbers that f32 and bf16 hold exactly in every order."""
+    m = 9_000_000
+    dy = torch.zeros(m, 8, device="cuda", dtype=torch.bfloat16)
+    dy[::70_001] = 1
+    dy[-1] = 1
+    dy = layout(dy, how)
+    x, w = torch.ones(m, 8, device="cuda", dtype=torch.bfloat16), torch.ones(8, 8, device="cuda", dtype=torch.bfloat16)
+    dx, dw, db = nn.linear_backward(dy, x, w)
+    hits = float(dy[:, 0].sum(dtype=torch.float64))
+    assert (db == hits).all() and (dw == hits).all() and torch.equal(dx, (dy * 8).contiguous())
+
+
 @pytest.mark.parametrize("dt", TYPES)
 def test_linear_large(dt):
     check_forward(dt, 5003, 1032, 1000, "gelu", True, True, "rows")
