@@ -3,13 +3,12 @@
 //
 // One persistent block per SM walks tiles of D. Warp 0 brings 64-deep stages of
 // both operands by TMA into 128-byte-swizzled shared memory, warp 1 issues
-// tcgen05.mma into one of two accumulators in Tensor Memory, and eight or
-// sixteen more warps empty the other one through the epilogue, so that the tensor cores wait neither
-// for memory nor for the epilogue. In the epilogue a lane has 32 neighbours in j
-// and a warp 32 in i: a chunk. Where TMA can address them, what the epilogue reads
-// comes into the warp's own slots of shared memory a chunk ahead and what it
-// writes leaves from there: a lane's own 32-byte accesses to 32 rows keep the
-// memory pipe busy for longer than the tensor cores take for a K of 1024.
+// tcgen05.mma into one of two accumulators in Tensor Memory, and eight or sixteen
+// more warps empty the other one through the epilogue, so that the tensor cores
+// wait neither for memory nor for the epilogue. In the epilogue a lane has 32
+// neighbours in j and a warp 32 in i: a chunk. Where TMA can address them, what
+// the epilogue reads comes into the warp's own slots of shared memory a chunk
+// ahead, and what it writes leaves from there.
 //
 // CTAS = 2: the two blocks of a cluster (the SMs of a pair) make one tile of 256 x
 // BN: each brings its 128 rows of A and half of B's, one mma reads both shared
@@ -38,8 +37,8 @@ namespace pz {
 constexpr int GEMM_BM = 128, GEMM_BK = 64;
 constexpr int GEMM_SMS = 148;
 
-// A chunk's slot: 32 rows of `width` (32 or 64) 16-bit values, one or two planes.
-__host__ __device__ constexpr int gemm_plane(int width) { return 32 * 2 * width; }
+// A chunk's slot: 32 rows of 32 16-bit values, one or two planes.
+constexpr int GEMM_PLANE = 32 * 64;
 
 template <int BN, int PL, int CTAS, class Epi>
 struct GemmShape {
@@ -47,15 +46,14 @@ struct GemmShape {
     static constexpr int BR = BN / CTAS;             // rows of B that a block brings
     static constexpr int A_BYTES = GEMM_BM * GEMM_BK * 2, B_BYTES = BR * GEMM_BK * 2;
     static constexpr int STAGE = PL * (A_BYTES + B_BYTES);
-    static constexpr int PLANE = gemm_plane(Epi::WIDTH);
-    static constexpr int WARP_SLOTS = Epi::PLANES * Epi::SLOTS * PLANE;
+    static constexpr int WARP_SLOTS = Epi::PLANES * Epi::SLOTS * GEMM_PLANE;
     static constexpr int THREADS = 32 * (2 + Epi::WARPS);
     static constexpr int SLOTS = Epi::WARPS * WARP_SLOTS;
     static constexpr int FIT = (224 * 1024 - SLOTS) / STAGE;
     static constexpr int STAGES = FIT > 6 ? 6 : FIT;
     static constexpr int ACCS = PL > 1 ? 2 : 1;      // main, small terms
     static constexpr int FLUSH = PL > 1 ? Epi::FLUSH : 0;
-    static constexpr int EVERY = Epi::WARPS / 4 * Epi::WIDTH;  // columns from one of a warp's chunks to the next
+    static constexpr int EVERY = Epi::WARPS * 8;  // columns from one of a warp's chunks to the next
     static constexpr int CHUNKS = (BN + EVERY - 1) / EVERY;   // of a warp in a tile, at most
     static constexpr int BUFS = 2 * ACCS * BN <= 512 ? 2 : 1;  // tiles in Tensor Memory
     static constexpr int COLS = BUFS * ACCS * BN;
@@ -71,7 +69,7 @@ struct GemmSide {
 };
 
 // What the epilogue reads and writes through slots: planes of arrays [batch][i][j]
-// (j contiguous) as tensor maps, in boxes of 32 rows x WIDTH.
+// (j contiguous) as tensor maps, in boxes of 32 x 32.
 struct GemmIo {
     CUtensorMap in[2], out[2];
     int reads, writes;  // whether through slots
@@ -238,34 +236,31 @@ __device__ __forceinline__ bool gemm_wait(uint64_t* bar, uint32_t parity, volati
     return true;
 }
 
-// Where 16 bytes (8 values, the c-th) of a row of a slot's plane are: 64- or
-// 128-byte swizzle, by the width.
-template <int WIDTH>
-__device__ __forceinline__ int slot_at(int row, int c) {
-    return WIDTH == 64 ? row * 128 + ((c ^ (row & 7)) << 4) : row * 64 + ((c ^ (row >> 1 & 3)) << 4);
-}
-// A lane's 32 values, the h-th of its row.
-template <int WIDTH>
-__device__ __forceinline__ void slot_load(const unsigned char* plane, int h, uint32_t* w) {
+// Where 16 bytes (8 values, the c-th) of a row of a slot's plane are (64-byte
+// swizzle).
+__device__ __forceinline__ int slot_at(int row, int c) { return row * 64 + ((c ^ (row >> 1 & 3)) << 4); }
+// A lane's 32 values.
+__device__ __forceinline__ void slot_load(const unsigned char* plane, uint32_t* w) {
 #pragma unroll
     for (int c = 0; c < 4; c++) {
-        const uint4 q = *reinterpret_cast<const uint4*>(plane + slot_at<WIDTH>(threadIdx.x % 32, h * 4 + c));
+        const uint4 q = *reinterpret_cast<const uint4*>(plane + slot_at(threadIdx.x % 32, c));
         w[4 * c] = q.x, w[4 * c + 1] = q.y, w[4 * c + 2] = q.z, w[4 * c + 3] = q.w;
     }
 }
-template <int WIDTH>
-__device__ __forceinline__ void slot_store(unsigned char* plane, int h, const uint32_t* w) {
+__device__ __forceinline__ void slot_store(unsigned char* plane, const uint32_t* w) {
 #pragma unroll
     for (int c = 0; c < 4; c++)
-        *reinterpret_cast<uint4*>(plane + slot_at<WIDTH>(threadIdx.x % 32, h * 4 + c)) =
+        *reinterpret_cast<uint4*>(plane + slot_at(threadIdx.x % 32, c)) =
             make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
 }
 
-// Epi: void operator()(const GemmUnit&, long long i, int j0, int cols, float* sum, const unsigned char* in, unsigned
-// char* out, int h) const for 32 columns from j0 (cols of them inside D) of row i, called by whole warps (rows past m
-// too). in, out: the chunk's slot where GemmIo says so (the same one; these are its h-th 32 columns), else null. WIDTH
-// of a chunk, PLANES of a slot, SLOTS of a warp, 4 to 16 WARPS. MIRROR:
-// where mirrored(unit, j0) says so, the chunk's mirror image is written as well, by turn(sum, slot). FLUSH: k blocks to a sum of the tensor cores, where a product has planes (0: all).
+// Epi: void operator()(const GemmUnit&, long long i, int j0, int cols, float* sum,
+// const unsigned char* in, unsigned char* out) const for 32 columns from j0 (cols
+// of them inside D) of row i, called by whole warps (rows past m too). in, out:
+// the chunk's slot where GemmIo says so (the same one), else null. PLANES of a
+// slot, SLOTS of a warp, 8 or 16 WARPS. MIRROR: where mirrored(unit, j0) says so,
+// the chunk's mirror image is written as well, by turn(sum, slot). FLUSH: k blocks
+// to a sum of the tensor cores, where a product has planes (0: all).
 template <int BN, int PL, int CTAS, class Epi>
 __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL, CTAS, Epi>::THREADS), 1)
     gemm_kernel(const __grid_constant__ GemmArgs g, const __grid_constant__ Epi epi, unsigned int* fault) {
@@ -414,7 +409,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
         }
     } else {
         // lanes 32 (warp % 4) .. of the accumulator are this warp's to read
-        const int quarter = warp % 4, from = (warp - 2) / 4 * Epi::WIDTH, own = rank * GEMM_BM + quarter * 32;
+        const int quarter = warp % 4, from = (warp - 2) / 4 * 32, own = rank * GEMM_BM + quarter * 32;
         constexpr int EVERY = S::EVERY;
         constexpr int NS = Epi::SLOTS, MOD = NS > 0 ? NS : 1;
         unsigned char* const mine = slots + (warp - 2) * S::WARP_SLOTS;
@@ -427,11 +422,11 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
             while (au < g.units) {
                 const bool there = ac < BN && aq.row0 + own < g.m && aq.j * BN + ac < g.n;
                 if (there) {
-                    unsigned char* const at = mine + asked % MOD * Epi::PLANES * S::PLANE;
-                    mbar_expect(&bars[asked % MOD], Epi::PLANES * S::PLANE);
+                    unsigned char* const at = mine + asked % MOD * Epi::PLANES * GEMM_PLANE;
+                    mbar_expect(&bars[asked % MOD], Epi::PLANES * GEMM_PLANE);
 #pragma unroll
                     for (int p = 0; p < Epi::PLANES; p++)
-                        tma_load(at + p * S::PLANE, &g.io.in[p], &bars[asked % MOD], aq.j * BN + ac, aq.row0 + own, aq.z);
+                        tma_load(at + p * GEMM_PLANE, &g.io.in[p], &bars[asked % MOD], aq.j * BN + ac, aq.row0 + own, aq.z);
                     asked++;
                     ac += EVERY;
                     return;
@@ -481,7 +476,6 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
             };
             const long long i = q.row0 + own + lane;
             const bool any = q.k0 < q.k1;
-            static_assert(!S::FLUSH || Epi::WIDTH == 32);
             float held[S::FLUSH ? S::CHUNKS : 1][32];  // FLUSH: the sums so far
             if constexpr (S::FLUSH > 0) {
 #pragma unroll
@@ -509,7 +503,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
             for (int m = 0; m < S::CHUNKS; m++) {
                 const int c = from + m * EVERY, j = q.j * BN + c;
                 if (c >= BN || j >= g.n || q.row0 + own >= g.m) break;
-                unsigned char* const at = mine + n % MOD * Epi::PLANES * S::PLANE;
+                unsigned char* const at = mine + n % MOD * Epi::PLANES * GEMM_PLANE;
                 if constexpr (NS > 0) {
                     if (writes || reads) {
                         // the slot of a chunk ahead, or this one's, is empty again
@@ -528,23 +522,19 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
                         if (!ok) break;
                     }
                 }
+                const int cols = g.n - j < 32 ? g.n - j : 32;
                 float v[32];
+                if constexpr (S::FLUSH > 0) {
 #pragma unroll
-                for (int h = 0; h < Epi::WIDTH / 32; h++) {
-                    const int jh = j + h * 32, cols = g.n - jh < 32 ? g.n - jh : 32;
-                    if (cols <= 0) break;
-                    if constexpr (S::FLUSH > 0) {
+                    for (int e = 0; e < 32; e++) v[e] = held[m][e];
+                } else {
+                    sum_of(c, v);
+                    if (!any) {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) v[e] = held[m][e];
-                    } else {
-                        sum_of(c + h * 32, v);
-                        if (!any) {
-#pragma unroll
-                            for (int e = 0; e < 32; e++) v[e] = 0.0f;
-                        }
+                        for (int e = 0; e < 32; e++) v[e] = 0.0f;
                     }
-                    epi(q, i, jh, cols, v, reads ? at : nullptr, writes ? at : nullptr, h);
                 }
+                epi(q, i, j, cols, v, reads ? at : nullptr, writes ? at : nullptr);
                 if constexpr (NS > 0) {
                     if (writes) {
                         fence_async();
@@ -552,7 +542,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
                         if (lane == 0) {  // (past m and n nothing is written)
 #pragma unroll
                             for (int p = 0; p < Epi::PLANES; p++)
-                                tma_store(&g.io.out[p], at + p * S::PLANE, j, q.row0 + own, q.z);
+                                tma_store(&g.io.out[p], at + p * GEMM_PLANE, j, q.row0 + own, q.z);
                             tma_store_commit();
                         }
                         if constexpr (Epi::MIRROR) {
@@ -565,7 +555,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
                                 if (lane == 0) {
 #pragma unroll
                                     for (int p = 0; p < Epi::PLANES; p++)
-                                        tma_store(&g.io.out[p], at + p * S::PLANE, q.row0 + own, j, q.z);
+                                        tma_store(&g.io.out[p], at + p * GEMM_PLANE, q.row0 + own, j, q.z);
                                     tma_store_commit();
                                 }
                             }
@@ -619,14 +609,13 @@ inline bool gemm_tma_ok(const GemmMat& m, long long rows, long long k, long long
 // The tensor map of a plane that an epilogue reads or writes: [batch][rows][cols],
 // cols contiguous. False where TMA cannot address it.
 inline bool gemm_io_map(CUtensorMap* m, const void* p, long long rs, long long cs, long long zs, long long rows,
-                        long long cols, long long batch, bool bf16, int width) {
+                        long long cols, long long batch, bool bf16) {
     if (cs != 1 || !gemm_tma_ok({p, rs, 1, zs}, rows, cols, batch)) return false;
     const cuuint64_t size[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch};
     const cuuint64_t stride[2] = {rows > 1 ? (cuuint64_t)rs * 2 : 16, batch > 1 ? (cuuint64_t)zs * 2 : 16};
-    const cuuint32_t box[3] = {(cuuint32_t)width, 32, 1};
+    const cuuint32_t box[3] = {32, 32, 1};
     return encode_tiled(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                        const_cast<void*>(p), size, stride, box,
-                        width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B) == CUDA_SUCCESS;
+                        const_cast<void*>(p), size, stride, box, CU_TENSOR_MAP_SWIZZLE_64B) == CUDA_SUCCESS;
 }
 
 inline bool gemm_map(GemmSide* s, int plane, const GemmMat& m, long long rows, long long k, long long batch, int tile,

@@ -71,8 +71,8 @@ __device__ __forceinline__ void store4(float* p, long long stride, int n, const 
 // beside their six products, and go straight.
 template <class T>
 struct Slotted {
-    static constexpr int PLANES = sizeof(T) == 2 ? 1 : 0, SLOTS = sizeof(T) == 2 ? 2 : 0, WARPS = sizeof(T) == 2 ? 16 : 8, FLUSH = 4;
-    static constexpr int WIDTH = sizeof(T) == 2 ? 32 : 32;
+    static constexpr int PLANES = sizeof(T) == 2 ? 1 : 0, SLOTS = sizeof(T) == 2 ? 2 : 0;
+    static constexpr int WARPS = sizeof(T) == 2 ? 16 : 8, FLUSH = 4;
     static constexpr bool MIRROR = false;
 };
 
@@ -121,7 +121,7 @@ struct LinearEpi : Slotted<T> {
         }
     }
     __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, float* z,
-                                               const unsigned char* in, unsigned char* out, int h) const {
+                                               const unsigned char* in, unsigned char* out) const {
         if (i >= m) return;
         uint32_t w[8 * sizeof(T)];  // 32 values
         if (bias) {
@@ -149,14 +149,14 @@ struct LinearEpi : Slotted<T> {
         });
         if (res.p) {  // (the residual may be y itself: a lane's are read before they are written)
             if (in)
-                slot_load<Slotted<T>::WIDTH>(in, h, w);
+                slot_load(in, w);
             else
                 load32(res.p + i * res.is + j0 * res.js, res.js, cols, reinterpret_cast<T*>(w));
             add32(w, z, T());
         }
         pack32(z, w, T());
         if (out)
-            slot_store<Slotted<T>::WIDTH>(out, h, w);
+            slot_store(out, w);
         else
             store32(y.p + i * y.is + j0 * y.js, y.js, cols, reinterpret_cast<const T*>(w));
     }
@@ -177,12 +177,12 @@ struct StoreEpi : Slotted<T> {
         if constexpr (sizeof(T) == 4) store4(out.p + i * out.is + j * out.js, along_i ? out.is : out.js, n, v);
     }
     __device__ __forceinline__ void operator()(const GemmUnit&, long long i, int j0, int cols, const float* v,
-                                               const unsigned char*, unsigned char* slot, int h) const {
+                                               const unsigned char*, unsigned char* slot) const {
         if (i >= m) return;
         uint32_t w[8 * sizeof(T)];
         pack32(v, w, T());
         if (slot)
-            slot_store<Slotted<T>::WIDTH>(slot, h, w);
+            slot_store(slot, w);
         else
             store32(out.p + i * out.is + j0 * out.js, out.js, cols, reinterpret_cast<const T*>(w));
     }
@@ -202,8 +202,8 @@ GemmIo io_of(const LinearEpi<T>& e, long long rows, long long cols) {
     GemmIo io{};
     constexpr bool bf16 = !std::is_same<T, __half>::value;
     if constexpr (sizeof(T) == 2) {
-        io.writes = gemm_io_map(&io.out[0], e.y.p, e.y.is, e.y.js, 0, rows, cols, 1, bf16, Slotted<T>::WIDTH);
-        io.reads = e.res.p && gemm_io_map(&io.in[0], e.res.p, e.res.is, e.res.js, 0, rows, cols, 1, bf16, Slotted<T>::WIDTH);
+        io.writes = gemm_io_map(&io.out[0], e.y.p, e.y.is, e.y.js, 0, rows, cols, 1, bf16);
+        io.reads = e.res.p && gemm_io_map(&io.in[0], e.res.p, e.res.is, e.res.js, 0, rows, cols, 1, bf16);
     }
     return io;
 }
@@ -211,8 +211,7 @@ template <class T>
 GemmIo io_of(const StoreEpi<T>& e, long long rows, long long cols) {
     GemmIo io{};
     if constexpr (sizeof(T) == 2)
-        io.writes = gemm_io_map(&io.out[0], e.out.p, e.out.is, e.out.js, 0, rows, cols, 1, !std::is_same<T, __half>::value,
-                                Slotted<T>::WIDTH);
+        io.writes = gemm_io_map(&io.out[0], e.out.p, e.out.is, e.out.js, 0, rows, cols, 1, !std::is_same<T, __half>::value);
     return io;
 }
 
@@ -228,7 +227,7 @@ struct PartEpi : Slotted<float> {
         store4(part + (split * m + i) * n + j, along_i ? n : 1, k, v);
     }
     __device__ __forceinline__ void operator()(const GemmUnit& q, long long i, int j0, int cols, const float* v,
-                                               const unsigned char*, unsigned char*, int) const {
+                                               const unsigned char*, unsigned char*) const {
         if (i < m) store32(part + (q.split * m + i) * n + j0, 1, cols, v);
     }
 };

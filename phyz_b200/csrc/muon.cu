@@ -173,9 +173,9 @@ __global__ void __launch_bounds__(256) normalize_kernel(const __grid_constant__ 
 __device__ __forceinline__ void pair_load(const unsigned char* in, float* v) {
     uint32_t w[16];
     float l[32];
-    slot_load<32>(in, 0, w);
+    slot_load(in, w);
     unpack32(w, v, __half());
-    slot_load<32>(in + gemm_plane(32), 0, w);
+    slot_load(in + GEMM_PLANE, w);
     unpack32(w, l, __half());
 #pragma unroll
     for (int k = 0; k < 32; k++) v[k] += l[k];
@@ -192,21 +192,21 @@ __device__ __forceinline__ void split(const float* v, __half* h, __half* l) {
 // in the workspace: all of this goes through slots.)
 template <int F>  // k blocks to a sum of the tensor cores (0: all)
 struct SquareEpi {
-    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8, FLUSH = F, WIDTH = 32;
+    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8, FLUSH = F;
     static constexpr bool MIRROR = true;
     float b, c;  // c / SCALE
     // the tile's mirror image is another one, unless it is inside a diagonal block
     __device__ __forceinline__ bool mirrored(const GemmUnit& q, int j0) const { return j0 < q.row0; }
     __device__ __forceinline__ void operator()(const GemmUnit& q, long long i, int j0, int cols, float* sum,
-                                               const unsigned char* in, unsigned char* out, int) const {
+                                               const unsigned char* in, unsigned char* out) const {
         float v[32];
         if (in) pair_load(in, v);
 #pragma unroll
         for (int k = 0; k < 32; k++) sum[k] = in ? fmaf(b, v[k], c * sum[k]) : c * sum[k];
         __half h[32], l[32];
         split(sum, h, l);
-        slot_store<32>(out, 0, reinterpret_cast<const uint32_t*>(h));
-        slot_store<32>(out + gemm_plane(32), 0, reinterpret_cast<const uint32_t*>(l));
+        slot_store(out, reinterpret_cast<const uint32_t*>(h));
+        slot_store(out + GEMM_PLANE, reinterpret_cast<const uint32_t*>(l));
     }
     __device__ __forceinline__ void turn(const float* v, unsigned char* out) const {
         __half h[32], l[32];
@@ -214,9 +214,9 @@ struct SquareEpi {
         const int lane = threadIdx.x % 32;
 #pragma unroll
         for (int k = 0; k < 32; k++) {
-            const int at = slot_at<32>(k, lane >> 3) + (lane & 7) * 2;
+            const int at = slot_at(k, lane >> 3) + (lane & 7) * 2;
             *reinterpret_cast<__half*>(out + at) = h[k];
-            *reinterpret_cast<__half*>(out + gemm_plane(32) + at) = l[k];
+            *reinterpret_cast<__half*>(out + GEMM_PLANE + at) = l[k];
         }
     }
 };
@@ -224,25 +224,25 @@ struct SquareEpi {
 // a X + sum; i along the rows of X, j along its columns.
 template <int F>
 struct StepEpi {
-    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8, FLUSH = F, WIDTH = 32;
+    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8, FLUSH = F;
     static constexpr bool MIRROR = false;
     __device__ __forceinline__ void operator()(const GemmUnit&, long long, int, int, const float* sum,
-                                               const unsigned char* in, unsigned char* out, int) const {
+                                               const unsigned char* in, unsigned char* out) const {
         float v[32];
         pair_load(in, v);
 #pragma unroll
         for (int k = 0; k < 32; k++) v[k] = fmaf(NS_A, v[k], sum[k] * (1.0f / SCALE));
         __half h[32], l[32];
         split(v, h, l);
-        slot_store<32>(out, 0, reinterpret_cast<const uint32_t*>(h));
-        slot_store<32>(out + gemm_plane(32), 0, reinterpret_cast<const uint32_t*>(l));
+        slot_store(out, reinterpret_cast<const uint32_t*>(h));
+        slot_store(out + GEMM_PLANE, reinterpret_cast<const uint32_t*>(l));
     }
 };
 
 // The last a X + sum, into the weights or the result.
 template <int F>
 struct LastEpi {
-    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8, FLUSH = F, WIDTH = 32;
+    static constexpr int PLANES = 2, SLOTS = 1, WARPS = 8, FLUSH = F;
     static constexpr bool MIRROR = false;
     Problem q;
     template <class T>
@@ -274,7 +274,7 @@ struct LastEpi {
         if (q.copy.p) write(q.copy, q.copy_dtype, at(q.copy), stride(q.copy), n, v);
     }
     __device__ __forceinline__ void operator()(const GemmUnit& u, long long i, int j0, int cols, float* sum,
-                                               const unsigned char* in, unsigned char*, int) const {
+                                               const unsigned char* in, unsigned char*) const {
         if (i >= q.rows) return;
         float v[32];
         pair_load(in, v);
@@ -512,9 +512,9 @@ cudaError_t multiply(const Pair& a, bool a_mn, const Pair& b, bool b_mn, long lo
     for (int h = 0; h < 2; h++) {
         ma[h] = {a.p + h * a.lo, a_mn ? 1 : a.pitch, a_mn ? a.pitch : 1, a.zs};
         mb[h] = {b.p + h * b.lo, b_mn ? 1 : b.pitch, b_mn ? b.pitch : 1, b.zs};
-        if (in.p && !gemm_io_map(&io.in[h], in.p + h * in.lo, in.pitch, 1, in.zs, rows, cols, batch, false, 32))
+        if (in.p && !gemm_io_map(&io.in[h], in.p + h * in.lo, in.pitch, 1, in.zs, rows, cols, batch, false))
             return cudaErrorInvalidValue;
-        if (out.p && !gemm_io_map(&io.out[h], out.p + h * out.lo, out.pitch, 1, out.zs, rows, cols, batch, false, 32))
+        if (out.p && !gemm_io_map(&io.out[h], out.p + h * out.lo, out.pitch, 1, out.zs, rows, cols, batch, false))
             return cudaErrorInvalidValue;
     }
     io.reads = in.p != nullptr;

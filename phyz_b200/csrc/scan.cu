@@ -287,7 +287,8 @@ __global__ void __launch_bounds__(NT, (Lane<T, BWD, OUT>::BLOCKS)) lane_kernel(c
             auto walk = [&](auto whole, auto marked) {
                 // values first, then the recurrence: a store between two loads
                 // would keep the second one waiting
-                float g[S], x[S], own[NIN == 4 ? S : 1], before[NIN == 4 ? S : 1];
+                float g[S], x[S];
+                [[maybe_unused]] float own[NIN == 4 ? S : 1], before[NIN == 4 ? S : 1];
 #pragma unroll
                 for (int v = 0; v < S; v++) {
                     const int e = (BWD ? S - 1 - v : v) * NT;
