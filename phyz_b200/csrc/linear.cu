@@ -260,23 +260,31 @@ __device__ __forceinline__ void planes_of(float x, __nv_bfloat16* p) {
     }
 }
 
-// rows x k values into 16-bit planes [outer][inner padded], in the order of src:
-// inner is the side that is contiguous there.
-template <class T>
-__global__ void __launch_bounds__(256) pack_kernel(const T* src, long long os, long long is, long long outer,
-                                                   long long inner, long long pitch, uint16_t* dst, long long plane) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= inner) return;
+// rows x k values into 16-bit planes [outer][pitch], in the order of src: inner is
+// the side that is contiguous there. A thread takes two neighbours, the threads go
+// through all pairs (I: an index type that holds their number).
+template <class T, class I>
+__global__ void __launch_bounds__(256) pack_kernel(const T* src, long long os, long long is, I outer, I inner, I pitch,
+                                                   uint32_t* dst, long long plane) {
+    const I pairs = pitch / 2, n = outer * pairs, step = (I)gridDim.x * 256;
 #pragma unroll 4
-    for (long long o = blockIdx.y; o < outer; o += gridDim.y) {
-        const T v = src[o * os + i * is];
+    for (I e = (I)blockIdx.x * 256 + threadIdx.x; e < n; e += step) {
+        const I o = e / pairs, i = (e - o * pairs) * 2;
+        const T* p = src + o * os + i * is;
+        T v[2] = {from_f32<T>(0.0f), from_f32<T>(0.0f)};
+        if (i < inner) v[0] = p[0];
+        if (i + 1 < inner) v[1] = p[is];
         if constexpr (sizeof(T) == 2) {
-            dst[o * pitch + i] = *reinterpret_cast<const uint16_t*>(&v);
+            dst[e] = *reinterpret_cast<const uint32_t*>(v);
         } else {
-            __nv_bfloat16 p[3];
-            planes_of(v, p);
+            __nv_bfloat16 x[3], y[3];
+            planes_of(v[0], x);
+            planes_of(v[1], y);
 #pragma unroll
-            for (int k = 0; k < 3; k++) dst[k * plane + o * pitch + i] = *reinterpret_cast<const uint16_t*>(&p[k]);
+            for (int k = 0; k < 3; k++) {
+                const __nv_bfloat162 w = __halves2bfloat162(x[k], y[k]);
+                dst[k * (plane / 2) + e] = *reinterpret_cast<const uint32_t*>(&w);
+            }
         }
     }
 }
@@ -306,12 +314,20 @@ struct Operand {
         }
         const bool mn = gemm_mn(mat, k);
         const long long outer = mn ? k : rows, inner = mn ? rows : k, os = mn ? mat.ks : mat.rs, is = mn ? 1 : mat.ks;
-        const long long across = (inner + 255) / 256, down = 8 * GEMM_SMS / across + 1;  // eight blocks to an SM
-        const dim3 grid((unsigned)across, (unsigned)(outer < down ? outer : down));
+        const long long n = outer * (pitch / 2), blocks = (n + 1023) / 1024;
+        const unsigned grid = (unsigned)(blocks < 16 * GEMM_SMS ? blocks : 16 * GEMM_SMS);
+        auto run = [&](auto* src) {
+            using T = std::remove_const_t<std::remove_pointer_t<decltype(src)>>;
+            if (n < 1ll << 31)
+                pack_kernel<T, uint32_t><<<grid, 256, 0, st>>>(src, os, is, (uint32_t)outer, (uint32_t)inner,
+                                                               (uint32_t)pitch, (uint32_t*)ws, plane);
+            else
+                pack_kernel<T, long long><<<grid, 256, 0, st>>>(src, os, is, outer, inner, pitch, (uint32_t*)ws, plane);
+        };
         if (dtype == PHYZB_DT_F32)
-            pack_kernel<<<grid, 256, 0, st>>>((const float*)mat.p, os, is, outer, inner, pitch, (uint16_t*)ws, plane);
+            run((const float*)mat.p);
         else
-            pack_kernel<<<grid, 256, 0, st>>>((const __half*)mat.p, os, is, outer, inner, pitch, (uint16_t*)ws, plane);
+            run((const __half*)mat.p);
         for (int p = 0; p < (dtype == PHYZB_DT_F32 ? 3 : 1); p++)
             out[p] = {ws + p * plane * 2, mn ? 1 : pitch, mn ? pitch : 1, 0};
         return cudaGetLastError();
@@ -542,16 +558,6 @@ constexpr int DZ_OUTER = 128;   // outer lines of a block, at most
 constexpr int DZ_INNER = 2048;  // inner values of a block, where it sums along them
 
 template <class T>
-__device__ __forceinline__ float dz_value(const DzArgs& a, long long o, long long i) {
-    float v = to_f32(((const T*)a.dy)[o * a.dy_o + i * a.dy_i]);
-    if (a.act != PHYZB_ACT_NONE) {
-        float z = to_f32(((const T*)a.pre)[o * a.pre_o + i * a.pre_i]), unused = 0.0f;
-        with_act(a.act, [&](auto kind) { act_grad_pair<decltype(kind)::value>(z, unused); });
-        v *= z;
-    }
-    return v;
-}
-template <class T>
 __device__ __forceinline__ void dz_store(const DzArgs& a, long long o, long long i, float v) {
     if (!a.dz) return;
     if (a.planes == 3) {
@@ -636,15 +642,25 @@ __global__ void __launch_bounds__(256) dz_features_kernel(const __grid_constant_
     __shared__ float sums[8];
     const long long i0 = (long long)blockIdx.x * DZ_INNER;
     for (long long o = blockIdx.y; o < a.outer; o += gridDim.y) {
-        float sum = 0.0f;
+        constexpr int N = DZ_INNER / 256;
+        float v[N], z[N], sum = 0.0f;
 #pragma unroll
-        for (int u = 0; u < DZ_INNER / 256; u++) {
+        for (int u = 0; u < N; u++) {
             const long long i = i0 + u * 256 + threadIdx.x;
-            if (i < a.inner) {
-                const float v = dz_value<T>(a, o, i);
-                dz_store<T>(a, o, i, v);
-                sum += v;
-            }
+            v[u] = i < a.inner ? to_f32(((const T*)a.dy)[o * a.dy_o + i * a.dy_i]) : 0.0f;
+            z[u] = i < a.inner && a.act != PHYZB_ACT_NONE ? to_f32(((const T*)a.pre)[o * a.pre_o + i * a.pre_i]) : 0.0f;
+        }
+        with_act(a.act, [&](auto kind) {
+#pragma unroll
+            for (int u = 0; u < N; u += 2) act_grad_pair<decltype(kind)::value>(z[u], z[u + 1]);
+        });
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            const long long i = i0 + u * 256 + threadIdx.x;
+            if (i >= a.inner) break;
+            v[u] *= z[u];
+            dz_store<T>(a, o, i, v[u]);
+            sum += v[u];
         }
         if (!a.part) continue;
 #pragma unroll
