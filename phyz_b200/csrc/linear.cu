@@ -542,7 +542,8 @@ cudaError_t forward(const phyzb_linear_args& a, char* ws, cudaStream_t st) {
 
 // ── backward ──────────────────────────────────────────────────────────────
 
-// dz = dy act'(pre) in dy's order (inner: its contiguous side), and the sums of
+// dz = dy act'(pre) in dy's order (inner: its contiguous side; the rows, where pre
+// has another order than dy), and the sums of
 // the unrounded dz over the rows: each block's part to part[block][n]. dz
 // [outer][pitch]: T, or three bf16 planes. dz or part may be null.
 struct DzArgs {
@@ -555,18 +556,20 @@ struct DzArgs {
     int lines;  // outer lines of a block
 };
 constexpr int DZ_OUTER = 128;   // outer lines of a block, at most
+constexpr int DZ_TURNED = 512;  // the same, where one operand is turned
 constexpr int DZ_INNER = 2048;  // inner values of a block, where it sums along them
 
+// (at: o * pitch + i)
 template <class T>
-__device__ __forceinline__ void dz_store(const DzArgs& a, long long o, long long i, float v) {
+__device__ __forceinline__ void dz_store(const DzArgs& a, long long at, float v) {
     if (!a.dz) return;
-    if (a.planes == 3) {
+    if (sizeof(T) == 4 && a.planes == 3) {
         __nv_bfloat16 p[3];
         planes_of(v, p);
 #pragma unroll
-        for (int k = 0; k < 3; k++) ((__nv_bfloat16*)a.dz)[k * a.plane + o * a.pitch + i] = p[k];
+        for (int k = 0; k < 3; k++) ((__nv_bfloat16*)a.dz)[k * a.plane + at] = p[k];
     } else {
-        ((T*)a.dz)[o * a.pitch + i] = from_f32<T>(v);
+        ((T*)a.dz)[at] = from_f32<T>(v);
     }
 }
 
@@ -615,7 +618,7 @@ __global__ void __launch_bounds__(256, 4) dz_rows_kernel(const __grid_constant__
             if (!a.dz) continue;
             if (sizeof(T) == 4 && a.planes == 3) {
 #pragma unroll
-                for (int e = 0; e < V; e++) dz_store<T>(a, o, i0 + e, v[e]);
+                for (int e = 0; e < V; e++) dz_store<T>(a, o * a.pitch + i0 + e, v[e]);
             } else if constexpr (V > 1) {
                 *reinterpret_cast<uint4*>((T*)a.dz + o * a.pitch + i0) = *reinterpret_cast<const uint4*>(out);
             } else {
@@ -644,22 +647,25 @@ __global__ void __launch_bounds__(256) dz_features_kernel(const __grid_constant_
     for (long long o = blockIdx.y; o < a.outer; o += gridDim.y) {
         constexpr int N = DZ_INNER / 256;
         float v[N], z[N], sum = 0.0f;
+        const long long left = a.inner - i0;
+        const int mine = (int)(left < DZ_INNER ? left : DZ_INNER) - (int)threadIdx.x;  // values from this thread's first on
+        const T* pd = (const T*)a.dy + o * a.dy_o + i0 + threadIdx.x;  // (contiguous: that is what makes it the inner side)
+        const T* pz = (const T*)a.pre + o * a.pre_o + (i0 + threadIdx.x) * a.pre_i;
 #pragma unroll
         for (int u = 0; u < N; u++) {
-            const long long i = i0 + u * 256 + threadIdx.x;
-            v[u] = i < a.inner ? to_f32(((const T*)a.dy)[o * a.dy_o + i * a.dy_i]) : 0.0f;
-            z[u] = i < a.inner && a.act != PHYZB_ACT_NONE ? to_f32(((const T*)a.pre)[o * a.pre_o + i * a.pre_i]) : 0.0f;
+            v[u] = u * 256 < mine ? to_f32(pd[u * 256]) : 0.0f;
+            z[u] = u * 256 < mine && a.act != PHYZB_ACT_NONE ? to_f32(pz[u * 256 * a.pre_i]) : 0.0f;
         }
         with_act(a.act, [&](auto kind) {
 #pragma unroll
             for (int u = 0; u < N; u += 2) act_grad_pair<decltype(kind)::value>(z[u], z[u + 1]);
         });
+        const long long at = o * a.pitch + i0 + threadIdx.x;
 #pragma unroll
         for (int u = 0; u < N; u++) {
-            const long long i = i0 + u * 256 + threadIdx.x;
-            if (i >= a.inner) break;
+            if (u * 256 >= mine) break;
             v[u] *= z[u];
-            dz_store<T>(a, o, i, v[u]);
+            dz_store<T>(a, at + u * 256, v[u]);
             sum += v[u];
         }
         if (!a.part) continue;
@@ -674,6 +680,68 @@ __global__ void __launch_bounds__(256) dz_features_kernel(const __grid_constant_
             a.part[blockIdx.x * a.outer + o] = s;
         }
         __syncthreads();
+    }
+}
+
+// dy and pre in different orders: inner = rows, a block takes DZ_TURNED rows of 32
+// features in tiles of 32 x 64. The operand whose features are contiguous (TDY: dy,
+// else pre) is read along them and turned in shared memory; the other is read, and
+// dz written, along the rows: 1320 x 34390 f16 with gelu, 272 MB, 132 us (2.1 TB/s, bound by instructions and the turn), where
+// reading one of the two against its order takes 233.
+template <class T, bool TDY>
+__global__ void __launch_bounds__(256) dz_mixed_kernel(const __grid_constant__ DzArgs a) {
+    constexpr int PITCH = 64 + 4 / sizeof(T);  // a tile's column goes to 32 different banks
+    __shared__ T tile[32 * PITCH];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const long long i0 = (long long)blockIdx.x * DZ_TURNED, i1 = i0 + DZ_TURNED < a.inner ? i0 + DZ_TURNED : a.inner;
+    const long long ti = TDY ? a.dy_i : a.pre_i, so = TDY ? a.pre_o : a.dy_o;
+    for (long long o0 = blockIdx.y * 32ll; o0 < a.outer; o0 += gridDim.y * 32ll) {
+        const int no = (int)(a.outer - o0 < 32 ? a.outer - o0 : 32);
+        const T* turned = (const T*)(TDY ? a.dy : a.pre) + o0 + lane + (i0 + warp) * ti;
+        const T* direct = (const T*)(TDY ? a.pre : a.dy) + (o0 + warp * 4) * so + i0 + lane;
+        long long at = (o0 + warp * 4) * a.pitch + i0 + lane;
+        float sum[4] = {};
+        for (long long ib = i0; ib < i1; ib += 64, turned += 64 * ti, direct += 64, at += 64) {
+            const int ni = (int)(i1 - ib < 64 ? i1 - ib : 64);
+            T t[8], d[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++)  // rows ib + 8 u + warp, features o0 + lane
+                t[u] = u * 8 + warp < ni && lane < no ? turned[u * 8 * ti] : from_f32<T>(0.0f);
+#pragma unroll
+            for (int u = 0; u < 8; u++)  // features o0 + 4 warp + u / 2, rows ib + 32 (u % 2) + lane
+                d[u] = u % 2 * 32 + lane < ni && warp * 4 + u / 2 < no ? direct[u / 2 * so + u % 2 * 32]
+                                                                       : from_f32<T>(0.0f);
+            __syncthreads();  // the last tile has been read
+#pragma unroll
+            for (int u = 0; u < 8; u++) tile[lane * PITCH + u * 8 + warp] = t[u];
+            __syncthreads();
+            float v[8], z[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float f = to_f32(tile[(warp * 4 + u / 2) * PITCH + u % 2 * 32 + lane]), g = to_f32(d[u]);
+                v[u] = TDY ? f : g;
+                z[u] = TDY ? g : f;
+            }
+            with_act(a.act, [&](auto kind) {
+#pragma unroll
+                for (int u = 0; u < 8; u += 2) act_grad_pair<decltype(kind)::value>(z[u], z[u + 1]);
+            });
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                if (u % 2 * 32 + lane >= ni || warp * 4 + u / 2 >= no) continue;
+                v[u] *= z[u];
+                dz_store<T>(a, at + u / 2 * a.pitch + u % 2 * 32, v[u]);
+                sum[u / 2] += v[u];
+            }
+        }
+        if (!a.part) continue;
+#pragma unroll
+        for (int f = 0; f < 4; f++) {
+#pragma unroll
+            for (int s = 16; s; s /= 2) sum[f] += __shfl_xor_sync(0xffffffffu, sum[f], s);
+            const long long o = o0 + warp * 4 + f;
+            if (lane == 0 && o < a.outer) a.part[blockIdx.x * a.outer + o] = sum[f];
+        }
     }
 }
 
@@ -698,6 +766,7 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float* part, lon
 struct Backward {
     bool features;            // dy has its rows contiguous: dz is [n][m padded]
     bool simt_dx, simt_dw;    // f32 on the FMA units
+    bool mixed, turn_dy;      // dy and pre in different orders; dy is the one by rows
     bool own_dz;              // dz is written (else dy is used as it is)
     int planes;               // of dz: 0 = T
     int lines;                // of a dz_rows_kernel block
@@ -716,7 +785,13 @@ struct Backward {
     }
     explicit Backward(const phyzb_linear_grad_args& a) {
         const bool f32 = a.dtype == PHYZB_DT_F32;
-        features = a.dy_stride[0] == 1 && a.dy_stride[1] != 1 && a.m > 1;
+        const auto by_features = [&](const int64_t (&s)[2]) { return s[0] == 1 && s[1] != 1; };
+        const auto by_rows = [&](const int64_t (&s)[2]) { return s[1] == 1 && s[0] != 1; };
+        features = by_features(a.dy_stride) && a.m > 1;
+        mixed = a.activation != PHYZB_ACT_NONE && a.m >= 32 && a.n >= 32;  // (a tile; fewer take one of the plain ways)
+        turn_dy = by_rows(a.dy_stride);
+        mixed = mixed && (turn_dy ? by_features(a.pre_stride) : features && by_rows(a.pre_stride));
+        features = features || mixed;
         outer = features ? a.n : a.m;
         inner = features ? a.m : a.n;
         pitch = up(inner, 8);
@@ -725,7 +800,8 @@ struct Backward {
         lines = DZ_OUTER;
         while (outer / lines >= 65535) lines *= 2;
         while (lines > 16 && (outer + lines - 1) / lines * ((inner + 255) / 256) < 4 * GEMM_SMS) lines /= 2;
-        blocks = features ? (inner + DZ_INNER - 1) / DZ_INNER : (outer + lines - 1) / lines;
+        const int along = mixed ? DZ_TURNED : DZ_INNER;
+        blocks = features ? (inner + along - 1) / along : (outer + lines - 1) / lines;
         // (both products of a layer have the same size: one way serves both)
         simt_dx = simt_dw = f32 && simt_is_faster((double)a.m, (double)a.n, (double)a.k);
         planes = f32 && !simt_dx ? 3 : 0;
@@ -787,7 +863,14 @@ cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st)
         auto wide = [&](const void* q, long long os, long long is) {
             return (uintptr_t)q % 16 == 0 && is == 1 && (p.outer == 1 || os % V == 0);
         };
-        if (p.features) {
+        if (p.mixed) {
+            const long long tiles = (p.outer + 31) / 32;
+            const dim3 grid((unsigned)p.blocks, (unsigned)(tiles < 65535 ? tiles : 65535));
+            if (p.turn_dy)
+                dz_mixed_kernel<T, true><<<grid, 256, 0, st>>>(d);
+            else
+                dz_mixed_kernel<T, false><<<grid, 256, 0, st>>>(d);
+        } else if (p.features) {
             dz_features_kernel<T><<<dim3((unsigned)p.blocks, (unsigned)(p.outer < 65535 ? p.outer : 65535)), 256, 0, st>>>(d);
         } else if (p.inner % V == 0 && wide(d.dy, d.dy_o, d.dy_i) &&
                    (a.activation == PHYZB_ACT_NONE || wide(d.pre, d.pre_o, d.pre_i))) {

@@ -189,10 +189,10 @@ def test_linear_rows_past_32_bit_offsets(dt):
     assert torch.equal(out, want)
 
 
-def check_backward(dt, m, k, n, act, bias, how, seed=0):
+def check_backward(dt, m, k, n, act, bias, how, seed=0, pre_how=None):
     g = gen(seed)
     x, w = layout(rnd(g, m, k, dt=dt), how), layout(rnd(g, n, k, dt=dt, std=1 / math.sqrt(k)), how)
-    pre, dy = layout(rnd(g, m, n, dt=dt), how), layout(rnd(g, m, n, dt=dt, std=0.5), how)
+    pre, dy = layout(rnd(g, m, n, dt=dt), pre_how or how), layout(rnd(g, m, n, dt=dt, std=0.5), how)
     dx, dw, db = nn.linear_backward(dy, x, w, pre if act != "none" else None, activation=act, bias=bias)
     z = pre.double().requires_grad_()
     slope = torch.autograd.grad(act64(z, act).sum(), z)[0] if act != "none" else torch.ones_like(z)
@@ -232,6 +232,15 @@ def test_linear_backward_activations(dt, act):
 def test_linear_backward_layouts(dt, how):
     check_backward(dt, 203, 136, 130, "gelu", True, how)
     check_backward(dt, 640, 64, 128, "silu", True, how)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("how,pre_how", [("rows", "features"), ("features", "rows"), ("padded", "features"),
+                                         ("features", "odd"), ("strided", "features")])
+@pytest.mark.parametrize("m,k,n", [(32, 64, 32), (33, 24, 95), (31, 40, 70), (2049, 96, 130), (4200, 8, 33)])
+def test_linear_backward_mixed_orders(dt, how, pre_how, m, k, n):
+    check_backward(dt, m, k, n, "gelu", True, how, pre_how=pre_how)
+    check_backward(dt, m, k, n, "tanh", False, how, pre_how=pre_how)
 
 
 @pytest.mark.parametrize("dt", TYPES)
