@@ -262,7 +262,8 @@ __device__ __forceinline__ void planes_of(float x, __nv_bfloat16* p) {
 
 // rows x k values into 16-bit planes [outer][pitch], in the order of src: inner is
 // the side that is contiguous there. A thread takes two neighbours, the threads go
-// through all pairs (I: an index type that holds their number).
+// through all pairs (I: an index type that holds their number). 120613 x 248 f32,
+// 300 MB, 69 us (4.4 TB/s).
 template <class T, class I>
 __global__ void __launch_bounds__(256) pack_kernel(const T* src, long long os, long long is, I outer, I inner, I pitch,
                                                    uint32_t* dst, long long plane) {
@@ -639,35 +640,73 @@ __global__ void __launch_bounds__(256, 4) dz_rows_kernel(const __grid_constant__
     }
 }
 
-// inner = rows: a block takes DZ_INNER of one feature's.
-template <class T>
-__global__ void __launch_bounds__(256) dz_features_kernel(const __grid_constant__ DzArgs a) {
+// inner = rows: a block takes DZ_INNER of one feature's, V neighbours a thread. The
+// same 403 MB as above in this order: 108 us (3.7 TB/s); one value at a time 259.
+template <class T, int V>
+__global__ void __launch_bounds__(256, 4) dz_features_kernel(const __grid_constant__ DzArgs a) {
     __shared__ float sums[8];
-    const long long i0 = (long long)blockIdx.x * DZ_INNER;
+    constexpr int GROUPS = DZ_INNER / 256 / V;
+    const long long i0 = (long long)blockIdx.x * DZ_INNER + threadIdx.x * V, left = a.inner - i0;
+    const int mine = (int)(left < DZ_INNER ? left : DZ_INNER);  // values from this thread's first on
     for (long long o = blockIdx.y; o < a.outer; o += gridDim.y) {
-        constexpr int N = DZ_INNER / 256;
-        float v[N], z[N], sum = 0.0f;
-        const long long left = a.inner - i0;
-        const int mine = (int)(left < DZ_INNER ? left : DZ_INNER) - (int)threadIdx.x;  // values from this thread's first on
-        const T* pd = (const T*)a.dy + o * a.dy_o + i0 + threadIdx.x;  // (contiguous: that is what makes it the inner side)
-        const T* pz = (const T*)a.pre + o * a.pre_o + (i0 + threadIdx.x) * a.pre_i;
-#pragma unroll
-        for (int u = 0; u < N; u++) {
-            v[u] = u * 256 < mine ? to_f32(pd[u * 256]) : 0.0f;
-            z[u] = u * 256 < mine && a.act != PHYZB_ACT_NONE ? to_f32(pz[u * 256 * a.pre_i]) : 0.0f;
-        }
+        float sum = 0.0f;
+        // (contiguous: that is what makes it the inner side)
+        const T *pd = (const T*)a.dy + o * a.dy_o + i0, *pz = (const T*)a.pre + o * a.pre_o + i0 * a.pre_i;
+        const long long at = o * a.pitch + i0;
         with_act(a.act, [&](auto kind) {
+            constexpr int ACT = decltype(kind)::value;
+            T d[DZ_INNER / 256], z[DZ_INNER / 256];
 #pragma unroll
-            for (int u = 0; u < N; u += 2) act_grad_pair<decltype(kind)::value>(z[u], z[u + 1]);
+            for (int g = 0; g < GROUPS; g++) {
+                const int i = g * 256 * V;
+                if (i >= mine) break;
+                if constexpr (V > 1) {
+                    *reinterpret_cast<uint4*>(d + g * V) = *reinterpret_cast<const uint4*>(pd + i);
+                    if (ACT != PHYZB_ACT_NONE) *reinterpret_cast<uint4*>(z + g * V) = *reinterpret_cast<const uint4*>(pz + i);
+                } else {
+                    d[g] = pd[i];
+                    if (ACT != PHYZB_ACT_NONE) z[g] = pz[i * a.pre_i];
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) {
+                if (g * 256 * V >= mine) break;
+                float v[V];
+#pragma unroll
+                for (int e = 0; e < V; e += 2) {
+                    const int f = V > 1 ? e + 1 : 0;
+                    v[e] = to_f32(d[g * V + e]);
+                    v[f] = to_f32(d[g * V + f]);
+                    if (ACT == PHYZB_ACT_NONE) continue;
+                    float p = to_f32(z[g * V + e]), q = to_f32(z[g * V + f]);
+                    act_grad_pair<ACT>(p, q);
+                    v[e] *= p;
+                    if (V > 1) v[f] *= q;
+                }
+#pragma unroll
+                for (int e = 0; e < V; e++) sum += v[e];
+                if (!a.dz) continue;
+                if constexpr (V == 1) {
+                    dz_store<T>(a, at + g * 256, v[0]);
+                } else if (sizeof(T) == 4 && a.planes == 3) {
+                    __nv_bfloat16 p[V][3], w[V];
+#pragma unroll
+                    for (int e = 0; e < V; e++) planes_of(v[e], p[e]);
+#pragma unroll
+                    for (int k = 0; k < 3; k++) {
+#pragma unroll
+                        for (int e = 0; e < V; e++) w[e] = p[e][k];
+                        *reinterpret_cast<uint2*>((__nv_bfloat16*)a.dz + k * a.plane + at + g * 256 * V) =
+                            *reinterpret_cast<const uint2*>(w);
+                    }
+                } else {
+                    T out[V];
+#pragma unroll
+                    for (int e = 0; e < V; e++) out[e] = from_f32<T>(v[e]);
+                    *reinterpret_cast<uint4*>((T*)a.dz + at + g * 256 * V) = *reinterpret_cast<const uint4*>(out);
+                }
+            }
         });
-        const long long at = o * a.pitch + i0 + threadIdx.x;
-#pragma unroll
-        for (int u = 0; u < N; u++) {
-            if (u * 256 >= mine) break;
-            v[u] *= z[u];
-            dz_store<T>(a, at + u * 256, v[u]);
-            sum += v[u];
-        }
         if (!a.part) continue;
 #pragma unroll
         for (int s = 16; s; s /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, s);
@@ -686,8 +725,8 @@ __global__ void __launch_bounds__(256) dz_features_kernel(const __grid_constant_
 // dy and pre in different orders: inner = rows, a block takes DZ_TURNED rows of 32
 // features in tiles of 32 x 64. The operand whose features are contiguous (TDY: dy,
 // else pre) is read along them and turned in shared memory; the other is read, and
-// dz written, along the rows: 1320 x 34390 f16 with gelu, 272 MB, 132 us (2.1 TB/s, bound by instructions and the turn), where
-// reading one of the two against its order takes 233.
+// dz written, along the rows: 1320 x 34390 f16 with gelu, 272 MB, 132 us (2.1 TB/s,
+// bound by instructions and the turn); 233 where one of the two is read against its order.
 template <class T, bool TDY>
 __global__ void __launch_bounds__(256) dz_mixed_kernel(const __grid_constant__ DzArgs a) {
     constexpr int PITCH = 64 + 4 / sizeof(T);  // a tile's column goes to 32 different banks
@@ -863,6 +902,8 @@ cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st)
         auto wide = [&](const void* q, long long os, long long is) {
             return (uintptr_t)q % 16 == 0 && is == 1 && (p.outer == 1 || os % V == 0);
         };
+        const bool neighbours = p.inner % V == 0 && wide(d.dy, d.dy_o, d.dy_i) &&
+                                (a.activation == PHYZB_ACT_NONE || wide(d.pre, d.pre_o, d.pre_i));
         if (p.mixed) {
             const long long tiles = (p.outer + 31) / 32;
             const dim3 grid((unsigned)p.blocks, (unsigned)(tiles < 65535 ? tiles : 65535));
@@ -871,9 +912,12 @@ cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st)
             else
                 dz_mixed_kernel<T, false><<<grid, 256, 0, st>>>(d);
         } else if (p.features) {
-            dz_features_kernel<T><<<dim3((unsigned)p.blocks, (unsigned)(p.outer < 65535 ? p.outer : 65535)), 256, 0, st>>>(d);
-        } else if (p.inner % V == 0 && wide(d.dy, d.dy_o, d.dy_i) &&
-                   (a.activation == PHYZB_ACT_NONE || wide(d.pre, d.pre_o, d.pre_i))) {
+            const dim3 grid((unsigned)p.blocks, (unsigned)(p.outer < 65535 ? p.outer : 65535));
+            if (neighbours)
+                dz_features_kernel<T, V><<<grid, 256, 0, st>>>(d);
+            else
+                dz_features_kernel<T, 1><<<grid, 256, 0, st>>>(d);
+        } else if (neighbours) {
             dz_rows_kernel<T, V><<<dim3((unsigned)((p.inner + 32 * V - 1) / (32 * V)), (unsigned)p.blocks), 256, 0, st>>>(d);
         } else {
             dz_rows_kernel<T, 1><<<dim3((unsigned)((p.inner + 31) / 32), (unsigned)p.blocks), 256, 0, st>>>(d);
