@@ -162,20 +162,18 @@ constexpr float LOG2E = 1.4426950408889634f;
 // within 2^-22 of the sigmoid near 1 and of e^z near 0
 __device__ __forceinline__ float sigmoid_f32(float z) { return sigmoid2_f32(z * LOG2E); }
 
-// Two of them by one reciprocal, 1 / (a b): exp and reciprocal share a unit of a
-// quarter of the lanes, and activations are what an epilogue takes longest over
-// (146 of 478 us at 262144 x 1024 values, before it had sixteen warps).
-// Arguments are cut at -60, where a sigmoid of 2^-60 stands for less, so that
-// a b stays finite.
-__device__ __forceinline__ void sigmoid2_pair(float x, float y, float& s, float& t) {
-    float e, f, r;
+// Two of them, s = 1 / (1 + e) with e = 2^-x, by one reciprocal, 1 / ((1 + e) (1 +
+// f)): exp and reciprocal share a unit of a quarter of the lanes, and activations are
+// what an epilogue takes longest over (146 of 478 us at 262144 x 1024 values, before
+// it had sixteen warps). Arguments are cut at -60, where a sigmoid of 2^-60 stands for
+// less, so that the product stays finite.
+__device__ __forceinline__ void sigmoid2_pair(float x, float y, float& e, float& f, float& s, float& t) {
+    float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(-x, 60.0f)));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(fminf(-y, 60.0f)));
-    e += 1.0f;
-    f += 1.0f;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e * f));
-    s = r * f;
-    t = r * e;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((1.0f + e) * (1.0f + f)));
+    s = r * (1.0f + f);
+    t = r * (1.0f + e);
 }
 
 // tanh z = 2 sigmoid(2z) - 1 = 2 s - 1; below 1/8, where that cancels, its series to
@@ -206,12 +204,14 @@ __device__ __forceinline__ void act_pair(float& x, float& y) {
         y = y > 0.0f || y != y ? y : 0.0f;
         return;
     }
-    float s, t;
-    sigmoid2_pair(act_inner<ACT>(x), act_inner<ACT>(y), s, t);
+    float e, f, s, t;
+    sigmoid2_pair(act_inner<ACT>(x), act_inner<ACT>(y), e, f, s, t);
     x = ACT == PHYZB_ACT_TANH ? (x == x ? tanh_of(x, s) : x) : x * s;
     y = ACT == PHYZB_ACT_TANH ? (y == y ? tanh_of(y, t) : y) : y * t;
 }
-// d act / dz of two values
+// d act / dz of two values. s (1 - s) is e s s: taken as a difference it is rounding
+// alone where s is near 1, and GELU multiplies it by z^3. It is exactly 0 where e is,
+// and the slope s then, whatever z is multiplied to (z^3 may be infinite).
 template <int ACT>
 __device__ __forceinline__ void act_grad_pair(float& x, float& y) {
     if (ACT == PHYZB_ACT_NONE) {
@@ -223,19 +223,16 @@ __device__ __forceinline__ void act_grad_pair(float& x, float& y) {
         y = y > 0.0f ? 1.0f : 0.0f;
         return;
     }
-    float s, t;
-    sigmoid2_pair(act_inner<ACT>(x), act_inner<ACT>(y), s, t);
-    auto slope = [](float z, float s) {
-        if (ACT == PHYZB_ACT_TANH) {
-            const float t = tanh_of(z, s);
-            return z == z ? fmaf(-t, t, 1.0f) : z;
-        }
-        const float q = fmaf(-s, s, s);  // s (1 - s)
-        if (ACT == PHYZB_ACT_SILU) return fmaf(q, z, s);
-        return fmaf(q, z * fmaf(z * z, 6.0f * GELU_C * GELU_K, 2.0f * GELU_C), s);
+    float e, f, s, t;
+    sigmoid2_pair(act_inner<ACT>(x), act_inner<ACT>(y), e, f, s, t);
+    auto slope = [](float z, float e, float s) {
+        const float q = e * s * s;
+        if (ACT == PHYZB_ACT_TANH) return z == z ? 4.0f * q : z;  // 1 - (2 s - 1)^2
+        if (ACT == PHYZB_ACT_SILU) return q == 0.0f ? s : fmaf(q, z, s);
+        return q == 0.0f ? s : fmaf(q, z * fmaf(z * z, 6.0f * GELU_C * GELU_K, 2.0f * GELU_C), s);
     };
-    x = slope(x, s);
-    y = slope(y, t);
+    x = slope(x, e, s);
+    y = slope(y, f, t);
 }
 
 }  // namespace pz
