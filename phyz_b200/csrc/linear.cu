@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(256, 4) dz_features_kernel(const __grid_consta
 #pragma unroll
             for (int g = 0; g < GROUPS; g++) {
                 const int i = g * 256 * V;
-                if (i >= mine) break;
+                if (i >= mine) continue;  // (leaving the loop here: f32 tanh 210 us instead of 193)
                 if constexpr (V > 1) {
                     *reinterpret_cast<uint4*>(d + g * V) = *reinterpret_cast<const uint4*>(pd + i);
                     if (ACT != PHYZB_ACT_NONE) *reinterpret_cast<uint4*>(z + g * V) = *reinterpret_cast<const uint4*>(pz + i);
@@ -670,7 +670,7 @@ __global__ void __launch_bounds__(256, 4) dz_features_kernel(const __grid_consta
             }
 #pragma unroll
             for (int g = 0; g < GROUPS; g++) {
-                if (g * 256 * V >= mine) break;
+                if (g * 256 * V >= mine) continue;
                 float v[V];
 #pragma unroll
                 for (int e = 0; e < V; e += 2) {

@@ -165,8 +165,8 @@ __device__ __forceinline__ float sigmoid_f32(float z) { return sigmoid2_f32(z * 
 // Two of them, s = 1 / (1 + e) with e = 2^-x, by one reciprocal, 1 / ((1 + e) (1 +
 // f)): exp and reciprocal share a unit of a quarter of the lanes, and activations are
 // what an epilogue takes longest over (146 of 478 us at 262144 x 1024 values, before
-// it had sixteen warps). Arguments are cut at -60, where a sigmoid of 2^-60 stands for
-// less, so that the product stays finite.
+// it had sixteen warps). Exponents are cut at 60, so that the product stays finite: a
+// sigmoid of less than 2^-60 is 2^-60. What multiplies it is bounded then (ACT_END).
 __device__ __forceinline__ void sigmoid2_pair(float x, float y, float& e, float& f, float& s, float& t) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(-x, 60.0f)));
@@ -195,6 +195,17 @@ __device__ __forceinline__ float act_inner(float z) {
     if (ACT == PHYZB_ACT_SILU) return z * LOG2E;
     return z * fmaf(z * z, 2.0f * LOG2E * GELU_C * GELU_K, 2.0f * LOG2E * GELU_C);
 }
+// |z| at which the exponent of SiLU's and GELU's sigmoid has come to the cut: from
+// there on the activation is 0 or z and its slope 0 or 1, to 2^-54.
+template <int ACT>
+constexpr float ACT_END = ACT == PHYZB_ACT_GELU ? 7.5f : 42.0f;
+
+// the larger one; a NaN stays a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
 // two values through the activation, in place (a NaN stays a NaN)
 template <int ACT>
 __device__ __forceinline__ void act_pair(float& x, float& y) {
@@ -206,12 +217,13 @@ __device__ __forceinline__ void act_pair(float& x, float& y) {
     }
     float e, f, s, t;
     sigmoid2_pair(act_inner<ACT>(x), act_inner<ACT>(y), e, f, s, t);
-    x = ACT == PHYZB_ACT_TANH ? (x == x ? tanh_of(x, s) : x) : x * s;
-    y = ACT == PHYZB_ACT_TANH ? (y == y ? tanh_of(y, t) : y) : y * t;
+    x = ACT == PHYZB_ACT_TANH ? (x == x ? tanh_of(x, s) : x) : max_nan(x, -ACT_END<ACT>) * s;
+    y = ACT == PHYZB_ACT_TANH ? (y == y ? tanh_of(y, t) : y) : max_nan(y, -ACT_END<ACT>) * t;
 }
 // d act / dz of two values. s (1 - s) is e s s: taken as a difference it is rounding
-// alone where s is near 1, and GELU multiplies it by z^3. It is exactly 0 where e is,
-// and the slope s then, whatever z is multiplied to (z^3 may be infinite).
+// alone where s is near 1, and GELU multiplies it by z^3, which is bounded by ACT_END
+// (a NaN is not over it, and stays one). tanh's slope is even in z: of |z| its e falls
+// to 0 and meets no cut.
 template <int ACT>
 __device__ __forceinline__ void act_grad_pair(float& x, float& y) {
     if (ACT == PHYZB_ACT_NONE) {
@@ -224,12 +236,13 @@ __device__ __forceinline__ void act_grad_pair(float& x, float& y) {
         return;
     }
     float e, f, s, t;
-    sigmoid2_pair(act_inner<ACT>(x), act_inner<ACT>(y), e, f, s, t);
+    auto inner = [](float z) { return act_inner<ACT>(ACT == PHYZB_ACT_TANH ? fabsf(z) : z); };
+    sigmoid2_pair(inner(x), inner(y), e, f, s, t);
     auto slope = [](float z, float e, float s) {
         const float q = e * s * s;
         if (ACT == PHYZB_ACT_TANH) return z == z ? 4.0f * q : z;  // 1 - (2 s - 1)^2
-        if (ACT == PHYZB_ACT_SILU) return q == 0.0f ? s : fmaf(q, z, s);
-        return q == 0.0f ? s : fmaf(q, z * fmaf(z * z, 6.0f * GELU_C * GELU_K, 2.0f * GELU_C), s);
+        const float w = ACT == PHYZB_ACT_SILU ? z : z * fmaf(z * z, 6.0f * GELU_C * GELU_K, 2.0f * GELU_C);
+        return fabsf(z) >= ACT_END<ACT> ? __saturatef(z) : fmaf(q, w, s);
     };
     x = slope(x, e, s);
     y = slope(y, f, t);

@@ -76,3 +76,44 @@ def check_slopes(dt, act, dy_how, pre_how, m, n, sizes):
 def test_slopes_of_large_values(dt, act, dy_how, pre_how):
     check_slopes(dt, act, dy_how, pre_how, 600, 64, LARGE)
     check_slopes(dt, act, dy_how, pre_how, 4096, 512, LARGE)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dy_how,pre_how", ORDERS)
+def test_slopes_of_large_negative_values(dt, act, dy_how, pre_how):
+    sizes = [-v for v in LARGE] + LARGE[::3]
+    check_slopes(dt, act, dy_how, pre_how, 600, 64, sizes)
+    check_slopes(dt, act, dy_how, pre_how, 4096, 512, sizes)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m,n", [(1, 40), (7, 64), (600, 64), (4096, 512)])
+@pytest.mark.parametrize("how", ["rows", "features"])
+def test_activations_of_large_values(dt, act, m, n, how):
+    """z s is off by some roundings of itself (s by 2^-23 |z| of itself where it is small: then z^2 s is under 1), and
+    nothing of z is left where s has vanished."""
+    x = layout(outliers(dt, LARGE + [-v for v in LARGE], m, n), how)
+    y = nn.linear(x, torch.eye(n, device="cuda", dtype=dt), activation=act)
+    want = act64(x.double(), act)
+    err = 16 * 2.0 ** -23 * (1 + want.abs())
+    assert torch.isfinite(y.double()).all()
+    assert ((y.double() - want).abs() <= err + U[dt] * (want.abs() + err) + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("act", ["tanh", "silu", "gelu"])
+def test_slopes_of_infinities_and_nan(dt, act):
+    """A layer of one feature, so that no product mixes elements: the slope's limits at the infinities, and a NaN stays
+    one, alone."""
+    pre = rnd(4, 256, 1, dt=dt)
+    dy, one = rnd(5, 256, 1, dt=dt), torch.ones(1, 1, device="cuda", dtype=dt)
+    clean = nn.linear_backward(dy, pre, one, pre, activation=act)[0]
+    pre[3], pre[64], pre[65] = float("nan"), float("inf"), float("-inf")
+    dx = nn.linear_backward(dy, pre, one, pre, activation=act)[0]
+    assert dx[3].isnan() and not dx[65].any()
+    assert dx[64].abs() <= 2.0 ** -20 if act == "tanh" else (dx[64] - dy[64]).abs() <= dy[64].abs() * 4 * U[dt]
+    keep = torch.ones(256, dtype=torch.bool, device="cuda")
+    keep[[3, 64, 65]] = False
+    assert torch.equal(dx[keep], clean[keep])
