@@ -150,23 +150,38 @@ __device__ __forceinline__ void with_act(int act, F f) {
     }
 }
 
-// sigmoid(z / log2 e) by the approximate exp2 and reciprocal (2 ulp and 1 ulp
-// each); exactly 0 and 1 at the ends.
-__device__ __forceinline__ float sigmoid2_f32(float z) {
-    float e, a;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-z));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.0f + e));
-    return a;
-}
 constexpr float LOG2E = 1.4426950408889634f;
-// within 2^-22 of the sigmoid near 1 and of e^z near 0
-__device__ __forceinline__ float sigmoid_f32(float z) { return sigmoid2_f32(z * LOG2E); }
 
-// Two of them, s = 1 / (1 + e) with e = 2^-x, by one reciprocal, 1 / ((1 + e) (1 +
-// f)): exp and reciprocal share a unit of a quarter of the lanes, and activations are
-// what an epilogue takes longest over (146 of 478 us at 262144 x 1024 values, before
-// it had sixteen warps). Exponents are cut at 60, so that the product stays finite: a
-// sigmoid of less than 2^-60 is 2^-60. What multiplies it is bounded then (ACT_END).
+// the larger and the smaller one; a NaN stays a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float m;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+
+// a = sigmoid(z) = 1 / (1 + e), e = 2^(-z log2 e), by the approximate exp2 and
+// reciprocal (2 ulp and 1 ulp each), and shut = 1 - a = e a: as a difference from the
+// rounded a it would be 6 % off at z = 16 and 0 from 17.4 on. e is cut at 2^120, so
+// that e a stays 1 there: a is then 2^-120 instead of less, which no f32 sum of
+// ordinary values shows. Exactly 1 and 0 for z from 88 on.
+__device__ __forceinline__ void gate_f32(float z, float& a, float& shut) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(min_nan(z * -LOG2E, 120.0f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.0f + e));
+    shut = e * a;
+}
+
+// sigmoid(z / log2 e) of two values, s = 1 / (1 + e) with e = 2^-z, by one
+// reciprocal, 1 / ((1 + e) (1 + f)): exp and reciprocal share a unit of a quarter of
+// the lanes, and activations are what an epilogue takes longest over (146 of 478 us at
+// 262144 x 1024 values, before it had sixteen warps). Exponents are cut at 60, so that
+// the product stays finite: a sigmoid of less than 2^-60 is 2^-60. What multiplies it
+// is bounded then (ACT_END).
 __device__ __forceinline__ void sigmoid2_pair(float x, float y, float& e, float& f, float& s, float& t) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(-x, 60.0f)));
@@ -200,12 +215,6 @@ __device__ __forceinline__ float act_inner(float z) {
 template <int ACT>
 constexpr float ACT_END = ACT == PHYZB_ACT_GELU ? 7.5f : 42.0f;
 
-// the larger one; a NaN stays a NaN
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float m;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
-    return m;
-}
 // two values through the activation, in place (a NaN stays a NaN)
 template <int ACT>
 __device__ __forceinline__ void act_pair(float& x, float& y) {

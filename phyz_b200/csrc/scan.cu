@@ -72,8 +72,9 @@ __global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ phyzb
     for (int v = 0; v < V; v++) h[v] = hp ? hp[v * a.h0_stride[1]] : 0.0f;
 #pragma unroll
     for (int v = 0; v < V; v++) {
-        const float s = sigmoid_f32(to_f32(g[v]));
-        const float u = (1.0f - s) * to_f32(x[v]);
+        float s, shut;
+        gate_f32(to_f32(g[v]), s, shut);
+        const float u = shut * to_f32(x[v]);
         h[v] = rp && rp[v * a.reset_stride[2]] ? u : fmaf(s, h[v], u);
         y[v] = from_f32<T>(h[v]);
     }
@@ -288,20 +289,22 @@ __global__ void __launch_bounds__(NT, (Lane<T, BWD, OUT>::BLOCKS)) lane_kernel(c
                 // values first, then the recurrence: a store between two loads
                 // would keep the second one waiting
                 float g[S], x[S];
-                [[maybe_unused]] float own[NIN == 4 ? S : 1], before[NIN == 4 ? S : 1];
+                [[maybe_unused]] float shut[NIN == 4 ? S : 1], slope[NIN == 4 ? S : 1];  // of dgate over dx
 #pragma unroll
                 for (int v = 0; v < S; v++) {
                     const int e = (BWD ? S - 1 - v : v) * NT;
-                    g[v] = sigmoid_f32(to_f32(in[e]));
+                    float q;
+                    gate_f32(to_f32(in[e]), g[v], q);
                     x[v] = to_f32(in[BOX + e]);
-                    if (!BWD) x[v] *= 1.0f - g[v];
+                    if (!BWD) x[v] *= q;
                     if constexpr (NIN == 4) {
-                        own[v] = to_f32(in[2 * BOX + e]);
-                        before[v] = to_f32(in[3 * BOX + e]);
+                        float before = to_f32(in[3 * BOX + e]);
+                        if (v == S - 1 && t == 0) before = h0;
+                        if (decltype(marked)::value && drops[RESET ? v : 0]) before = 0.0f;
+                        shut[v] = q;
+                        slope[v] = g[v] * (before - to_f32(in[2 * BOX + e]));
                     }
                 }
-                if constexpr (NIN == 4)
-                    if (t == 0) before[S - 1] = h0;
 #pragma unroll
                 for (int v = 0; v < S; v++) {
                     const int row = BWD ? S - 1 - v : v;
@@ -317,9 +320,9 @@ __global__ void __launch_bounds__(NT, (Lane<T, BWD, OUT>::BLOCKS)) lane_kernel(c
                         h = drop ? x[v] : fmaf(g[v], h, x[v]);
                         out[row * NT] = from_f32<T>(h);
                     } else {
-                        const float d = h + x[v], dx = (1.0f - g[v]) * d;
+                        const float d = h + x[v], dx = shut[v] * d;
                         out[row * NT] = from_f32<T>(dx);
-                        out[BOX + row * NT] = from_f32<T>(dx * g[v] * ((drop ? 0.0f : before[v]) - own[v]));
+                        out[BOX + row * NT] = from_f32<T>(dx * slope[v]);
                         h = drop ? 0.0f : g[v] * d;
                     }
                 }
@@ -408,17 +411,17 @@ __global__ void __launch_bounds__(NT) loose_kernel(const __grid_constant__ Side 
     const float h0 = BWD && OUT && s.h0 ? s.h0[b * s.h0_b + c * s.h0_c] : 0.0f;
     float A = 1.0f, h = start_of<OUT>(s, b, c, sp);
     for (long long p = 0; p < n; p += L) {
-        float g[L], x[L], own[NIN == 4 ? L : 1], before[NIN == 4 ? L : 1];
+        float g[L], x[L], shut[L], slope[NIN == 4 ? L : 1];  // of dgate over dx
         bool drop[L];
 #pragma unroll
         for (int u = 0; u < L; u++) {
-            g[u] = sigmoid_f32(to_f32(raw[0][u]));
+            gate_f32(to_f32(raw[0][u]), g[u], shut[u]);
             x[u] = to_f32(raw[1][u]);
-            if (!BWD) x[u] *= 1.0f - g[u];
+            if (!BWD) x[u] *= shut[u];
             drop[u] = RESET && drops[u];
             if constexpr (NIN == 4) {
-                own[u] = to_f32(raw[2][u]);
-                before[u] = drop[u] ? 0.0f : t0 == 0 && p + u == n - 1 ? h0 : to_f32(raw[3][u]);
+                const float before = drop[u] ? 0.0f : t0 == 0 && p + u == n - 1 ? h0 : to_f32(raw[3][u]);
+                slope[u] = g[u] * (before - to_f32(raw[2][u]));
             }
         }
         load(p + L);
@@ -435,9 +438,9 @@ __global__ void __launch_bounds__(NT) loose_kernel(const __grid_constant__ Side 
                 *out[0] = from_f32<T>(h);
                 out[0] += ostep[0];
             } else {
-                const float d = h + x[u], dx = (1.0f - g[u]) * d;
+                const float d = h + x[u], dx = shut[u] * d;
                 *out[0] = from_f32<T>(dx);
-                *out[1] = from_f32<T>(dx * g[u] * (before[u] - own[u]));
+                *out[1] = from_f32<T>(dx * slope[u]);
                 out[0] += ostep[0];
                 out[1] += ostep[1];
                 h = drop[u] ? 0.0f : g[u] * d;

@@ -117,3 +117,86 @@ def test_slopes_of_infinities_and_nan(dt, act):
     keep = torch.ones(256, dtype=torch.bool, device="cuda")
     keep[[3, 64, 65]] = False
     assert torch.equal(dx[keep], clean[keep])
+
+
+# ── gated scan: gates that are nearly shut ────────────────────────────────
+
+# 1 - a is e a with e = 2^-x, x the gate over log 2: x is off by some 2^-24 of itself (29 at a gate of 20), the
+# exponential, the reciprocal and the products by a few roundings, so 1 - a is within 32 roundings of itself however
+# small it is. Every sum here is of values of one sign, so what t steps add is t roundings more, and the relative
+# tolerance holds for each element by itself.
+def near_each(got, want, t, dt):
+    tol = (64 + 4 * t) * 2.0 ** -23 + U[dt]
+    small = 2.0 ** -25 if dt is torch.float16 else 2.0 ** -126
+    assert ((got.double() - want).abs() <= tol * want.abs() + small).all(), \
+        f"relative error {float(((got.double() - want) / want).abs().max()):.3g}"
+
+
+SHUT = [(1, 1, 64), (3, 1, 7), (3, 40, 64), (5, 40, 7), (1, 3000, 64), (1, 3000, 3)]  # one step, tiles, plain, both cut
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,t,c", SHUT)
+@pytest.mark.parametrize("resets", [False, True])
+def test_scan_inputs_through_shut_gates(dt, b, t, c, resets):
+    gate = (8 + 12 * torch.rand(b, t, c, device="cuda", generator=torch.Generator(device="cuda").manual_seed(6))).to(dt)
+    x = (rnd(7, b, t, c).abs() + 0.5).to(dt)
+    reset = (torch.arange(t, device="cuda") % 16 == 5).to(torch.uint8).expand(b, t) if resets else None
+    h, last = nn.gated_scan(x, gate, None, reset)
+    state, want = torch.zeros(b, c, device="cuda", dtype=torch.float64), torch.empty_like(x, dtype=torch.float64)
+    a, shut = torch.sigmoid(gate.double()), torch.sigmoid(-gate.double())
+    for k in range(t):
+        if resets and k % 16 == 5:
+            state = torch.zeros_like(state)
+        state = a[:, k] * state + shut[:, k] * x[:, k].double()
+        want[:, k] = state
+    near_each(h, want, t, dt)
+    near_each(last, state, t, torch.float32)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("b,t,c", SHUT)
+@pytest.mark.parametrize("resets", [False, True])
+def test_scan_gradients_through_shut_gates(dt, b, t, c, resets):
+    gate = (8 + 12 * torch.rand(b, t, c, device="cuda", generator=torch.Generator(device="cuda").manual_seed(8))).to(dt)
+    x, h, dh = ((rnd(s, b, t, c).abs() + 0.5).to(dt) for s in (9, 10, 11))
+    x = -x  # (so that h - x does not cancel either)
+    h0, dl = rnd(12, b, c).abs() + 0.5, rnd(13, b, c).abs()
+    reset = (torch.arange(t, device="cuda") % 16 == 5).to(torch.uint8).expand(b, t) if resets else None
+    dx, dg, dh0 = nn.gated_scan_backward(dh, x, gate, h, h0, reset, dl)
+    a, shut = torch.sigmoid(gate.double()), torch.sigmoid(-gate.double())
+    before = torch.cat([h0.double()[:, None], h.double()[:, :-1]], 1)
+    want_x, want_g, d = torch.empty_like(a), torch.empty_like(a), dl.double()
+    for k in range(t - 1, -1, -1):
+        drop = resets and k % 16 == 5
+        d = d + dh[:, k].double()
+        want_x[:, k] = shut[:, k] * d
+        want_g[:, k] = a[:, k] * shut[:, k] * ((0 if drop else before[:, k]) - x[:, k].double()) * d
+        d = torch.zeros_like(d) if drop else a[:, k] * d
+    near_each(dx, want_x, t, dt)
+    near_each(dg, want_g, t, dt)
+    near_each(dh0, d, t, torch.float32)
+
+
+@pytest.mark.parametrize("t,c", [(1, 64), (1, 7), (40, 64), (40, 7)])
+def test_scan_of_extreme_gates(t, c):
+    """Open and shut to the end of the range, and a NaN, which stays in its chain and is not taken for a gate."""
+    x, h0 = rnd(14, 4, t, c), rnd(15, 4, c)
+    for value in (200.0, 3e38, float("inf")):
+        h, last = nn.gated_scan(x, torch.full_like(x, value), h0)
+        assert torch.equal(h, h0[:, None].expand_as(h)) and torch.equal(last, h0)
+        h, last = nn.gated_scan(x, torch.full_like(x, -value), h0)
+        assert torch.equal(h, x) and torch.equal(last, x[:, -1])
+        dx, dg, dh0 = nn.gated_scan_backward(x, x, torch.full_like(x, -value), x, h0)
+        assert torch.equal(dx, x) and dg.abs().max() <= 2.0 ** -80 and dh0.abs().max() <= 2.0 ** -80
+    gate = torch.zeros_like(x)
+    want, _ = nn.gated_scan(x, gate, h0)
+    gate[1, 0, 2] = float("nan")
+    reset = torch.zeros(4, t, dtype=torch.uint8, device="cuda")
+    reset[:, 0] = 1  # (the state is dropped, the gate still weighs x)
+    h, _ = nn.gated_scan(x, gate, h0)
+    hr, _ = nn.gated_scan(x, gate, h0, reset)
+    dx, _, _ = nn.gated_scan_backward(x, x, gate, x, h0, reset)
+    assert h[1, :, 2].isnan().all() and hr[1, :, 2].isnan().all() and dx[1, 0, 2].isnan()
+    h[1, :, 2] = want[1, :, 2]
+    assert torch.equal(h, want)
