@@ -387,6 +387,9 @@ int simt_splits(long long rows, long long cols, long long k) {
     return s < 2 ? 1 : (int)s;
 }
 
+// Whether a result [i][j] is contiguous in i: lanes then run along i, else along j.
+bool along_i_of(const int64_t* stride) { return stride[1] != 1 && stride[0] == 1; }
+
 template <class Epi>
 cudaError_t simt_multiply(const SimtOperand& a, const SimtOperand& b, long long rows, long long cols, long long k,
                           int splits, bool along_i, char* part, const Epi& epi, cudaStream_t st) {
@@ -526,10 +529,9 @@ cudaError_t forward(const phyzb_linear_args& a, char* ws, cudaStream_t st) {
     if constexpr (sizeof(T) == 4) {
         if (way == SIMT) {
             // (i = rows here; the epilogue takes either order)
-            const bool along_i = a.y_stride[1] != 1 && a.y_stride[0] == 1;
             return simt_multiply({(const float*)a.x, a.x_stride[0], a.x_stride[1]},
                                  {(const float*)a.w, a.w_stride[0], a.w_stride[1]}, a.m, a.n, a.k,
-                                 simt_splits(a.m, a.n, a.k), along_i, ws, epilogue<T>(a, true), st);
+                                 simt_splits(a.m, a.n, a.k), along_i_of(a.y_stride), ws, epilogue<T>(a, true), st);
         }
     }
     const Forward f(a);
@@ -942,7 +944,7 @@ cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st)
         if constexpr (sizeof(T) == 4) {
             if (p.simt_dx) {
                 e = simt_multiply({(const float*)zp, zr, zn}, {(const float*)a.w, a.w_stride[1], a.w_stride[0]}, a.m, a.k,
-                                  a.n, p.split_dx, rf, part,
+                                  a.n, p.split_dx, along_i_of(a.dx_stride), part,
                                   store_epi<T>({(T*)a.dx, a.dx_stride[0], a.dx_stride[1]}, a.m), st);
             }
         }
@@ -960,7 +962,7 @@ cudaError_t backward(const phyzb_linear_grad_args& a, char* ws, cudaStream_t st)
         if constexpr (sizeof(T) == 4) {
             if (p.simt_dw)
                 return simt_multiply({(const float*)zp, zn, zr}, {(const float*)a.x, a.x_stride[1], a.x_stride[0]}, a.n,
-                                     a.k, a.m, p.split_dw, false, part,
+                                     a.k, a.m, p.split_dw, along_i_of(a.dw_stride), part,
                                      store_epi<T>(dw, a.n), st);
         }
         GemmMat x[3];

@@ -200,3 +200,47 @@ def test_scan_of_extreme_gates(t, c):
     assert h[1, :, 2].isnan().all() and hr[1, :, 2].isnan().all() and dx[1, 0, 2].isnan()
     h[1, :, 2] = want[1, :, 2]
     assert torch.equal(h, want)
+
+
+# ── small f32 layers: the order of a gradient's result ────────────────────
+
+def best_us(f):
+    """Device time of one of ten calls captured in a graph, the best of twelve replays."""
+    f()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(10):
+            f()
+    best = 1e9
+    for _ in range(12):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        graph.replay()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b) * 100)
+    return best
+
+
+@pytest.mark.parametrize("order", ["rows", "features"])
+def test_small_gradient_is_written_along_its_order(order):
+    """dx = dy w of an 8 to 128 layer's mirror image is the product that its forward makes, and takes as long (within
+    half; stored against its order it took 28 us where it takes 13)."""
+    x, wide, w = layout(rnd(20, 65536, 8), order), layout(rnd(21, 65536, 128), order), rnd(22, 128, 8)
+    narrow = w.t().contiguous()  # the layer 128 -> 8
+    forward = best_us(lambda: nn.linear(x, w))
+    dx = best_us(lambda: nn.linear_backward(x, wide, narrow, bias=False, need_dw=False))
+    assert dx <= 1.5 * forward, (dx, forward)
+
+
+@pytest.mark.parametrize("m,k,n", [(40, 30, 70), (3000, 30, 64), (65536, 24, 12)])
+def test_small_gradients_in_either_order(m, k, n):
+    """dw and dx where the caller keeps them the other way round: the same values."""
+    x, w, dy = rnd(23, m, k), rnd(24, n, k), rnd(25, m, n)
+    dx, dw, _ = nn.linear_backward(dy, x, w, bias=False)
+    tx, tw = torch.full((k, m), float("nan"), device="cuda"), torch.full((k, n), float("nan"), device="cuda")
+    args = nn._LINEAR_GRAD.pack(0, 0, 0, m, k, n, dy.data_ptr(), n, 1, 0, 0, 0, x.data_ptr(), k, 1, w.data_ptr(), k, 1,
+                                tx.data_ptr(), 1, m, tw.data_ptr(), 1, n, 0)
+    nn._linear_grad(args, 0)
+    assert torch.equal(tx.t(), dx) and torch.equal(tw.t(), dw)
