@@ -296,6 +296,8 @@ int phyzb_nn_status(int32_t device) {
         PZ_TRY(check_device(device));
         DeviceGuard g(device);
         unsigned int linear = 0, scan = 0, muon = 0;
+        // (the copies below are ordered after the default stream's work, not after a non-blocking stream's)
+        PZ_CUDA(cudaDeviceSynchronize());
         PZ_CUDA(pz::linear_faults(&linear));
         PZ_CUDA(pz::scan_faults(&scan));
         PZ_CUDA(pz::muon_faults(&muon));

@@ -244,3 +244,23 @@ def test_small_gradients_in_either_order(m, k, n):
                                 tx.data_ptr(), 1, m, tw.data_ptr(), 1, n, 0)
     nn._linear_grad(args, 0)
     assert torch.equal(tx.t(), dx) and torch.equal(tw.t(), dw)
+
+
+# ── waits ─────────────────────────────────────────────────────────────────
+
+def test_status_waits_for_every_stream():
+    """What it reports is of all calls so far: work on a side stream (which does not wait for the default one, nor the
+    other way round) has finished when it returns."""
+    x, w = rnd(26, 512, 64, dt=torch.bfloat16), rnd(27, 64, 64, dt=torch.bfloat16)
+    nn.linear(x, w)
+    nn.status()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # a tenth of a second
+        y = nn.linear(x, w)
+        done = side.record_event()
+    assert not done.query()
+    nn.status()
+    assert done.query()
+    assert torch.equal(y, nn.linear(x, w))
