@@ -15,18 +15,20 @@ struct SimtOperand {
 // 256 threads compute a 128 x 64 tile, 8 x 4 values each (two groups of four
 // rows 64 apart, four columns), from stages of 16 k in shared memory; the next
 // stage is loaded into registers while the current one is multiplied. blockIdx
-// = (tiles of i, tiles of j, split of the k range). Bound by instructions: 65536 x
+// = (tiles of i, tiles of j, split of the k range), or with wide (tiles of j, of i,
+// split): a grid's second side ends at 65535. Bound by instructions: 65536 x
 // 30 x 64 with bias, tanh and pre-activations, 41 MB, 18.5 us. ALONG_I: D is contiguous in
 // i; lanes then run along i, and the epilogue gets four values along it.
 // Epi: each(f) calls f(kind) once, and f void four(kind, int split, long long i, long long j, const float* v, int n,
 // bool along_i)
 template <bool ALONG_I, class Epi>
 __global__ void __launch_bounds__(256) simt_gemm_kernel(SimtOperand A, SimtOperand B, long long M, long long N,
-                                                        long long K, long long per, Epi epi) {
+                                                        long long K, long long per, bool wide, Epi epi) {
     constexpr int TM = 128, TN = 64, TK = 16;
     __shared__ __align__(16) float As[TK][TM + 4];
     __shared__ __align__(16) float Bs[TK][TN + 4];
-    const long long i0 = (long long)blockIdx.x * TM, j0 = (long long)blockIdx.y * TN;
+    const long long i0 = (long long)(wide ? blockIdx.y : blockIdx.x) * TM;
+    const long long j0 = (long long)(wide ? blockIdx.x : blockIdx.y) * TN;
     const long long k0 = blockIdx.z * per, k1 = k0 + per < K ? k0 + per : K;
     const int t = threadIdx.x, tj = ALONG_I ? t / 16 : t % 16, ti = ALONG_I ? t % 16 : t / 16;
     // consecutive threads walk the operand's unit stride: a thread's elements of a
@@ -107,12 +109,14 @@ __global__ void __launch_bounds__(256) simt_gemm_kernel(SimtOperand A, SimtOpera
 template <class Epi>
 cudaError_t simt_gemm(const SimtOperand& A, const SimtOperand& B, long long M, long long N, long long K, int splits,
                       bool along_i, const Epi& epi, cudaStream_t s) {
-    const dim3 grid((unsigned)((M + 127) / 128), (unsigned)((N + 63) / 64), (unsigned)splits);
+    const unsigned ti = (unsigned)((M + 127) / 128), tj = (unsigned)((N + 63) / 64);
+    const bool wide = tj > 65535;
+    const dim3 grid(wide ? tj : ti, wide ? ti : tj, (unsigned)splits);
     const long long per = (K + splits - 1) / splits;
     if (along_i)
-        simt_gemm_kernel<true><<<grid, 256, 0, s>>>(A, B, M, N, K, per, epi);
+        simt_gemm_kernel<true><<<grid, 256, 0, s>>>(A, B, M, N, K, per, wide, epi);
     else
-        simt_gemm_kernel<false><<<grid, 256, 0, s>>>(A, B, M, N, K, per, epi);
+        simt_gemm_kernel<false><<<grid, 256, 0, s>>>(A, B, M, N, K, per, wide, epi);
     return cudaGetLastError();
 }
 

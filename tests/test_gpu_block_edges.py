@@ -264,3 +264,22 @@ def test_status_waits_for_every_stream():
     nn.status()
     assert done.query()
     assert torch.equal(y, nn.linear(x, w))
+
+
+# ── more features than a launch has blocks along its second side ──────────
+
+@pytest.mark.parametrize("order", ["rows", "features"])
+def test_small_layers_of_millions_of_features(order):
+    """Small whole numbers, which f32 sums hold exactly in every order."""
+    n = 4_200_000
+    x = layout((torch.arange(9, device="cuda") + 1.0)[:, None], order)
+    w = (torch.arange(n, device="cuda") % 97).float()[:, None]
+    y = nn.linear(x, w)
+    assert torch.equal(y, x * w.t())
+    few = nn.linear(x[:4], w.expand(n, 2)[:, ::2])
+    assert torch.equal(few, y[:4])
+    # as the inputs' side: dx [9][n], dw [3][n]
+    dy, v = layout(x.repeat(1, 3), order), torch.ones(3, 1, device="cuda") * w.t()
+    dx, dw, _ = nn.linear_backward(dy, y, v, bias=False)
+    assert torch.equal(dx, 3 * x * w.t())
+    assert torch.equal(dw, (x * x).sum() * w.t().expand(3, n))
