@@ -82,7 +82,7 @@ struct GemmArgs {
     int ti, tj;           // tiles of ROWS and of BN
     int kblocks;          // of 64 in all
     int splits;           // ranges of k; a unit is (tile, split, batch)
-    int per;              // k blocks of a split
+    int per;              // k blocks of a split, one at least
     int units;
     int symmetric;        // D = D^T: tiles wholly above the diagonal blocks are left out
     uint32_t idesc;       // instruction descriptor (types, orders, shape)
@@ -475,7 +475,6 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
                 }
             };
             const long long i = q.row0 + own + lane;
-            const bool any = q.k0 < q.k1;
             float held[S::FLUSH ? S::CHUNKS : 1][32];  // FLUSH: the sums so far
             if constexpr (S::FLUSH > 0) {
 #pragma unroll
@@ -529,10 +528,6 @@ __global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__((GemmShape<BN, PL
                     for (int e = 0; e < 32; e++) v[e] = held[m][e];
                 } else {
                     sum_of(c, v);
-                    if (!any) {
-#pragma unroll
-                        for (int e = 0; e < 32; e++) v[e] = 0.0f;
-                    }
                 }
                 epi(q, i, j, cols, v, reads ? at : nullptr, writes ? at : nullptr);
                 if constexpr (NS > 0) {
@@ -692,6 +687,7 @@ cudaError_t gemm_launch_as(const GemmMat* a, const GemmMat* b, long long ma, lon
     g.kblocks = (int)((k + GEMM_BK - 1) / GEMM_BK);
     g.splits = splits;
     g.per = (g.kblocks + splits - 1) / splits;
+    if ((splits - 1) * g.per >= g.kblocks) return cudaErrorInvalidValue;  // (the kernel waits for sums of every split)
     g.symmetric = symmetric;
     const long long tiles = symmetric ? (long long)(S::ROWS / BN) * g.ti * (g.ti + 1) / 2 : (long long)g.ti * g.tj;
     if (tiles * splits * batch >= 1 << 30) return cudaErrorInvalidValue;

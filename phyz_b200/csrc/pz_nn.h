@@ -11,13 +11,6 @@
 
 namespace pz {
 
-// A matrix in device memory: element (r, c) at p[r * rs + c * cs].
-struct NnMat {
-    void* p = nullptr;
-    long long rs = 0, cs = 0;
-    explicit operator bool() const { return p != nullptr; }
-};
-
 // linear.cu. Workspace sizes are exact for the same arguments.
 long long linear_workspace(const phyzb_linear_args& a);
 cudaError_t linear_forward(const phyzb_linear_args& a, void* ws, cudaStream_t s);
