@@ -549,6 +549,12 @@ cudaError_t forward(const phyzb_linear_args& a, char* ws, cudaStream_t st) {
 // has another order than dy), and the sums of
 // the unrounded dz over the rows: each block's part to part[block][n]. dz
 // [outer][pitch]: T, or three bf16 planes. dz or part may be null.
+//
+// A 16-bit layer's dz is rounded to its type, as the tensor cores take it: dy, which it
+// is made of, has no more bits, and a second plane would double both products. It is
+// most of what a gradient is off by beyond its own rounding (bf16 65536 x 1024 x 1024:
+// 2.3e-3 to 64 bits, 1.7e-3 with an unrounded dz; f16 2.9e-4, 2.1e-4). In f16 a dz
+// under 2^-25 is lost, which is the half of dy's own last place.
 struct DzArgs {
     const void *dy, *pre;
     long long dy_o, dy_i, pre_o, pre_i;  // strides along outer and inner
@@ -578,7 +584,7 @@ __device__ __forceinline__ void dz_store(const DzArgs& a, long long at, float v)
 
 // inner = features. V neighbours per thread, 256 threads = 32 along the features
 // x 8 rows. Bound by memory, and by the slope's instructions: 65536 x 1024 bf16
-// with gelu, 403 MB, 86 us (4.7 TB/s).
+// with gelu, 403 MB, 90 us (4.5 TB/s; tanh and silu 15 less).
 template <class T, int V>
 __global__ void __launch_bounds__(256, 4) dz_rows_kernel(const __grid_constant__ DzArgs a) {
     __shared__ float sums[8][32 * V];
@@ -643,7 +649,8 @@ __global__ void __launch_bounds__(256, 4) dz_rows_kernel(const __grid_constant__
 }
 
 // inner = rows: a block takes DZ_INNER of one feature's, V neighbours a thread. The
-// same 403 MB as above in this order: 108 us (3.7 TB/s); one value at a time 259.
+// same 403 MB as above in this order: 100 us (4.0 TB/s), 110 with the column sums; one
+// value at a time 259.
 template <class T, int V>
 __global__ void __launch_bounds__(256, 4) dz_features_kernel(const __grid_constant__ DzArgs a) {
     __shared__ float sums[8];
@@ -727,8 +734,10 @@ __global__ void __launch_bounds__(256, 4) dz_features_kernel(const __grid_consta
 // dy and pre in different orders: inner = rows, a block takes DZ_TURNED rows of 32
 // features in tiles of 32 x 64. The operand whose features are contiguous (TDY: dy,
 // else pre) is read along them and turned in shared memory; the other is read, and
-// dz written, along the rows: 1320 x 34390 f16 with gelu, 272 MB, 132 us (2.1 TB/s,
-// bound by instructions and the turn); 233 where one of the two is read against its order.
+// dz written, along the rows: 1320 x 34390 f16 with gelu, 272 MB, 100 us with the column
+// sums (2.7 TB/s, bound by instructions and the turn); 233 where one of the two was read
+// against its order. A row-major dy comes to a feature-major layer where the loss takes
+// its difference from row-major targets.
 template <class T, bool TDY>
 __global__ void __launch_bounds__(256) dz_mixed_kernel(const __grid_constant__ DzArgs a) {
     constexpr int PITCH = 64 + 4 / sizeof(T);  // a tile's column goes to 32 different banks

@@ -291,7 +291,7 @@ struct LastEpi {
 // [128 rows][l] in blocks of 64 columns, 128-byte swizzled: as it lies it is the
 // operand with k along l (X X^T) and the one with k along its rows (P X). What is
 // left of five iterations is latency: three products and epilogues of a microsecond
-// and more each. 8 matrices of 128 x 128: 42 us; as 17 launches 104.
+// and more each. 8 matrices of 128 x 128: 43 us; as 17 launches 104.
 constexpr int SMALL_THREADS = 512;
 constexpr int SMALL_BLOCK = 128 * 128;  // bytes of 128 rows of 64 values
 

@@ -47,7 +47,7 @@ struct alignas(16) Bytes16 {
 
 // V = 1: any strides. V = 16 bytes of values: channels contiguous and aligned.
 // Bound by memory and by a launch's own two microseconds: 4096 x 256 f32, 21 MB,
-// 4.6 us.
+// 5.5 us.
 template <class T, int V>
 __global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ phyzb_scan_args a) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -144,12 +144,12 @@ constexpr int NT = 128;  // threads of a block; its chains in lane_kernel: cw al
 
 // Boxes of 4 KB, two stages ahead and two behind: 24 KB a block forward, 48
 // backward (six and four blocks to an SM). Measured: 64 x 64 x 16384 f32 in the
-// history's order with resets 131 us, 6.2 TB/s or 95 % of a plain copy; backward 64 x
-// 1024 x 1024 bf16 141 us, 5.7 TB/s; 2 x 32769 x 512 bf16, cut in 108, 64 us with
+// history's order with resets 132 us, 6.2 TB/s or 94 % of a plain copy; backward 64 x
+// 1024 x 1024 bf16 138 us, 5.9 TB/s; 2 x 32769 x 512 bf16, cut in 108, 65 us with
 // its first launch's 27. Longer boxes or a third stage leave room for fewer
 // blocks: 188 us instead of 149 backward. Blocks of 64 threads: the same. Eight
 // warps to 32 chains, each with a run of the steps and a join a tile, took 32
-// instructions a value and 86 us where this takes 64.
+// instructions a value and 86 us where this takes 65.
 template <class T, bool BWD, bool OUT>
 struct Lane {
     static constexpr int S = 32 / (int)sizeof(T);  // steps of a tile

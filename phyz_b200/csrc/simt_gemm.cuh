@@ -17,7 +17,7 @@ struct SimtOperand {
 // stage is loaded into registers while the current one is multiplied. blockIdx
 // = (tiles of i, tiles of j, split of the k range), or with wide (tiles of j, of i,
 // split): a grid's second side ends at 65535. Bound by instructions: 65536 x
-// 30 x 64 with bias, tanh and pre-activations, 41 MB, 18.5 us. ALONG_I: D is contiguous in
+// 30 x 64 with bias, tanh and pre-activations, 41 MB, 20.2 us. ALONG_I: D is contiguous in
 // i; lanes then run along i, and the epilogue gets four values along it.
 // Epi: each(f) calls f(kind) once, and f void four(kind, int split, long long i, long long j, const float* v, int n,
 // bool along_i)

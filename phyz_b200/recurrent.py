@@ -57,7 +57,10 @@ class _Layer:
 
 
 class RecurrentModel:
-    """Rows in and out are [worlds, steps, features] in bfloat16; reset [worlds, steps] marks episode starts."""
+    """Rows in and out are [worlds, steps, features] in bfloat16; reset [worlds, steps] marks episode starts.
+
+    Nothing here waits for the device. `nn.status()` does, and raises if a kernel gave up a wait and left its outputs
+    unfinished: to be called where a program waits anyway, such as before it saves a checkpoint."""
 
     def __init__(self, cfg: RecurrentCfg, device: int = 0, seed: int = 0):
         self.cfg, self.device = cfg, torch.device("cuda", device)
