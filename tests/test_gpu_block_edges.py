@@ -252,9 +252,11 @@ def test_status_waits_for_every_stream():
     """What it reports is of all calls so far: work on a side stream (which does not wait for the default one, nor the
     other way round) has finished when it returns."""
     x, w = rnd(26, 512, 64, dt=torch.bfloat16), rnd(27, 64, 64, dt=torch.bfloat16)
-    nn.linear(x, w)
-    nn.status()
     side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        nn.linear(x, w)  # (so that nothing is set up or allocated below)
+    nn.status()
     torch.cuda.synchronize()
     with torch.cuda.stream(side):
         torch.cuda._sleep(200_000_000)  # a tenth of a second
